@@ -27,6 +27,7 @@
 #include <type_traits>
 
 #include "decode_common.h"
+#include "lds_tiles.h"
 
 namespace ti {
 namespace {
@@ -80,45 +81,6 @@ constexpr int kXcds = 8;              // MI355X: 8 XCDs of 32 CUs, one L2 each
 constexpr int kUnitCost = 9;
 static_assert(kMinChunkTiles > kUnitCost, "every balanced run must reach a key tile");
 
-typedef __attribute__((address_space(3))) void* lds_ptr_t;
-
-// One 1 KiB load into LDS: lane i's 16 bytes at rsrc + voff land at LDS byte lds + 16 i. Issued
-// as assembly, which the compiler's wait insertion does not see: its own waits for the loads it
-// knows stay at least as strict (vector memory operations complete in issue order, so hidden
-// loads only add to what a count waits for), and the kernel waits for these loads explicitly
-// before each stage barrier. The builtin form instead makes the compiler wait for every load
-// into a stage array before reading that array, all loads issued since included, which defeats
-// a pipeline that keeps two tiles in flight. Nor does the compiler's hazard recogniser see it: a
-// descriptor word written by v_readfirstlane or v_readlane (VALU) must be five wait states old when
-// a buffer instruction reads it, and m0 one, which the s_nop provides.
-__device__ __forceinline__ void load_lds16(u32x4 rsrc, uint32_t voff, const uint16_t* lds) {
-  const uint32_t m0 = uint32_t(reinterpret_cast<uintptr_t>((lds_ptr_t)(lds)));
-  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "{m0}"(m0)
-               : "memory");
-}
-
-// The cache row at byte offset `off` from `base`.
-__device__ __forceinline__ const uint16_t* at_bytes(const uint16_t* base, uint64_t off) {
-  return reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(base) + off);
-}
-
-// Buffer descriptor words of [base, base + bytes) (raw, no stride), uniform.
-__device__ __forceinline__ u32x4 rsrc_words(const uint16_t* base, uint32_t bytes) {
-  const uint64_t addr = reinterpret_cast<uint64_t>(base);
-  return u32x4{uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(addr)))),
-               uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(addr >> 32) & 0xffffu))),
-               uint32_t(__builtin_amdgcn_readfirstlane(int(bytes))), uint32_t(kBufferRsrcWord3)};
-}
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-
-// ds_read_b64_tr_b16 (measured on gfx950): within each 16-lane group, output lane j receives
-// element j % 4 of the 8-byte rows addressed by lanes j/4, j/4 + 4, j/4 + 8, j/4 + 12.
-__device__ __forceinline__ u32x2 lds_read_tr4(const uint16_t* p) {
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p));
-}
-
 // LDS slot of 16-byte chunk c of K/V tile row r is c ^ lds_swizzle(r). On gfx950 a ds_read_b128
 // serves 16 lanes per cycle over 64 banks: lanes {0-3, 12-15, 20-23, 24-27} together, then
 // {4-11, 16-19, 28-31}, and the same for lanes 32-63 (measured with SQ_LDS_BANK_CONFLICT). With
@@ -130,33 +92,6 @@ __device__ __forceinline__ int lds_swizzle(int r) { return (r ^ ((r << 1) & 8)) 
 // each, measured the same way); the V operand reads of one half-wave touch 8 rows, 4 lanes per 32
 // bytes of a row, so XOR-ing the chunk index with 2r puts every row's 32 bytes on distinct banks.
 __device__ __forceinline__ int lds_swizzle_v(int r) { return (2 * r) & 14; }
-
-// Maxima without the quieting of NaN operands that fmaxf's other spellings cost (v_max returns the
-// other operand for a quiet NaN, as fmaxf does).
-__device__ __forceinline__ float max2(float x, float y) {
-  float r;
-  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(x), "v"(y));
-  return r;
-}
-__device__ __forceinline__ float max3(float x, float y, float z) {
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
-  return r;
-}
-
-// Max over the four 16-lane rows of the wave (lanes n, n+16, n+32, n+48).
-__device__ __forceinline__ float row_group_max(float x) {
-  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float row_group_sum(float x) {
-  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
 
 // Query and key extent of sequence b, clamped as the entry point documents.
 struct SeqExtent {
