@@ -12,6 +12,11 @@
  *                                            engine/model_runner.py:538-637)
  *   - QK-norm + RoPE (+ append), sigmoid     (replace kernels/qknorm_rope.py, kernels/act_mul.py's
  *     gate (+ in decode's epilogue)          fused_sigmoid_mul around the path)
+ *   - latent attention (one shared vector    (no reference counterpart: a smaller cache per token)
+ *     a token): input side, absorbed decode
+ *     on the pages, expanded prefill
+ *   - attention weight of cached tokens and  (no reference counterpart: fewer cached tokens)
+ *     eviction by it
  *
  * Conventions shared by every entry point
  *   - All tensor pointers are DEVICE pointers owned by the caller. The library never allocates,
@@ -429,6 +434,124 @@ int ti_gqa_decode_paged_noalloc(const void* q, int64_t q_stride_b, int64_t q_str
 
 /* Size in bytes of the per-GPU static scratch of ti_gqa_decode_paged_noalloc. */
 int64_t ti_gqa_decode_scratch_bytes(void);
+
+/*
+ * Latent attention: every cached token is one vector [c | k_r] of latent_dim + rope_dim values that all
+ * heads share (c the normalised latent, k_r the rotated key part), in rows laid out as a cache of one KV
+ * head, [num_blocks, page_size, 1, latent_dim + rope_dim]. latent_dim 512 or 256, rope_dim 64. The
+ * reference has no latent layers; these stand beside its input side, decode and varlen prefill.
+ *
+ * Input side of a latent layer in one launch. For every token t:
+ *   q_out[t, h]     = rotate(q_rope[t, h])                                    h < num_heads (may be 0)
+ *   row[slot[t]]    = [ c / sqrt(mean c^2 + eps) * (weight_offset + weight) | rotate(key_rope[t]) ]
+ * with rotate(x)_i = x_i cos_i - x_{i+32} sin_i, rotate(x)_{i+32} = x_{i+32} cos_i + x_i sin_i, i < 32
+ * (cos, sin [n_tokens, >= 32] at cs_stride_t, 0 for one row; columns from 32 on are not read). 32-bit
+ * arithmetic, each value rounded once. Slots that are negative or >= num_slots are skipped; duplicate
+ * slots within a call are unsupported. q_out may be q_rope itself (same strides). All rows 16-byte
+ * aligned, strides multiples of 8 elements.
+ */
+int ti_latent_rope_append(const void* q_rope, int64_t q_stride_t, int64_t q_stride_h, void* q_out,
+                          int64_t out_stride_t, int64_t out_stride_h, const void* latent,
+                          int64_t latent_stride_t, const void* key_rope, int64_t key_stride_t,
+                          const void* weight, float weight_offset, const void* cos, const void* sin,
+                          int64_t cs_stride_t, void* latent_cache, int64_t cache_row_stride,
+                          int64_t num_slots, const int32_t* slot_mapping, int32_t n_tokens,
+                          int32_t num_heads, int32_t latent_dim, int32_t rope_dim, float eps,
+                          int32_t dtype, void* stream);
+
+/* Workspace of ti_latent_decode_paged for these host-known sizes (no device values). */
+int ti_latent_decode_workspace_bytes(int32_t batch, int32_t new_tokens, int32_t num_heads,
+                                     int32_t latent_dim, int64_t* workspace_bytes_out);
+
+/*
+ * Latent attention on the pages, absorbed form: for query i of a sequence's last new_tokens tokens
+ * (new_tokens = 1: a decode step; more: drafted tokens to verify, or a short chunk)
+ *   out[b, i, h] = softmax_j( scale * q[b, i, h] . row_b[j] ) @ row_b[j, 0:latent_dim],
+ *   j <= seqlen[b] - new_tokens + i
+ * where row_b[j] is the cache row of the sequence's token j and q is given in the cache's space (q_nope
+ * times the key's up-projection, then the rotated part). A query that sees nothing gives zeros. Block ids
+ * outside [0, num_blocks) below seqlen are absent (masked, never loaded); entries at or beyond
+ * ceil(seqlen / page_size) are not read. Any page_size.
+ *   q        [batch, new_tokens, num_heads, latent_dim + rope_dim], last dim contiguous, strides multiples
+ *            of 8 elements
+ *   latent_cache  contiguous rows; num_blocks * page_size < 2^31
+ *   out      [batch, new_tokens, num_heads, latent_dim] contiguous
+ *   workspace  ti_latent_decode_workspace_bytes bytes, 16-byte aligned, contents need no initialisation
+ */
+int ti_latent_decode_paged(const void* q, int64_t q_stride_b, int64_t q_stride_t, int64_t q_stride_h,
+                           const void* latent_cache, const int32_t* block_table,
+                           int64_t block_table_stride, const int32_t* seqlen, void* out,
+                           void* workspace, int64_t workspace_bytes, int32_t batch, int32_t new_tokens,
+                           int32_t num_heads, int32_t latent_dim, int32_t rope_dim, int32_t page_size,
+                           int64_t num_blocks, int32_t max_blocks_per_seq, float scale, int32_t dtype,
+                           void* stream);
+
+/*
+ * Latent attention over packed chunks, expanded form: sequence b's queries are rows
+ * [cu_seqlens_q[b], cu_seqlens_q[b+1]) of q, its keys rows [cu_seqlens_k[b], cu_seqlens_k[b+1]) of kv
+ * (the up-projected latents, [kn | v] of head_dim each) and key_rope (shared by the heads):
+ *   out[i, h] = softmax_j( scale * (q[i, h, :head_dim] . kn[j, h] + q[i, h, head_dim:] . key_rope[j]) ) @ v[j, h]
+ * with the causal mask aligned to the last key (query i sees keys j <= k_len - q_len + i), or without it.
+ * A query that sees nothing gives zeros. max_seqlen_q is at least the longest chunk; rows of longer ones
+ * are not all written. Offsets beyond total_q / total_k are cut off. head_dim 128 or 64, rope_dim 64;
+ * rows 16-byte aligned, strides multiples of 8 elements, token strides of kv and key_rope below 2^24.
+ * The role of the reference's varlen kernel (kernels/gqa_varlen.py:40-185).
+ */
+int ti_latent_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* kv,
+                      int64_t kv_stride_t, int64_t kv_stride_h, const void* key_rope,
+                      int64_t key_stride_t, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                      void* out, int64_t out_stride_t, int64_t out_stride_h, int32_t batch,
+                      int32_t total_q, int32_t total_k, int32_t max_seqlen_q, int32_t num_heads,
+                      int32_t head_dim, int32_t rope_dim, int32_t causal, float scale, int32_t dtype,
+                      void* stream);
+
+/* Workspace of ti_cache_mass for these host-known sizes. */
+int ti_cache_mass_workspace_bytes(int32_t batch, int32_t new_tokens, int32_t num_q_heads,
+                                  int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                                  int32_t max_blocks_per_seq, int64_t* workspace_bytes_out);
+
+/*
+ * Attention weight that each cached token receives from a sequence's last new_tokens queries, summed
+ * over them and over the query heads of a KV head, added to mass:
+ *   mass[b, g, t] += sum_{i, h in group g} softmax_t( scale * q[b, i, h] . K_b[t, g] ),
+ *   query i seeing t <= seqlen[b] - new_tokens + i
+ * Floats of mass at and beyond seqlen[b] are not touched. Absent blocks and queries that see nothing give
+ * no weight. No atomics: the same call gives the same bits. head_dim 128 or 256, or a latent cache's 320
+ * or 576 (one KV head).
+ *   q        [batch, new_tokens, num_q_heads, head_dim], last dim contiguous, strides multiples of 8
+ *   k_cache  [num_blocks, page_size, num_kv_heads, head_dim] contiguous
+ *   mass     [batch, num_kv_heads, >= max_blocks_per_seq * page_size] fp32 at mass_stride_b / _h
+ * No reference counterpart (the reference never drops cached tokens).
+ */
+int ti_cache_mass(const void* q, int64_t q_stride_b, int64_t q_stride_t, int64_t q_stride_h,
+                  const void* k_cache, const int32_t* block_table, int64_t block_table_stride,
+                  const int32_t* seqlen, float* mass, int64_t mass_stride_b, int64_t mass_stride_h,
+                  void* workspace, int64_t workspace_bytes, int32_t batch, int32_t new_tokens,
+                  int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                  int64_t num_blocks, int32_t max_blocks_per_seq, float scale, int32_t dtype,
+                  void* stream);
+
+/*
+ * Cut each (sequence, KV head) of a paged cache to at most `budget` tokens and copy those to the blocks of
+ * a new table. A sequence of n <= budget tokens keeps all; otherwise the first `sinks` and the last
+ * `recent` tokens stay and the rest of the budget goes to the greatest mass, ties to the lowest position
+ * (NaN counts as least, -0 as 0; sinks + recent <= budget). Kept tokens keep their order:
+ *   kept[b, g, j]      position of the j-th kept token, -1 from new_seqlen[b] on      [B, H_kv, budget]
+ *   new_seqlen[b]      min(seqlen[b], budget)
+ *   mass_out[b, g, j]  its mass, 0 from new_seqlen[b] on                     [B, H_kv, mass_capacity]
+ *   slot j of new_block_table[b] = the cache row of token kept[b, g, j]  (K, and V unless v_cache is NULL)
+ * The new table's blocks must not be among those that any table still in use (this call's among them)
+ * holds; block ids outside [0, num_blocks) are skipped. head_dim a multiple of 8; mass_capacity >=
+ * max_blocks_per_seq * page_size, the new table holds min(budget, that) tokens. mass_out is not mass.
+ * No reference counterpart.
+ */
+int ti_evict_kvcache(void* k_cache, void* v_cache, const float* mass, int64_t mass_stride_b,
+                     int64_t mass_stride_h, int64_t mass_capacity, const int32_t* block_table,
+                     int64_t block_table_stride, const int32_t* seqlen, const int32_t* new_block_table,
+                     int64_t new_table_stride, int32_t* kept, int32_t* new_seqlen, float* mass_out,
+                     int32_t batch, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                     int64_t num_blocks, int32_t max_blocks_per_seq, int32_t new_blocks_per_seq,
+                     int32_t budget, int32_t sinks, int32_t recent, int32_t dtype, void* stream);
 
 /* Text of the last error reported on the calling thread ("" when none). */
 const char* ti_last_error(void);

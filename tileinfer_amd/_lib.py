@@ -7,6 +7,7 @@ here). There is no fallback: a missing library raises. (_pycalls.so beside it on
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import importlib.machinery
 import importlib.util
@@ -32,7 +33,7 @@ TI_DECODE_MFMA = 1
 TI_DECODE_SCALAR = 2
 TI_DECODE_REUSE_KV = 0x10
 TI_DECODE_STREAM_KV = 0x20
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 # Every symbol declared in include/tileinfer_amd.h, with its ctypes signature.
 _c_i32, _c_i64, _c_vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
@@ -97,6 +98,29 @@ SIGNATURES = {
                                                    _c_i32, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32,
                                                    _c_i32, _c_vp]),
     "ti_gqa_decode_scratch_bytes": (ctypes.c_int64, []),
+    "ti_latent_rope_append": (ctypes.c_int, [_c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp,
+                                             _c_i64, _c_vp, _c_i64, _c_vp, ctypes.c_float, _c_vp,
+                                             _c_vp, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp, _c_i32,
+                                             _c_i32, _c_i32, _c_i32, ctypes.c_float, _c_i32, _c_vp]),
+    "ti_latent_decode_workspace_bytes": (ctypes.c_int, [_c_i32, _c_i32, _c_i32, _c_i32, _I64P]),
+    "ti_latent_decode_paged": (ctypes.c_int, [_c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_i64,
+                                              _c_vp, _c_vp, _c_vp, _c_i64, _c_i32, _c_i32, _c_i32,
+                                              _c_i32, _c_i32, _c_i32, _c_i64, _c_i32,
+                                              ctypes.c_float, _c_i32, _c_vp]),
+    "ti_latent_prefill": (ctypes.c_int, [_c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp, _c_i64,
+                                         _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32,
+                                         _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, ctypes.c_float,
+                                         _c_i32, _c_vp]),
+    "ti_cache_mass_workspace_bytes": (ctypes.c_int, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,
+                                                     _c_i32, _I64P]),
+    "ti_cache_mass": (ctypes.c_int, [_c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_i64, _c_vp,
+                                     _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i32, _c_i32, _c_i32,
+                                     _c_i32, _c_i32, _c_i32, _c_i64, _c_i32, ctypes.c_float, _c_i32,
+                                     _c_vp]),
+    "ti_evict_kvcache": (ctypes.c_int, [_c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64,
+                                        _c_vp, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_i32, _c_i32,
+                                        _c_i32, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32,
+                                        _c_i32, _c_i32, _c_vp]),
     "ti_last_error": (ctypes.c_char_p, []),
     "ti_abi_version": (ctypes.c_int32, []),
 }
@@ -223,3 +247,10 @@ def stream_handle(device: torch.device) -> int:
         index = device.index if device.index is not None else torch.cuda.current_device()
         return _raw_stream(index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def on(device: torch.device):
+    """Context in which ``device`` is the current one: library calls launch there."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)

@@ -1,0 +1,449 @@
+// Attention weight that each cached token receives from a sequence's last queries (gfx950): for sequence b
+// and KV head g, over the rows r = (query i of the last `new`, head of the group),
+//   mass[b, g, t] += sum_r softmax_t( scale * q_r . K[t] ),  query i seeing t <= seqlen - new + i,
+// the running sums by which a cache is cut to its heaviest tokens (cache_evict.hip). Everything past the
+// products of 16-bit values is 32 bits; a token's sum is made by one lane in a fixed order, so calls repeat
+// bit for bit.
+//
+// A wave takes 16 TT tokens of one KV head, whose K rows it reads from the pages into registers as MFMA
+// operands (lane l: row l % 16, 8 values of k-group l / 16), and multiplies them with 16 rows of queries at
+// a time, S^T[16 tokens x 16 rows] as in the paged decode.
+//   Up to 16 rows (a decode step): the scores are kept, 4 bytes a row and token against 2 D of the K row,
+//     beside each workgroup's (max, sum) of every row; a second kernel joins those and adds the weights.
+//     K is read once.
+//   More rows (a window of queries): scores would outweigh K, so they are computed twice: once for the
+//     (max, sum) of every wave and row, joined by a small kernel, and once for the weights.
+#include "lds_tiles.h"
+
+namespace ti {
+namespace {
+
+struct MassArgs {
+  const uint16_t* q;
+  int64_t q_sb, q_st, q_sh;  // q [B, new, Hq, D] strides (elements)
+  const uint16_t* k_cache;   // rows [num_blocks * page_size][hkv][D]
+  const int32_t* block_table;
+  int64_t bt_stride;
+  const int32_t* seqlen;
+  float* mass;  // [B, hkv, >= max_blocks * page_size]
+  int64_t m_sb, m_sh;
+  float* scores;  // [B, hkv, rows][tokens]  (up to 16 rows)
+  float* part;    // [B, hkv][parts][rows][2]  (max, sum) of a part, max in exp2 units
+  float* stats;   // [B, hkv][rows][2]  (max, 1 / sum)  (more than 16 rows)
+  int32_t new_tokens, hkv, group, rows, num_blocks32, page_size, max_blocks;
+  int32_t parts;   // parts of a sequence of the greatest length
+  int64_t tokens;  // that length, a multiple of 4
+  float scale_log2;
+};
+
+constexpr int kFewRows = 16;
+
+__device__ __forceinline__ int mass_len(const MassArgs& a, int b) {
+  const int64_t cap = int64_t(a.max_blocks) * a.page_size;
+  const int n = max(a.seqlen[b], 0);
+  return int64_t(n) > cap ? int(cap) : n;
+}
+
+// The K operands of tokens t0 + 16 tt + (0 .. 15), as lane (n, g) holds them, and whether this lane's
+// accumulator tokens (4 g + e of each tile) exist.
+template <int D, int TT>
+struct KeyTile {
+  u32x4 k[TT][D / 32];
+  uint32_t there[TT];  // bit j: token 16 tt + j is in the sequence and its block in the cache
+};
+
+template <int D, int TT>
+__device__ __forceinline__ void load_keys(const MassArgs& a, int b, int h, int len, int t0, KeyTile<D, TT>& x) {
+  const int lane = threadIdx.x & 63;
+  const int n = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt) {
+    const int t = t0 + 16 * tt + n;
+    int id = -1, in_page = 0;
+    if (t < len) {
+      const int page = t / a.page_size;
+      in_page = t - page * a.page_size;
+      id = a.block_table[b * a.bt_stride + page];
+    }
+    const bool ok = uint32_t(id) < uint32_t(a.num_blocks32);
+    x.there[tt] = uint32_t(__builtin_amdgcn_ballot_w64(ok)) & 0xffffu;
+    const uint16_t* src = a.k_cache + ((int64_t(ok ? id : 0) * a.page_size + in_page) * a.hkv + h) * D + 8 * g;
+#pragma unroll
+    for (int kk = 0; kk < D / 32; ++kk) x.k[tt][kk] = ok ? load16(src + 32 * kk) : u32x4{};
+  }
+}
+
+// Scores, in exp2 units, of the tile's tokens (4 g + e of each 16) and row r0 + n; -inf where the row does
+// not see the token. Rows behind the last are all -inf.
+template <int D, int TT, typename Tag>
+__device__ __forceinline__ void score_rows(const MassArgs& a, int b, int h, int len, int t0, int r0,
+                                           const KeyTile<D, TT>& x, float (&s)[TT][4]) {
+  const int lane = threadIdx.x & 63;
+  const int n = lane & 15, g = lane >> 4;
+  const int r = min(r0 + n, a.rows - 1);
+  const int tok = r / a.group, head = h * a.group + (r - tok * a.group);
+  const uint16_t* src = a.q + b * a.q_sb + tok * a.q_st + head * a.q_sh + 8 * g;
+  u32x4 q[D / 32];
+#pragma unroll
+  for (int kk = 0; kk < D / 32; ++kk) q[kk] = load16(src + 32 * kk);
+  f32x4 acc[TT];
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt) acc[tt] = f32x4{};
+#pragma unroll
+  for (int kk = 0; kk < D / 32; ++kk) {
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) acc[tt] = mfma16x16x32(x.k[tt][kk], q[kk], acc[tt], Tag{});
+  }
+  const int last = r0 + n < a.rows ? len - a.new_tokens + tok : -1;
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int j = 4 * g + e;
+      const bool seen = ((x.there[tt] >> j) & 1) && t0 + 16 * tt + j <= last;
+      s[tt][e] = seen ? acc[tt][e] * a.scale_log2 : -INFINITY;
+    }
+  }
+}
+
+// (max, sum) of each row over the wave's tokens.
+template <int TT>
+__device__ __forceinline__ void row_stats(const float (&s)[TT][4], float& m, float& l) {
+  m = -INFINITY;
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = max2(m, s[tt][e]);
+  }
+  m = row_group_max(m);
+  const float base = m == -INFINITY ? 0.f : m;
+  l = 0.f;
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) l += fast_exp2(s[tt][e] - base);
+  }
+  l = row_group_sum(l);
+}
+
+// Up to 16 rows: scores of 64 TT tokens a workgroup, and its (max, sum) of every row.
+template <int D, int TT, typename Tag>
+__global__ __launch_bounds__(256) void mass_scores_kernel(MassArgs a) {
+  __shared__ float s_ml[4][16][2];
+  const int b = blockIdx.z, h = blockIdx.y;
+  const int len = mass_len(a, b);
+  const int wg0 = int(blockIdx.x) * 64 * TT;
+  if (wg0 >= len) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n = lane & 15, g = lane >> 4;
+  const int t0 = wg0 + wave * 16 * TT;
+  KeyTile<D, TT> x;
+  load_keys<D, TT>(a, b, h, len, t0, x);
+  float s[TT][4], m, l;
+  score_rows<D, TT, Tag>(a, b, h, len, t0, 0, x, s);
+  if (n < a.rows) {
+    float* dst = a.scores + ((int64_t(b) * a.hkv + h) * a.rows + n) * a.tokens + t0 + 4 * g;
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+      if (t0 + 16 * tt + 4 * g < len) {
+        *reinterpret_cast<f32x4*>(dst + 16 * tt) = f32x4{s[tt][0], s[tt][1], s[tt][2], s[tt][3]};
+      }
+    }
+  }
+  row_stats<TT>(s, m, l);
+  if (g == 0) {
+    s_ml[wave][n][0] = m;
+    s_ml[wave][n][1] = l;
+  }
+  __syncthreads();
+  if (threadIdx.x < unsigned(a.rows)) {
+    float top = -INFINITY, sum = 0.f;
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, s_ml[w][threadIdx.x][0]);
+    const float base = top == -INFINITY ? 0.f : top;
+    for (int w = 0; w < 4; ++w) sum += s_ml[w][threadIdx.x][1] * fast_exp2(s_ml[w][threadIdx.x][0] - base);
+    float* dst = a.part + (((int64_t(b) * a.hkv + h) * a.parts + blockIdx.x) * a.rows + threadIdx.x) * 2;
+    dst[0] = top;
+    dst[1] = sum;
+  }
+}
+
+// (max, 1 / sum) of a row from its parts; 16 lanes of consecutive threads join one row.
+__device__ __forceinline__ void join_parts(const float* part, int parts, int64_t stride, int lane16, float& m,
+                                           float& inv) {
+  m = -INFINITY;
+  float l = 0.f;
+  for (int p = lane16; p < parts; p += 16) {
+    const float pm = part[p * stride], pl = part[p * stride + 1];
+    const float mn = fmaxf(m, pm);
+    const float base = mn == -INFINITY ? 0.f : mn;
+    l = l * fast_exp2(m - base) + pl * fast_exp2(pm - base);
+    m = mn;
+  }
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) {
+    const float om = __shfl_xor(m, d, 64), ol = __shfl_xor(l, d, 64);
+    const float mn = fmaxf(m, om);
+    const float base = mn == -INFINITY ? 0.f : mn;
+    l = l * fast_exp2(m - base) + ol * fast_exp2(om - base);
+    m = mn;
+  }
+  inv = l != 0.f ? 1.f / l : 0.f;  // a row that sees nothing gives nothing
+}
+
+constexpr int kAddTokens = 1024;  // tokens of a workgroup of mass_add_kernel
+
+// The weights of up to 16 rows from their scores, added to the sums.
+__global__ __launch_bounds__(256) void mass_add_kernel(MassArgs a, int part_tokens) {
+  __shared__ float s_stat[kFewRows][2];
+  const int b = blockIdx.z, h = blockIdx.y;
+  const int len = mass_len(a, b);
+  const int wg0 = int(blockIdx.x) * kAddTokens;
+  if (wg0 >= len) return;
+  const int64_t bh = int64_t(b) * a.hkv + h;
+  const int parts = (len + part_tokens - 1) / part_tokens;
+  const int row = threadIdx.x >> 4;
+  if (row < a.rows) {
+    float m, inv;
+    join_parts(a.part + (bh * a.parts * a.rows + row) * 2, parts, 2 * int64_t(a.rows), threadIdx.x & 15, m, inv);
+    if ((threadIdx.x & 15) == 0) {
+      s_stat[row][0] = m == -INFINITY ? 0.f : m;
+      s_stat[row][1] = inv;
+    }
+  }
+  __syncthreads();
+  const int t = wg0 + 4 * int(threadIdx.x);
+  if (t >= len) return;
+  const float* src = a.scores + bh * a.rows * a.tokens + t;
+  float w[4] = {};
+  for (int r = 0; r < a.rows; ++r) {
+    const f32x4 s = *reinterpret_cast<const f32x4*>(src + r * a.tokens);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] += fast_exp2(s[e] - s_stat[r][0]) * s_stat[r][1];
+  }
+  float* dst = a.mass + b * a.m_sb + h * a.m_sh + t;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (t + e < len) dst[e] += w[e];
+  }
+}
+
+// More than 16 rows, first pass: (max, sum) of every wave and row.
+template <int D, int TT, typename Tag>
+__global__ __launch_bounds__(256) void mass_stats_kernel(MassArgs a) {
+  const int b = blockIdx.z, h = blockIdx.y;
+  const int len = mass_len(a, b);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int part = int(blockIdx.x) * 4 + wave;
+  const int t0 = part * 16 * TT;
+  if (t0 >= len) return;
+  KeyTile<D, TT> x;
+  load_keys<D, TT>(a, b, h, len, t0, x);
+  float* dst = a.part + ((int64_t(b) * a.hkv + h) * a.parts + part) * a.rows * 2;
+  for (int r0 = 0; r0 < a.rows; r0 += 16) {
+    float s[TT][4], m, l;
+    score_rows<D, TT, Tag>(a, b, h, len, t0, r0, x, s);
+    row_stats<TT>(s, m, l);
+    const int r = r0 + (lane & 15);
+    if (lane < 16 && r < a.rows) {
+      dst[2 * r] = m;
+      dst[2 * r + 1] = l;
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void mass_join_kernel(MassArgs a, int part_tokens) {
+  const int b = blockIdx.z, h = blockIdx.y;
+  const int parts = (mass_len(a, b) + part_tokens - 1) / part_tokens;
+  const int row = int(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  if (row >= a.rows) return;
+  const int64_t bh = int64_t(b) * a.hkv + h;
+  float m, inv;
+  join_parts(a.part + (bh * a.parts * a.rows + row) * 2, parts, 2 * int64_t(a.rows), threadIdx.x & 15, m, inv);
+  if ((threadIdx.x & 15) == 0) {
+    float* dst = a.stats + (bh * a.rows + row) * 2;
+    dst[0] = m == -INFINITY ? 0.f : m;
+    dst[1] = inv;
+  }
+}
+
+// Second pass: the weights, added to the sums.
+template <int D, int TT, typename Tag>
+__global__ __launch_bounds__(256) void mass_weights_kernel(MassArgs a) {
+  const int b = blockIdx.z, h = blockIdx.y;
+  const int len = mass_len(a, b);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n = lane & 15, g = lane >> 4;
+  const int t0 = (int(blockIdx.x) * 4 + wave) * 16 * TT;
+  if (t0 >= len) return;
+  KeyTile<D, TT> x;
+  load_keys<D, TT>(a, b, h, len, t0, x);
+  const float* stats = a.stats + (int64_t(b) * a.hkv + h) * a.rows * 2;
+  float w[TT][4] = {};
+  for (int r0 = 0; r0 < a.rows; r0 += 16) {
+    float s[TT][4];
+    score_rows<D, TT, Tag>(a, b, h, len, t0, r0, x, s);
+    const int r = min(r0 + n, a.rows - 1);
+    const float m = stats[2 * r], inv = stats[2 * r + 1];
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[tt][e] += fast_exp2(s[tt][e] - m) * inv;
+    }
+  }
+  float* dst = a.mass + b * a.m_sb + h * a.m_sh;
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float y = w[tt][e];
+#pragma unroll
+      for (int d = 1; d < 16; d <<= 1) y += __shfl_xor(y, d, 64);
+      const int t = t0 + 16 * tt + 4 * g + e;
+      if (n == 0 && t < len) dst[t] += y;
+    }
+  }
+}
+
+// 16-token tiles of a wave: what its K rows leave of the registers.
+constexpr int tiles_of(int d) { return d <= 128 ? 4 : 2; }
+
+struct MassSizes {
+  int32_t part_tokens, parts;
+  int64_t tokens, scores, part, stats, bytes;  // floats, bytes
+};
+
+MassSizes mass_sizes(int32_t batch, int32_t hkv, int32_t rows, int32_t d, int64_t tokens) {
+  MassSizes s;
+  const bool few = rows <= kFewRows;
+  s.part_tokens = 16 * tiles_of(d) * (few ? 4 : 1);
+  s.parts = int32_t(ceil_div(tokens, s.part_tokens));
+  s.tokens = ceil_div(tokens, 4) * 4;
+  const int64_t bh = int64_t(batch) * hkv;
+  s.scores = few ? bh * rows * s.tokens : 0;
+  s.part = bh * s.parts * rows * 2;
+  s.stats = few ? 0 : bh * rows * 2;
+  s.bytes = ((s.scores + s.part + s.stats) * 4 + 15) & ~int64_t(15);
+  return s;
+}
+
+int check_mass(const char* who, int32_t batch, int32_t new_tokens, int32_t hq, int32_t hkv, int32_t d,
+               int32_t page_size, int32_t max_blocks) {
+  if (d != 128 && d != 256 && d != 320 && d != 576) {
+    return fail(TI_EUNSUPPORTED, "%s: head_dim %d not built (128, 256, 320, 576)", who, d);
+  }
+  if (batch < 0 || batch > 65535 || new_tokens <= 0 || hq <= 0 || hkv <= 0 || hkv > 65535 || hq % hkv != 0 ||
+      int64_t(new_tokens) * (hq / hkv) > (1 << 20)) {
+    return fail(TI_EINVAL, "%s: bad sizes batch=%d new_tokens=%d heads=%d/%d", who, batch, new_tokens, hq, hkv);
+  }
+  if (page_size <= 0 || max_blocks < 0 || int64_t(max_blocks) * page_size > INT32_MAX - 1024) {
+    return fail(TI_EINVAL, "%s: bad cache page_size=%d max_blocks_per_seq=%d", who, page_size, max_blocks);
+  }
+  return TI_OK;
+}
+
+template <int D, typename Tag>
+void launch_mass(const MassArgs& a, const MassSizes& sz, unsigned batch, hipStream_t s) {
+  constexpr int TT = tiles_of(D);
+  const unsigned hkv = unsigned(a.hkv);
+  const dim3 grid(unsigned(ceil_div(a.tokens, 64 * TT)), hkv, batch);
+  if (a.rows <= kFewRows) {
+    hipLaunchKernelGGL((mass_scores_kernel<D, TT, Tag>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL(mass_add_kernel, dim3(unsigned(ceil_div(a.tokens, kAddTokens)), hkv, batch), dim3(256), 0,
+                       s, a, sz.part_tokens);
+    return;
+  }
+  hipLaunchKernelGGL((mass_stats_kernel<D, TT, Tag>), grid, dim3(256), 0, s, a);
+  hipLaunchKernelGGL(mass_join_kernel, dim3(unsigned(ceil_div(a.rows, 16)), hkv, batch), dim3(256), 0, s, a,
+                     sz.part_tokens);
+  hipLaunchKernelGGL((mass_weights_kernel<D, TT, Tag>), grid, dim3(256), 0, s, a);
+}
+
+template <typename Tag>
+void launch_mass_dim(const MassArgs& a, const MassSizes& sz, int d, unsigned batch, hipStream_t s) {
+  if (d == 128) launch_mass<128, Tag>(a, sz, batch, s);
+  else if (d == 256) launch_mass<256, Tag>(a, sz, batch, s);
+  else if (d == 320) launch_mass<320, Tag>(a, sz, batch, s);
+  else launch_mass<576, Tag>(a, sz, batch, s);
+}
+
+}  // namespace
+}  // namespace ti
+
+extern "C" int ti_cache_mass_workspace_bytes(int32_t batch, int32_t new_tokens, int32_t num_q_heads,
+                                             int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                                             int32_t max_blocks_per_seq, int64_t* workspace_bytes_out) {
+  using namespace ti;
+  const char* who = "ti_cache_mass_workspace_bytes";
+  int rc = check_mass(who, batch, new_tokens, num_q_heads, num_kv_heads, head_dim, page_size, max_blocks_per_seq);
+  if (rc != TI_OK) return rc;
+  if (!workspace_bytes_out) return fail(TI_EINVAL, "%s: null output", who);
+  *workspace_bytes_out = mass_sizes(batch, num_kv_heads, new_tokens * (num_q_heads / num_kv_heads), head_dim,
+                                    int64_t(max_blocks_per_seq) * page_size).bytes;
+  return TI_OK;
+}
+
+extern "C" int ti_cache_mass(const void* q, int64_t q_stride_b, int64_t q_stride_t, int64_t q_stride_h,
+                             const void* k_cache, const int32_t* block_table, int64_t block_table_stride,
+                             const int32_t* seqlen, float* mass, int64_t mass_stride_b, int64_t mass_stride_h,
+                             void* workspace, int64_t workspace_bytes, int32_t batch, int32_t new_tokens,
+                             int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                             int64_t num_blocks, int32_t max_blocks_per_seq, float scale, int32_t dtype,
+                             void* stream) {
+  using namespace ti;
+  const char* who = "ti_cache_mass";
+  if (dtype != TI_DTYPE_BF16 && dtype != TI_DTYPE_F16) {
+    return fail(TI_EUNSUPPORTED, "%s: dtype code %d is not bf16/fp16", who, dtype);
+  }
+  int rc = check_mass(who, batch, new_tokens, num_q_heads, num_kv_heads, head_dim, page_size, max_blocks_per_seq);
+  if (rc != TI_OK) return rc;
+  if (num_blocks < 0 || num_blocks > INT32_MAX) {
+    return fail(TI_EINVAL, "%s: bad cache num_blocks=%lld", who, static_cast<long long>(num_blocks));
+  }
+  const int64_t tokens = int64_t(max_blocks_per_seq) * page_size;
+  if (mass_stride_h < tokens || mass_stride_b < 0) {
+    return fail(TI_EINVAL, "%s: mass rows of %lld floats for sequences of up to %lld tokens", who,
+                static_cast<long long>(mass_stride_h), static_cast<long long>(tokens));
+  }
+  if (batch == 0 || tokens == 0) return TI_OK;
+  const int32_t rows = new_tokens * (num_q_heads / num_kv_heads);
+  const MassSizes sz = mass_sizes(batch, num_kv_heads, rows, head_dim, tokens);
+  if (!q || !k_cache || !block_table || !seqlen || !mass || !workspace) return fail(TI_EINVAL, "%s: null pointer", who);
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) |
+        reinterpret_cast<uintptr_t>(workspace)) & 15) != 0 ||
+      q_stride_b % 8 != 0 || q_stride_t % 8 != 0 || q_stride_h % 8 != 0) {
+    return fail(TI_EINVAL, "%s: q, cache and workspace must be 16-byte aligned, q strides multiples of 8", who);
+  }
+  if (workspace_bytes < sz.bytes) {
+    return fail(TI_EINVAL, "%s: workspace %lld < %lld bytes", who, static_cast<long long>(workspace_bytes),
+                static_cast<long long>(sz.bytes));
+  }
+  MassArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_sb = q_stride_b;
+  a.q_st = q_stride_t;
+  a.q_sh = q_stride_h;
+  a.k_cache = static_cast<const uint16_t*>(k_cache);
+  a.block_table = block_table;
+  a.bt_stride = block_table_stride;
+  a.seqlen = seqlen;
+  a.mass = mass;
+  a.m_sb = mass_stride_b;
+  a.m_sh = mass_stride_h;
+  a.scores = static_cast<float*>(workspace);
+  a.part = a.scores + sz.scores;
+  a.stats = a.part + sz.part;
+  a.new_tokens = new_tokens;
+  a.hkv = num_kv_heads;
+  a.group = num_q_heads / num_kv_heads;
+  a.rows = rows;
+  a.num_blocks32 = int32_t(num_blocks);
+  a.page_size = page_size;
+  a.max_blocks = max_blocks_per_seq;
+  a.parts = sz.parts;
+  a.tokens = sz.tokens;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == TI_DTYPE_BF16) launch_mass_dim<Bf16>(a, sz, head_dim, unsigned(batch), s);
+  else launch_mass_dim<F16>(a, sz, head_dim, unsigned(batch), s);
+  return check_launch(who);
+}
