@@ -316,3 +316,28 @@ def test_a_latent_layer_end_to_end(dev):
         absorbed = torch.einsum("thl,hld->thd", o.float(), wv)
         # Both round kv or q and o to 16 bits (2^-8 each of terms of about one) and P twice.
         torch.testing.assert_close(expanded.float(), absorbed, atol=6 * 2.0 ** -8, rtol=2.0 ** -6)
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_decode_of_many_tiles_streams_or_keeps_shared_pages(shared, dev):
+    """Enough tiles for the streaming loads, with private pages and with a prefix that half of the batch shares:
+    the same values through either table."""
+    say(f"latent decode many tiles shared={shared}")
+    g = torch.Generator(device=dev).manual_seed(51)
+    page, b, width = 16, 40, 130
+    lens = torch.randint(1500, width * page + 1, (b,), generator=g, device=dev, dtype=torch.int32)
+    pool = torch.randn(b * width, page, 1, 576, generator=g, device=dev).to(BF16)
+    table = torch.randperm(b * width, generator=g, device=dev).to(torch.int32).view(b, width)
+    if shared:
+        for i in range(1, b // 2):
+            pool[table[i, :50].long()] = pool[table[0, :50].long()]
+    q = torch.randn(b, 24, 576, generator=g, device=dev).to(BF16)
+    out = latent_decode_paged_fn(q, pool, table, lens, page, scale=SCALE)
+    if shared:
+        one = table.clone()
+        one[1:b // 2, :50] = table[0, :50]
+        assert torch.equal(bits(latent_decode_paged_fn(q, pool, one, lens, page, scale=SCALE)), bits(out))
+    for i in (0, b // 2, b - 1):
+        exact, limit = ref.latent_decode(q[i:i + 1, None].cpu(), pool.cpu(), table[i:i + 1].cpu(), lens[i:i + 1].cpu(),
+                                         page, SCALE)
+        _within(out[i:i + 1, None], exact, limit, f"sequence {i}")

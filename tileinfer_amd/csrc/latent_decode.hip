@@ -7,28 +7,33 @@
 // tokens before position seqlen - new_tokens + i + 1. The caller multiplies o by the value's
 // up-projection.
 //
-// Work: the rows of a sequence are its (query, head) pairs. A workgroup's four waves hold RB rows of one
-// sequence and walk its tokens in tiles of 32, which are staged in LDS once and read twice, as K and as
-// V. Waves are RG row groups times DS column groups: a wave computes the scores of its group's rows
-// (every column group the same ones, so neither scores nor softmax statistics cross waves) and its
-// L / DS columns of the output:
-//   S^T[32 tokens x 16 rows] = K[32 x E] . Q^T[E x 16]     (16x16x32, E/32 steps, Q in registers)
-//   O^T[16 d x 16 rows]     += V^T[16 d x 32] . P^T[32 x 16]
-// in which an accumulator's row is its lane's column and the softmax stays in the lane, as in the paged
-// prefill; P goes to the second product as the first one left it (the order of a tile's tokens is the
-// same in P and in the transposed reads of V).
+// Work: the rows of a sequence are its (query, head) pairs. A workgroup of eight waves holds RB = 16 RG rows
+// of one sequence and walks its tokens in tiles of 32, staged in LDS once and read twice, as K and as V:
+//   S^T[16 tokens x 16 rows] = K[16 x E] . Q^T[E x 16]     (16x16x32) cut over the waves by tokens, rows and
+//                              k (KS parts of E), Q in registers; the parts go through LDS
+//   O^T[16 d x 16 rows]     += V^T[16 d x 32] . P^T[32 x 16]   every wave its 16 rows and L RG / 8 columns
+// in which an accumulator's row is its lane's column. The waves of a row group add the parts of S up in the
+// same order and keep the same statistics, so the softmax stays in the lane, as in the paged prefill; P
+// goes to the second product as S^T lies (the order of a tile's tokens is the same in P and in the
+// transposed reads of V). No product is computed twice, so that the waves' LDS reads (178 KB a tile) take a
+// third of the time in which the tile's 36 KB come from HBM, and a tile is held for about as long.
 //
 // The batch's tiles (row blocks times sequences times tiles) are one list, cut into runs of equal length,
 // one for each workgroup; a unit (sequence, row block) that lies in one run is written by it, others
 // leave (m, l, o) parts in 32 bits that a second kernel joins in the order of the runs.
+#include <type_traits>
+
 #include "lds_tiles.h"
 
 namespace ti {
 namespace {
 
 constexpr int kTile = 32;       // tokens of a tile
+constexpr int kWaves = 8;
+constexpr int kStages = 4;      // latents of tiles in LDS: two in use, two on their way
+constexpr int kRopeStages = 3;  // rotated parts: one in use, two on their way
 constexpr int kRope = 64;       // rotated dimensions beside the latent
-constexpr int kIdSlots = 1024;  // block ids staged at a time
+constexpr int kIdSlots = 512;   // block ids staged at a time
 constexpr float kSlack = 8.f;   // exp2 units a row maximum may rise before O is rescaled
 
 struct LatentArgs {
@@ -43,7 +48,7 @@ struct LatentArgs {
   float* part_ml;  // [runs][2][RB][2] their (m, l), m in exp2 units
   int32_t* first_tile;  // [B + 1] each sequence's first tile, and the total
   int32_t batch, new_tokens, heads, rows, row_blocks, num_blocks32, page_size, page_shift, max_blocks;
-  int32_t runs, min_tiles;
+  int32_t runs;
   float scale_log2;
 };
 
@@ -55,13 +60,30 @@ __device__ __forceinline__ int latent_len(const LatentArgs& a, int b) {
   return int64_t(n) > cap ? int(cap) : n;
 }
 
-// Runs in use and the run that holds position u of the list (runs are [floor(i T / R), floor((i + 1) T / R))).
-__device__ __forceinline__ int64_t runs_of(const LatentArgs& a, int64_t total) {
-  return max(int64_t(1), min(int64_t(a.runs), total / a.min_tiles));
-}
-__device__ __forceinline__ int64_t run_at(int64_t u, int64_t total, int64_t runs) {
-  return ((u + 1) * runs - 1) / total;
-}
+// Lists of at least this many tiles (75 MB at L = 512) load their rows with the streaming policy: 64 sequences of
+// 16,384 tokens 203 us against 224, 64 of 100 to 4,000 in turn with others 58.1 against 61.9; shorter ones,
+// which the last-level cache may still hold, keep the default one (one of 32,000: 29.6 us against 31.7).
+constexpr uint32_t kStreamTiles = 2048;
+
+// Shortest run of tiles: two, or one where the list is so short that its first tiles' latency is all there is
+// (one sequence of 700 tokens, 24 heads: 14.3 us against 16.1 with two; four of 1,000: 16.4 against 15.6).
+constexpr uint32_t kShortTiles = 48;
+
+// The list of `total` tiles cut into runs, the first `rest` of them one tile longer. All in 32 bits (the host
+// refuses longer lists): a 64-bit division takes about half a microsecond at the start of every workgroup.
+struct Runs {
+  uint32_t runs, base, rest;
+  __device__ __forceinline__ Runs(const LatentArgs& a, uint32_t total) {
+    runs = max(1u, min(uint32_t(a.runs), total / (total <= kShortTiles ? 1u : 2u)));
+    base = total / runs;
+    rest = total - base * runs;
+  }
+  __device__ __forceinline__ uint32_t start(uint32_t i) const { return i * base + min(i, rest); }
+  __device__ __forceinline__ uint32_t holding(uint32_t u) const {  // the run of position u
+    const uint32_t longer = rest * (base + 1);
+    return u < longer ? u / (base + 1) : rest + (u - longer) / base;
+  }
+};
 
 __device__ __forceinline__ int wave_scan(int x, int lane) {
 #pragma unroll
@@ -72,15 +94,32 @@ __device__ __forceinline__ int wave_scan(int x, int lane) {
   return x;
 }
 
-// One load of 16 bytes a lane into LDS: lane i's land at byte lds + 16 i.
-__device__ __forceinline__ void load_lds16_at(const uint16_t* src, const uint16_t* lds) {
-  const uint32_t m0 = uint32_t(__builtin_amdgcn_readfirstlane(int(reinterpret_cast<uintptr_t>((lds_ptr_t)(lds)))));
-  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(m0) : "memory");
+// One load of 16 bytes a lane into LDS, from base + off of each lane: lane i's land at byte lds + 16 i.
+// STREAM: with the nt bit, for bytes that are read once.
+template <bool STREAM>
+__device__ __forceinline__ void load_lds16_from(uint64_t base, uint32_t off, const uint16_t* lds) {
+  const uint32_t m0 = uint32_t(reinterpret_cast<uintptr_t>((lds_ptr_t)(lds)));
+  if constexpr (STREAM) {
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(base), "{m0}"(m0) : "memory");
+  } else {
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(m0) : "memory");
+  }
+}
+template <bool STREAM>
+__device__ __forceinline__ void load_lds16_at(uint64_t src, const uint16_t* lds) {
+  const uint32_t m0 = uint32_t(reinterpret_cast<uintptr_t>((lds_ptr_t)(lds)));
+  if constexpr (STREAM) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(src), "{m0}"(m0) : "memory");
+  } else {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(m0) : "memory");
+  }
 }
 
-// LDS place of 16-byte chunk c of a tile's row r is c ^ swz8(r) (rows of L + 64 values start 32 banks
-// apart). A ds_read_b128 serves rows {0-3, 12-15} of one chunk with rows {4-11} of its neighbour, a
-// transposed read two neighbouring chunks of eight rows: both hit every bank quad once.
+// LDS places of 16-byte chunk c of a tile's row r: c ^ swz16(r) in the latents' rows (whole 256-byte
+// blocks), c ^ swz8(r) in the 128-byte rows of the rotated parts. A ds_read_b128 serves rows {0-3, 12-15}
+// of one chunk with rows {4-11} of its neighbour, a transposed read two neighbouring chunks of eight
+// rows; either way these are 16 different bank quads.
+__device__ __forceinline__ int swz16(int r) { return ((2 * r) & 15) ^ ((r & 8) ? 9 : 0); }
 __device__ __forceinline__ int swz8(int r) {
   const int u = (r >> 1) & 7;
   return ((2 * u) & 7) ^ ((u & 4) ? 5 : 0);
@@ -91,306 +130,419 @@ __device__ __forceinline__ void wait_loads_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// L: latent size. RT: 16-row tiles of a wave. RG: row groups, DS: column groups (RG * DS = 4 waves).
-template <int L, int RT, int RG, int DS, int STAGES, typename Tag>
-__global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void latent_decode_kernel(LatentArgs a) {
+// L: latent size. RG: row groups of 16. KS: parts of E in the first product.
+template <int L, int RG, int KS, typename Tag>
+__global__ __launch_bounds__(64 * kWaves, 2) void latent_decode_kernel(LatentArgs a) {
   constexpr int E = L + kRope;
-  constexpr int KK = E / 32;
-  constexpr int CH = E / 8;                    // 16-byte chunks of a row
-  constexpr int NL = kTile * CH / 64 / 4;      // loads of a wave and tile
-  constexpr int NDT = L / 16 / DS;             // 16-column tiles of a wave
-  constexpr int RB = RG * RT * 16;
-  constexpr int kStageElems = kTile * E;
-  static_assert(RG * DS == 4 && kTile * CH % 256 == 0 && STAGES >= 2);
+  constexpr int KK = E / 32 / KS;                   // k-steps of a wave
+  constexpr int CH = L / 8;                         // 16-byte chunks of a latent
+  constexpr int NLAT = kTile * CH / 64 / kWaves;    // loads of a wave and tile: of latents,
+  constexpr int kRopeWaves = kTile * 8 / 64;        // and in the first waves one of rotated parts
+  constexpr int DG = kWaves / RG;                   // column groups
+  constexpr int NDT = L / 16 / DG;                  // 16-column tiles of a wave
+  constexpr int RB = RG * 16;
+  constexpr int kLat = kTile * L, kRot = kTile * kRope;
+  static_assert(2 * RG * KS <= kWaves && KK * KS * 32 == E);
 
-  __shared__ __align__(16) uint16_t s_kv[STAGES * kStageElems];
+  __shared__ __align__(16) uint16_t s_lat[kStages * kLat];
+  __shared__ __align__(16) uint16_t s_rot[kRopeStages * kRot];
+  __shared__ f32x4 s_s[2][KS][RG][2][64];  // scores of the next tile and of this one
   __shared__ int s_ids[kIdSlots];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
-  const int rg = wave / DS, ds = wave % DS;
+  const int rg = wave % RG, dg = wave / RG;                  // of the second product
+  const int q_tt = wave & 1, q_rg = (wave >> 1) % RG;       // of the first
+  const int q_ks = min(wave / (2 * RG), KS - 1);             // waves without a part of it repeat one
 
   // The batch's tiles, this run's share of them, and the sequence in which it starts.
-  int64_t total = 0;
+  uint32_t total = 0;
+  int nt = 0, incl = 0;  // of the last 64 sequences looked at
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    const int nt = b0 + lane < a.batch ? (latent_len(a, b0 + lane) + kTile - 1) / kTile : 0;
-    const int incl = wave_scan(nt, lane);
+    nt = b0 + lane < a.batch ? (latent_len(a, b0 + lane) + kTile - 1) / kTile : 0;
+    incl = wave_scan(nt, lane);
     if (blockIdx.x == 0 && wave == 0 && b0 + lane < a.batch) a.first_tile[b0 + lane] = int(total) + incl - nt;
-    total += __builtin_amdgcn_readlane(incl, 63);
+    total += uint32_t(__builtin_amdgcn_readlane(incl, 63));
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) a.first_tile[a.batch] = int(total);
-  total *= a.row_blocks;
-  const int64_t runs = runs_of(a, total);
-  if (int64_t(blockIdx.x) >= runs || total == 0) return;
-  const int64_t start = blockIdx.x * total / runs, end = (blockIdx.x + 1) * total / runs;
+  total *= uint32_t(a.row_blocks);
+  const Runs runs(a, total);
+  if (blockIdx.x >= runs.runs || total == 0) return;
+  const uint32_t start = runs.start(blockIdx.x), end = runs.start(blockIdx.x + 1);
   int b = 0;
-  int64_t unit0 = 0;  // position of sequence b's first tile
+  uint32_t unit0 = 0;  // position of sequence b's first tile
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    const int nt = b0 + lane < a.batch ? (latent_len(a, b0 + lane) + kTile - 1) / kTile : 0;
-    const int incl = wave_scan(nt, lane);
-    const int sum = __builtin_amdgcn_readlane(incl, 63);
-    if (unit0 + int64_t(sum) * a.row_blocks > start) {
-      const uint64_t past = __builtin_amdgcn_ballot_w64(unit0 + int64_t(incl) * a.row_blocks > start);
+    if (a.batch > 64) {
+      nt = b0 + lane < a.batch ? (latent_len(a, b0 + lane) + kTile - 1) / kTile : 0;
+      incl = wave_scan(nt, lane);
+    }
+    const uint32_t sum = uint32_t(__builtin_amdgcn_readlane(incl, 63));
+    if (unit0 + sum * a.row_blocks > start) {
+      const uint64_t past = __builtin_amdgcn_ballot_w64(unit0 + uint32_t(incl) * a.row_blocks > start);
       const int l = __builtin_ctzll(past);
       b = b0 + l;
-      unit0 += int64_t(__builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(nt, l)) * a.row_blocks;
+      unit0 += uint32_t(__builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(nt, l)) * a.row_blocks;
       break;
     }
-    unit0 += int64_t(sum) * a.row_blocks;
+    unit0 += sum * a.row_blocks;
   }
 
-  // This lane's part of a tile's loads: row and byte of the row, and its operand reads.
-  int load_row[NL], load_off[NL];
+  // This lane's part of a tile's loads. Row r's latent is chunks [CH r, CH (r + 1)) of the stage, its
+  // rotated part 8 chunks behind the latents; a wave's load takes 64 chunks.
+  uint32_t lat_off[NLAT];
 #pragma unroll
-  for (int i = 0; i < NL; ++i) {
-    const int f = (wave * NL + i) * 64 + lane;
-    load_row[i] = f / CH;
-    load_off[i] = 8 * ((f % CH) ^ swz8(load_row[i]));
+  for (int i = 0; i < NLAT; ++i) {
+    const int f = (wave * NLAT + i) * 64 + lane;
+    lat_off[i] = 16 * ((f % CH) ^ swz16(f / CH));
   }
-  int k_at[2];  // K chunk 4 kk + g of row n, for even and odd kk (elements)
+  const int rope_row = (wave * 8 + (lane >> 3)) & (kTile - 1);
+  const uint32_t rope_off = 2 * L + 16 * ((lane & 7) ^ swz8(rope_row));
+  // Its operand reads (elements): of K row 16 q_tt + n each k-step, of V row 4 g + n / 4 chunk
+  // 2 dt + (lane & 2) / 2 by dt % 8.
+  int k_at[KK], v_at[NDT];
 #pragma unroll
-  for (int o = 0; o < 2; ++o) k_at[o] = n * E + 8 * ((4 * o + g) ^ swz8(n));
-  int v_at[4];  // V chunk 2 dt + (lane & 2) / 2 of row 4 g + n / 4, for dt % 4
+  for (int i = 0; i < KK; ++i) {
+    const int kk = q_ks * KK + i, r = 16 * q_tt + n;
+    k_at[i] = kk < L / 32 ? r * L + 8 * ((4 * kk + g) ^ swz16(n))
+                          : r * kRope + 8 * ((4 * (kk - L / 32) + g) ^ swz8(n));
+  }
   {
     const int r = 4 * g + (n >> 2);
 #pragma unroll
-    for (int o = 0; o < 4; ++o) v_at[o] = r * E + 8 * ((2 * o + ((lane >> 1) & 1)) ^ swz8(r)) + 4 * (lane & 1);
+    for (int o = 0; o < NDT; ++o) {
+      v_at[o] = r * L + 8 * ((2 * (dg * NDT + o) + ((lane >> 1) & 1)) ^ swz16(r)) + 4 * (lane & 1);
+    }
   }
+  uint64_t zero_row = reinterpret_cast<uint64_t>(g_zero_latent);
+  asm("" : "+s"(zero_row));  // held, not looked up again for every tile
 
-  for (int64_t p = start; p < end;) {
+  for (uint32_t p = start; p < end;) {
     const int len = latent_len(a, b);
-    const int nt = (len + kTile - 1) / kTile;
-    const int64_t rel = p - unit0;
-    if (rel >= int64_t(nt) * a.row_blocks) {
-      unit0 += int64_t(nt) * a.row_blocks;
+    const int tiles = (len + kTile - 1) / kTile;
+    const uint32_t rel = p - unit0;
+    if (rel >= uint32_t(tiles) * a.row_blocks) {
+      unit0 += uint32_t(tiles) * a.row_blocks;
       ++b;
       continue;
     }
-    const int rb = int(rel / nt);
-    const int t0 = int(rel - int64_t(rb) * nt);
-    const int t1 = int(min(int64_t(nt), t0 + (end - p)));
-    const int row0 = rb * RB + rg * RT * 16;
+    const int rb = a.row_blocks == 1 ? 0 : int(rel / uint32_t(tiles));
+    const int t0 = int(rel) - rb * tiles;
+    const int t1 = min(tiles, t0 + int(end - p));
 
-    u32x4 q[RT][KK];
-    int limit[RT];  // last position that this lane's rows see
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int r = min(row0 + rt * 16 + n, a.rows - 1);  // rows behind the last are not stored
+    u32x4 q[KK];
+    {
+      const int r = min(rb * RB + q_rg * 16 + n, a.rows - 1);  // rows behind the last are not stored
       const int tok = r / a.heads, h = r - tok * a.heads;
-      limit[rt] = len - a.new_tokens + tok;
-      const uint16_t* src = a.q + b * a.q_sb + tok * a.q_st + h * a.q_sh + 8 * g;
+      const uint16_t* src = a.q + b * a.q_sb + tok * a.q_st + h * a.q_sh + 32 * KK * q_ks + 8 * g;
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) q[rt][kk] = load16(src + 32 * kk);
+      for (int kk = 0; kk < KK; ++kk) q[kk] = load16(src + 32 * kk);
     }
-    f32x4 o[NDT][RT];
-    float m[RT], l[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      m[rt] = -INFINITY;
-      l[rt] = 0.f;
-#pragma unroll
-      for (int dt = 0; dt < NDT; ++dt) o[dt][rt] = f32x4{};
+    // Rows that no other workgroup reads are streamed (kPolicyStream). A sequence whose first block another one
+    // also starts with shares pages with it (prefix caching shares whole chains of blocks from the first on).
+    bool stream = a.row_blocks == 1 && total >= kStreamTiles;
+    if (stream) {
+      const int first = a.block_table[b * a.bt_stride];
+      for (int b0 = 0; b0 < a.batch; b0 += 64) {
+        const int other = b0 + lane;
+        if (__builtin_amdgcn_ballot_w64(other < a.batch && other != b &&
+                                        a.block_table[min(other, a.batch - 1) * a.bt_stride] == first)) {
+          stream = false;
+        }
+      }
     }
+    const int row = rb * RB + rg * 16 + n;
+    const int limit = len - a.new_tokens + min(row, a.rows - 1) / a.heads;  // last position that it sees
+    f32x4 o[NDT];
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) o[dt] = f32x4{};
 
     // Tiles in pieces whose block ids fit s_ids.
-    const int piece = int(min(int64_t(1) << 30, int64_t(kIdSlots - 2) * a.page_size / kTile));
+    const int piece = int(min(int64_t(1) << 24, int64_t(kIdSlots - 2) * a.page_size / kTile));
     for (int a0 = t0; a0 < t1; a0 += piece) {
       const int a1 = min(t1, a0 + piece);
       const int page0 = a0 * kTile / a.page_size;
       const int pages = (min(a1 * kTile, len) - 1) / a.page_size - page0 + 1;
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the last piece is read
-      for (int i = threadIdx.x; i < pages; i += 256) s_ids[i] = a.block_table[b * a.bt_stride + page0 + i];
+      for (int i = threadIdx.x; i < pages; i += 64 * kWaves) {
+        s_ids[i] = a.block_table[b * a.bt_stride + page0 + i];
+      }
       // Everything that the compiler knows of has landed too, q among it, so that it places no wait of its
       // own (which would also wait for the tiles in flight) in the loop below.
       __builtin_amdgcn_s_waitcnt(0);
       asm volatile("s_barrier" ::: "memory");
 
-      uint32_t there[STAGES];  // the staged tiles' tokens that exist, next tile first
-      auto issue = [&](int t, int stage) {
-        const int pos = t * kTile + (lane & 31);
-        int row = -1;
-        if (pos < len) {
-          const int page = a.page_shift >= 0 ? pos >> a.page_shift : pos / a.page_size;
-          const int id = s_ids[page - page0];
-          if (uint32_t(id) < uint32_t(a.num_blocks32)) row = id * a.page_size + (pos - page * a.page_size);
-        }
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-          // An absent token's row is zeros, not what the cache may hold there.
-          const int r = __shfl(row, load_row[i], 64);
-          const uint16_t* base = r >= 0 ? a.cache : g_zero_latent;
-          load_lds16_at(base + (uint64_t(uint32_t(max(r, 0))) * E + load_off[i]),
-                        s_kv + stage * kStageElems + (wave * NL + i) * 512);
-        }
-        return uint32_t(__builtin_amdgcn_ballot_w64(row >= 0));
+      // Token lane % 32 of the tile to load next: position, slot of its block id, place in the block. They
+      // advance tile by tile, without a division.
+      int pos = a0 * kTile + (lane & (kTile - 1));
+      int slot = a.page_shift >= 0 ? pos >> a.page_shift : pos / a.page_size;
+      int in_page = pos - slot * a.page_size;
+      slot -= page0;
+      const int step_slots = kTile / a.page_size, step_rest = kTile % a.page_size;
+      auto read_id = [&]() { return s_ids[min(slot, kIdSlots - 1)]; };
+      // Address of that token's row given its block id, and on to the next tile; zeros for an absent token,
+      // not what the cache may hold there.
+      uint32_t here = 0;  // the tile's tokens that exist
+      auto row_of = [&](int id) {
+        const bool ok = pos < min(len, a1 * kTile) && uint32_t(id) < uint32_t(a.num_blocks32);
+        here = uint32_t(__builtin_amdgcn_ballot_w64(ok));
+        const uint64_t at = reinterpret_cast<uint64_t>(a.cache) +
+                            uint64_t(uint32_t(id * a.page_size + in_page)) * (2 * E);
+        pos += kTile;
+        slot += step_slots;
+        in_page += step_rest;
+        const bool over = in_page >= a.page_size;
+        slot += over ? 1 : 0;
+        in_page -= over ? a.page_size : 0;
+        return ok ? at : zero_row;
       };
-      int stage = 0;
-      constexpr int kAhead = STAGES == 2 ? 2 : STAGES - 1;
+      auto issue_as = [&](auto policy, uint64_t at, int i) __attribute__((always_inline)) {  // tile a0 + i
+        constexpr bool STREAM = decltype(policy)::value;
+        const int lo = int(uint32_t(at)), hi = int(uint32_t(at >> 32));
+        uint16_t* to = s_lat + (i & (kStages - 1)) * kLat;
+        if constexpr (CH == 64) {  // a load is one row: its address is uniform
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        if (a0 + i < a1) there[i] = issue(a0 + i, i);
-      }
-      for (int t = a0; t < a1; ++t) {
-        // Tile t has landed in every wave's part of the stage.
-        if constexpr (STAGES == 2) {
-          if (t + 1 < a1) wait_loads_barrier<NL>();
+          for (int j = 0; j < NLAT; ++j) {
+            const int r = wave * NLAT + j;
+            const uint64_t src = uint64_t(uint32_t(__builtin_amdgcn_readlane(lo, r))) |
+                                 uint64_t(uint32_t(__builtin_amdgcn_readlane(hi, r))) << 32;
+            load_lds16_from<STREAM>(src, lat_off[j], to + r * 512);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < NLAT; ++j) {
+            const int r = ((wave * NLAT + j) * 64 + lane) / CH;
+            const uint64_t src = uint64_t(uint32_t(__shfl(lo, r, 64))) | uint64_t(uint32_t(__shfl(hi, r, 64))) << 32;
+            load_lds16_at<STREAM>(src + lat_off[j], to + (wave * NLAT + j) * 512);
+          }
+        }
+        if (wave < kRopeWaves) {
+          const uint64_t src = uint64_t(uint32_t(__shfl(lo, rope_row, 64))) |
+                               uint64_t(uint32_t(__shfl(hi, rope_row, 64))) << 32;
+          load_lds16_at<STREAM>(src + rope_off, s_rot + int(unsigned(i) % kRopeStages) * kRot + wave * 512);
+        }
+      };
+      auto issue = [&](uint64_t at, int i) __attribute__((always_inline)) {
+        if (stream) issue_as(std::true_type{}, at, i);
+        else issue_as(std::false_type{}, at, i);
+      };
+      // Waits until all but this wave's loads of the `more` newest tiles have landed, and for the others' too.
+      auto landed = [&](int more) {
+        if (wave < kRopeWaves) {
+          if (more >= 2) wait_loads_barrier<2 * (NLAT + 1)>();
+          else if (more == 1) wait_loads_barrier<NLAT + 1>();
           else wait_loads_barrier<0>();
         } else {
-          const int more = min(kAhead - 1, a1 - 1 - t);
-          if (more >= 2) wait_loads_barrier<2 * NL>();
-          else if (more == 1) wait_loads_barrier<NL>();
+          if (more >= 2) wait_loads_barrier<2 * NLAT>();
+          else if (more == 1) wait_loads_barrier<NLAT>();
           else wait_loads_barrier<0>();
         }
+      };
+      // The first product of tile a0 + i. All reads before the first MFMA (sched_barrier: left to itself the
+      // compiler reads each operand right before its MFMA and waits for it).
+      u32x4 k[KK];
+      auto read_keys = [&](int i) {
+        const uint16_t* lat = s_lat + (i & (kStages - 1)) * kLat;
+        const uint16_t* rot = s_rot + int(unsigned(i) % kRopeStages) * kRot;
+#pragma unroll
+        for (int j = 0; j < KK; ++j) {
+          // the last part's last two k-steps are the rotated ones
+          const uint16_t* from = j < KK - 2 ? lat : q_ks == KS - 1 ? rot : lat;
+          k[j] = *reinterpret_cast<const u32x4*>(from + k_at[j]);
+        }
+      };
+      auto score = [&](int i) {
+        f32x4 s[2] = {};
+#pragma unroll
+        for (int j = 0; j < KK; ++j) s[j & 1] = mfma16x16x32(k[j], q[j], s[j & 1], Tag{});
+        if (wave < 2 * RG * KS) s_s[i & 1][q_ks][q_rg][q_tt][lane] = s[0] + s[1];
+      };
+      uint32_t there[kStages - 1];  // of tiles t, t + 1 and t + 2
+#pragma unroll
+      for (int i = 0; i < kStages - 1; ++i) {
+        const uint64_t at = row_of(read_id());
+        there[i] = here;
+        if (a0 + i < a1) issue(at, i);
+      }
+      uint64_t next = row_of(read_id());
+      uint32_t next_there = here;
+      landed(a1 - 1 - a0);
+      read_keys(0);
+      __builtin_amdgcn_sched_barrier(0);
+      score(0);
+      landed(min(1, a1 - 2 - a0));
+      for (int t = a0; t < a1; ++t) {
+        // Here the scores of tile t, its V and the K of tile t + 1 are in LDS and tile t - 1 is free.
+        const int i = t - a0;
+        if (t + kStages - 1 < a1) issue(next, i + kStages - 1);
         const uint32_t mask = there[0];
+        there[0] = there[1];
+        there[1] = there[2];
+        there[2] = next_there;
+        const int next_id = read_id();
+        f32x4 y[KS][2];
 #pragma unroll
-        for (int i = 0; i + 1 < kAhead; ++i) there[i] = there[i + 1];
-        if constexpr (STAGES > 2) {
-          const int into = stage == 0 ? STAGES - 1 : stage - 1;
-          if (t + kAhead < a1) there[kAhead - 1] = issue(t + kAhead, into);
+        for (int j = 0; j < KS; ++j) {
+          y[j][0] = s_s[i & 1][j][rg][0][lane];
+          y[j][1] = s_s[i & 1][j][rg][1][lane];
         }
-        const uint16_t* kv = s_kv + stage * kStageElems;
-
-        f32x4 s[2][RT];
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) s[tt][rt] = f32x4{};
-        }
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-#pragma unroll
-          for (int tt = 0; tt < 2; ++tt) {
-            const u32x4 k = *reinterpret_cast<const u32x4*>(kv + k_at[kk & 1] + 64 * (kk >> 1) + 16 * tt * E);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) s[tt][rt] = mfma16x16x32(k, q[rt][kk], s[tt][rt], Tag{});
-          }
-        }
-        const bool whole = mask == 0xffffffffu && t * kTile + kTile - 1 <= len - a.new_tokens;
-        u32x4 pb[RT];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          float x[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = s[e >> 2][rt][e & 3] * a.scale_log2;
-          if (!whole) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int j = 16 * (e >> 2) + 4 * g + (e & 3);
-              if (!((mask >> j) & 1) || t * kTile + j > limit[rt]) x[e] = -INFINITY;
-            }
-          }
-          float top = x[0];
-#pragma unroll
-          for (int e = 1; e < 8; ++e) top = max2(top, x[e]);
-          top = row_group_max(top);
-          if (__builtin_amdgcn_ballot_w64(top > m[rt] + kSlack)) {  // m = -inf at first
-            const float mn = fmaxf(m[rt], top);
-            const float c = mn == -INFINITY ? 1.f : fast_exp2(m[rt] - mn);
-            m[rt] = mn;
-            l[rt] *= c;
-#pragma unroll
-            for (int dt = 0; dt < NDT; ++dt) o[dt][rt] *= c;
-          }
-          const float base = m[rt] == -INFINITY ? 0.f : m[rt];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            x[e] = fast_exp2(x[e] - base);
-            l[rt] += x[e];
-          }
-          // P is rounded to the cache's type for the matrix unit, as in the paged decode: at most half a
-          // step of each weight, while l sums the unrounded ones in 32 bits.
-#pragma unroll
-          for (int e = 0; e < 4; ++e) pb[rt][e] = pack2(x[2 * e], x[2 * e + 1], Tag{});
-        }
+        read_keys(i + 1);  // behind the last tile, of what is there: those scores are not used
+        u32x2 v[NDT][2];
+        const uint16_t* lat = s_lat + (i & (kStages - 1)) * kLat;
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) {
-          const int at = v_at[dt & 3] + 64 * (dt >> 2) + ds * NDT * 16;
-          const u32x2 lo = lds_read_tr4(kv + at), hi = lds_read_tr4(kv + at + 16 * E);
-          const u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
+          v[dt][0] = lds_read_tr4(lat + v_at[dt]);
+          v[dt][1] = lds_read_tr4(lat + v_at[dt] + 16 * L);
+        }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) o[dt][rt] = mfma16x16x32(v, pb[rt], o[dt][rt], Tag{});
+        for (int j = 1; j < KS; ++j) {
+          y[0][0] += y[j][0];
+          y[0][1] += y[j][1];
         }
-        if constexpr (STAGES == 2) {
-          asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the stage is read
-          if (t + 2 < a1) there[1] = issue(t + 2, stage);
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = y[0][e >> 2][e & 3] * a.scale_log2;
+        if (mask != 0xffffffffu || t * kTile + kTile - 1 > len - a.new_tokens) {  // uniform
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int j = 16 * (e >> 2) + 4 * g + (e & 3);
+            if (!((mask >> j) & 1) || t * kTile + j > limit) x[e] = -INFINITY;
+          }
         }
-        stage = stage == STAGES - 1 ? 0 : stage + 1;
+        float top = max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max2(x[6], x[7]));
+        top = row_group_max(top);
+        if (__builtin_amdgcn_ballot_w64(top > m + kSlack)) {  // m = -inf at first
+          const float mn = fmaxf(m, top);
+          const float c = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
+          m = mn;
+          l *= c;
+#pragma unroll
+          for (int dt = 0; dt < NDT; ++dt) o[dt] *= c;
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        score(i + 1);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = fast_exp2(x[e] - base);
+        l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        // P is rounded to the cache's type for the matrix unit, as in the paged decode: at most half a
+        // step of each weight, while l sums the unrounded ones in 32 bits.
+        const u32x4 pb = {pack2(x[0], x[1], Tag{}), pack2(x[2], x[3], Tag{}), pack2(x[4], x[5], Tag{}),
+                          pack2(x[6], x[7], Tag{})};
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) {
+          o[dt] = mfma16x16x32(u32x4{v[dt][0][0], v[dt][0][1], v[dt][1][0], v[dt][1][1]}, pb, o[dt], Tag{});
+        }
+        next = row_of(next_id);
+        next_there = here;
+        landed(t + kStages - 1 < a1 ? 1 : 0);  // tile t + 2, and every wave is done with tile t
       }
     }
 
-    const bool complete = t0 == 0 && t1 == nt;
-    const int64_t part = (int64_t(blockIdx.x) * 2 + (p == start ? 0 : 1)) * RB + rg * RT * 16;
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int r = row0 + rt * 16 + n;
-      const float lt = row_group_sum(l[rt]);
-      if (r >= a.rows) continue;
-      if (complete) {
-        const float inv = lt != 0.f ? 1.f / lt : 0.f;  // a row that sees nothing is zero
-        uint16_t* dst = a.out + (int64_t(b) * a.rows + r) * L + ds * NDT * 16 + 4 * g;
+    l = row_group_sum(l);
+    if (row < a.rows) {
+      if (t0 == 0 && t1 == tiles) {
+        const float inv = l != 0.f ? 1.f / l : 0.f;  // a row that sees nothing is zero
+        uint16_t* dst = a.out + (int64_t(b) * a.rows + row) * L + dg * NDT * 16 + 4 * g;
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) {
-          const f32x4 y = o[dt][rt] * inv;
+          const f32x4 y = o[dt] * inv;
           *reinterpret_cast<u32x2*>(dst + 16 * dt) = u32x2{pack2(y[0], y[1], Tag{}), pack2(y[2], y[3], Tag{})};
         }
       } else {
-        float* dst = a.part_o + (part + rt * 16 + n) * L + ds * NDT * 16 + 4 * g;
+        const int64_t part = (int64_t(blockIdx.x) * 2 + (p == start ? 0 : 1)) * RB + rg * 16 + n;
+        float* dst = a.part_o + part * L + dg * NDT * 16 + 4 * g;
 #pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<f32x4*>(dst + 16 * dt) = o[dt][rt];
-        if (g == 0 && ds == 0) {
-          float* ml = a.part_ml + (part + rt * 16 + n) * 2;
-          ml[0] = m[rt];
-          ml[1] = lt;
-        }
+        for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<f32x4*>(dst + 16 * dt) = o[dt];
+        if (g == 0 && dg == 0) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(m, l);
       }
     }
-    p += t1 - t0;
+    p += uint32_t(t1 - t0);
   }
 }
 
-// Joins the parts of units that several runs share, one workgroup of L / 4 threads for each row, in the
-// order of the runs; rows of sequences without tokens are zero.
+// Joins the parts of units that several runs share, one workgroup for each row, in a fixed order; rows of
+// sequences without tokens are zero. The parts' weights first (one latency for all of them), then
+// 1024 / L groups of threads each sum every so many-th part, eight in flight, and add up through LDS.
+constexpr int kMergeParts = 1024;  // parts of a unit whose weights are held at a time
+
 template <int L, typename Tag>
-__global__ __launch_bounds__(L / 4) void latent_merge_kernel(LatentArgs a, int rb_rows) {
+__global__ __launch_bounds__(256) void latent_merge_kernel(LatentArgs a, int rb_rows) {
+  constexpr int COLS = L / 4, GROUPS = 256 / COLS;
+  __shared__ float s_c[kMergeParts];
+  __shared__ float s_red[4][2];
+  __shared__ f32x4 s_o[GROUPS - 1][COLS];
   const int b = blockIdx.x / a.rows, r = blockIdx.x - b * a.rows;
   const int rb = r / rb_rows, rr = r - rb * rb_rows;
   const int f0 = a.first_tile[b], f1 = a.first_tile[b + 1];
-  const int64_t total = int64_t(a.first_tile[a.batch]) * a.row_blocks;
-  const int64_t nt = f1 - f0;
-  uint16_t* dst = a.out + (int64_t(b) * a.rows + r) * L + 4 * threadIdx.x;
+  const uint32_t total = uint32_t(a.first_tile[a.batch]) * a.row_blocks;
+  const uint32_t nt = uint32_t(f1 - f0);
+  const int col = threadIdx.x % COLS, group = threadIdx.x / COLS;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint16_t* dst = a.out + (int64_t(b) * a.rows + r) * L + 4 * col;
   if (nt == 0) {
-    *reinterpret_cast<u32x2*>(dst) = u32x2{0, 0};
+    if (group == 0) *reinterpret_cast<u32x2*>(dst) = u32x2{0, 0};
     return;
   }
-  const int64_t runs = runs_of(a, total);
-  const int64_t u0 = int64_t(f0) * a.row_blocks + rb * nt;
-  const int64_t i0 = run_at(u0, total, runs), i1 = run_at(u0 + nt - 1, total, runs);
+  const Runs runs(a, total);
+  const uint32_t u0 = uint32_t(f0) * a.row_blocks + rb * nt;
+  const int i0 = int(runs.holding(u0)), i1 = int(runs.holding(u0 + nt - 1));
   if (i0 == i1) return;  // written by its run
-  const int64_t first = (i0 * 2 + (i0 * total / runs == u0 ? 0 : 1)) * rb_rows + rr;
-  auto part = [&](int64_t i) { return i == i0 ? first : i * 2 * rb_rows + rr; };
+  const int parts = i1 - i0 + 1;  // at most the runs, of which there are no more than kMergeParts
+  // Part i0 is that run's first one (slot 0) if the unit begins with the run, else its last (slot 1).
+  const int64_t row0 = int64_t(i0) * 2 * rb_rows + rr;
+  const int64_t row_first = row0 + (runs.start(i0) == u0 ? 0 : rb_rows);
+  auto part = [&](int i) { return i == 0 ? row_first : row0 + int64_t(i) * 2 * rb_rows; };
   float top = -INFINITY;
-  for (int64_t i = i0; i <= i1; ++i) top = fmaxf(top, a.part_ml[part(i) * 2]);
-  const float base = top == -INFINITY ? 0.f : top;
-  f32x4 o = {};
-  float l = 0.f;
-#pragma unroll 8
-  for (int64_t i = i0; i <= i1; ++i) {
-    const int64_t at = part(i);
-    const float c = fast_exp2(a.part_ml[at * 2] - base);
-    l += c * a.part_ml[at * 2 + 1];
-    const f32x4 x = *reinterpret_cast<const f32x4*>(a.part_o + at * L + 4 * threadIdx.x);
-    o += c * x;
+  float m[kMergeParts / 256], l[kMergeParts / 256];
+#pragma unroll
+  for (int k = 0; k < kMergeParts / 256; ++k) {
+    const int i = 256 * k + int(threadIdx.x);
+    m[k] = -INFINITY;
+    l[k] = 0.f;
+    if (i < parts) {
+      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + part(i) * 2);
+      m[k] = ml.x;
+      l[k] = ml.y;
+    }
+    top = fmaxf(top, m[k]);
   }
-  const float inv = l != 0.f ? 1.f / l : 0.f;
-  o *= inv;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+  if (lane == 0) s_red[wave][0] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(s_red[0][0], s_red[1][0]), fmaxf(s_red[2][0], s_red[3][0]));
+  const float base = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < kMergeParts / 256; ++k) {
+    const float c = fast_exp2(m[k] - base);
+    s_c[256 * k + threadIdx.x] = c;
+    sum += c * l[k];
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
+  if (lane == 0) s_red[wave][1] = sum;
+  __syncthreads();
+  sum = (s_red[0][1] + s_red[1][1]) + (s_red[2][1] + s_red[3][1]);
+  f32x4 o = {};
+#pragma unroll 8
+  for (int i = group; i < parts; i += GROUPS) {
+    o += s_c[i] * *reinterpret_cast<const f32x4*>(a.part_o + part(i) * L + 4 * col);
+  }
+  if (group > 0) s_o[group - 1][col] = o;
+  __syncthreads();
+  if (group > 0) return;
+#pragma unroll
+  for (int k = 0; k + 1 < GROUPS; ++k) o += s_o[k][col];
+  o *= sum != 0.f ? 1.f / sum : 0.f;
   *reinterpret_cast<u32x2*>(dst) = u32x2{pack2(o[0], o[1], Tag{}), pack2(o[2], o[3], Tag{})};
 }
 
 // Rows of a workgroup for a sequence's rows.
-int rows_per_block(int32_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+int rows_per_block(int32_t rows) { return rows <= 16 ? 16 : 32; }
 
-int plan_runs(int32_t rb) { return device_cu_count() * (rb <= 32 ? 2 : 1); }
 
 int64_t align16(int64_t x) { return (x + 15) & ~int64_t(15); }
 
@@ -404,7 +556,7 @@ LatentSizes latent_sizes(int32_t batch, int32_t new_tokens, int32_t heads, int32
   const int32_t rows = new_tokens * heads;
   s.rb = rows_per_block(rows);
   s.row_blocks = int32_t(ceil_div(rows, s.rb));
-  s.runs = plan_runs(s.rb);
+  s.runs = device_cu_count() < kMergeParts ? device_cu_count() : kMergeParts;  // one workgroup a CU: its LDS
   s.o_floats = int64_t(s.runs) * 2 * s.rb * latent;
   s.ml_floats = int64_t(s.runs) * 2 * s.rb * 2;
   s.bytes = align16((s.o_floats + s.ml_floats) * 4 + (int64_t(batch) + 1) * 4);
@@ -426,11 +578,10 @@ int check_latent(const char* who, int32_t batch, int32_t new_tokens, int32_t hea
 
 template <int L, typename Tag>
 void launch_latent(const LatentArgs& a, int rb, hipStream_t s) {
-  const dim3 grid(unsigned(a.runs)), block(256);
-  if (rb == 16) hipLaunchKernelGGL((latent_decode_kernel<L, 1, 1, 4, 2, Tag>), grid, block, 0, s, a);
-  else if (rb == 32) hipLaunchKernelGGL((latent_decode_kernel<L, 1, 2, 2, 2, Tag>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((latent_decode_kernel<L, 2, 2, 2, 3, Tag>), grid, block, 0, s, a);
-  hipLaunchKernelGGL((latent_merge_kernel<L, Tag>), dim3(unsigned(a.batch * a.rows)), dim3(L / 4), 0, s, a, rb);
+  const dim3 grid(unsigned(a.runs)), block(64 * kWaves);
+  if (rb == 16) hipLaunchKernelGGL((latent_decode_kernel<L, 1, L == 512 ? 3 : 2, Tag>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((latent_decode_kernel<L, 2, 2, Tag>), grid, block, 0, s, a);
+  hipLaunchKernelGGL((latent_merge_kernel<L, Tag>), dim3(unsigned(a.batch * a.rows)), dim3(256), 0, s, a, rb);
 }
 
 }  // namespace
@@ -471,6 +622,11 @@ extern "C" int ti_latent_decode_paged(const void* q, int64_t q_stride_b, int64_t
     return fail(TI_EINVAL, "%s: max_blocks_per_seq %d x page_size %d exceeds 2^31", who,
                 max_blocks_per_seq, page_size);
   }
+  const LatentSizes sz = latent_sizes(batch, new_tokens, num_heads, latent_dim);
+  if (int64_t(batch) * sz.row_blocks * (ceil_div(int64_t(max_blocks_per_seq) * page_size, kTile) + 1) > INT32_MAX) {
+    return fail(TI_EINVAL, "%s: batch %d x %d tokens x %d rows is more than one call takes", who, batch,
+                max_blocks_per_seq * page_size, new_tokens * num_heads);
+  }
   if (batch == 0) return TI_OK;
   if (!q || !seqlen || !out || !workspace || (max_blocks_per_seq > 0 && (!latent_cache || !block_table))) {
     return fail(TI_EINVAL, "%s: null pointer", who);
@@ -480,7 +636,6 @@ extern "C" int ti_latent_decode_paged(const void* q, int64_t q_stride_b, int64_t
       q_stride_b % 8 != 0 || q_stride_t % 8 != 0 || q_stride_h % 8 != 0) {
     return fail(TI_EINVAL, "%s: q, cache, out and workspace must be 16-byte aligned, q strides multiples of 8", who);
   }
-  const LatentSizes sz = latent_sizes(batch, new_tokens, num_heads, latent_dim);
   if (workspace_bytes < sz.bytes) {
     return fail(TI_EINVAL, "%s: workspace %lld < %lld bytes", who, static_cast<long long>(workspace_bytes),
                 static_cast<long long>(sz.bytes));
@@ -508,7 +663,6 @@ extern "C" int ti_latent_decode_paged(const void* q, int64_t q_stride_b, int64_t
   a.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(unsigned(page_size)) : -1;
   a.max_blocks = max_blocks_per_seq;
   a.runs = sz.runs;
-  a.min_tiles = 4;
   a.scale_log2 = scale * 1.4426950408889634f;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (latent_dim == 512) {
