@@ -486,6 +486,10 @@ int ti_latent_decode_paged(const void* q, int64_t q_stride_b, int64_t q_stride_t
                            int64_t num_blocks, int32_t max_blocks_per_seq, float scale, int32_t dtype,
                            void* stream);
 
+/* Workspace of ti_latent_prefill for these host-known sizes; 0: the call takes one workgroup per unit. */
+int ti_latent_prefill_workspace_bytes(int32_t batch, int32_t total_q, int32_t total_k, int32_t num_heads,
+                                      int32_t head_dim, int64_t* workspace_bytes_out);
+
 /*
  * Latent attention over packed chunks, expanded form: sequence b's queries are rows
  * [cu_seqlens_q[b], cu_seqlens_q[b+1]) of q, its keys rows [cu_seqlens_k[b], cu_seqlens_k[b+1]) of kv
@@ -494,16 +498,19 @@ int ti_latent_decode_paged(const void* q, int64_t q_stride_b, int64_t q_stride_t
  * with the causal mask aligned to the last key (query i sees keys j <= k_len - q_len + i), or without it.
  * A query that sees nothing gives zeros. max_seqlen_q is at least the longest chunk; rows of longer ones
  * are not all written. Offsets beyond total_q / total_k are cut off. head_dim 128 or 64, rope_dim 64;
- * rows 16-byte aligned, strides multiples of 8 elements, token strides of kv and key_rope below 2^24.
+ * rows 16-byte aligned, strides multiples of 8 elements, token strides of kv and key_rope below 2^24, scale
+ * not negative. With a workspace of ti_latent_prefill_workspace_bytes (16-byte aligned, contents need no
+ * initialisation) units of 128 query rows may be cut between workgroups and joined; with NULL every unit is
+ * one workgroup's.
  * The role of the reference's varlen kernel (kernels/gqa_varlen.py:40-185).
  */
 int ti_latent_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* kv,
                       int64_t kv_stride_t, int64_t kv_stride_h, const void* key_rope,
                       int64_t key_stride_t, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
-                      void* out, int64_t out_stride_t, int64_t out_stride_h, int32_t batch,
-                      int32_t total_q, int32_t total_k, int32_t max_seqlen_q, int32_t num_heads,
-                      int32_t head_dim, int32_t rope_dim, int32_t causal, float scale, int32_t dtype,
-                      void* stream);
+                      void* out, int64_t out_stride_t, int64_t out_stride_h, void* workspace,
+                      int64_t workspace_bytes, int32_t batch, int32_t total_q, int32_t total_k,
+                      int32_t max_seqlen_q, int32_t num_heads, int32_t head_dim, int32_t rope_dim,
+                      int32_t causal, float scale, int32_t dtype, void* stream);
 
 /* Workspace of ti_cache_mass for these host-known sizes. */
 int ti_cache_mass_workspace_bytes(int32_t batch, int32_t new_tokens, int32_t num_q_heads,

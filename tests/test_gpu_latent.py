@@ -163,6 +163,12 @@ PREFILLS = [
     (8, 64, BF16, [(5, 3), (70, 65), (129, 0)], True),
     (2, 128, F16, [(257, 640)], False),
     (1, 64, BF16, [(31, 63), (65, 66)], False),
+    # more units than CUs: one workgroup each
+    (48, 64, BF16, [(700, 700), (1, 9), (50, 130)], True),
+    (33, 128, F16, [(1100, 1100)], True),
+    # cut units: few heads over long keys, blocks that see nothing, empty sequences between others
+    (2, 128, BF16, [(300, 2500), (0, 0), (0, 40), (400, 130), (1, 1999)], True),
+    (1, 64, F16, [(129, 3001)] + [(3, 70)] * 70, True),
 ]
 
 

@@ -5,21 +5,25 @@
 // for the queries i and keys j of one sequence, causal and aligned to the last key (query i sees the
 // keys j <= k_len - q_len + i). A first chunk has k_len = q_len, a continuation more keys than queries.
 //
-// Work unit: (sequence, head, 128 query rows), one workgroup of four waves of 32 rows. Keys come in tiles
-// of 64, loaded straight into LDS one tile ahead and read by all waves:
+// Work unit: (head, sequence, 128 query rows). A workgroup of four waves of 32 rows walks a unit's keys in
+// tiles of 64, loaded straight into LDS one tile ahead and read by all waves:
 //   S^T[64 keys x 32 rows]  = K[64 x (DN + 64)] . Q^T        (16x16x32, Q in registers)
 //   O^T[DN x 32 rows]      += V^T[DN x 64] . P^T             (16x16x32, V by transposed reads)
 // with an accumulator's row its lane's column, as in the paged prefill. Two workgroups fit a CU, so that
-// one's softmax runs beside the other's products. The last query blocks, which see the most keys, come
-// first; the blocks of one head follow each other at a distance of H, so with a multiple of 8 heads they
-// share an XCD's L2.
+// one's softmax runs beside the other's products.
+//
+// Two schedules. Per unit: one workgroup each, the last query blocks, which see the most keys, first; no
+// workspace. Balanced: the tiles of all units are one list (by head, sequence, block), cut into equal runs,
+// one for each of the workgroups that fit the GPU; a unit that lies in one run is written by it, others
+// leave (m, l, o) parts in 32 bits that a second kernel joins in the order of the runs. Under a causal mask
+// a first chunk's units differ by a factor of its length, and few heads or a short chunk are fewer units
+// than CUs. Consecutive runs go to the same XCD, whose L2 then serves a head's keys to its blocks.
 #include "lds_tiles.h"
 
 namespace ti {
 namespace {
 
 constexpr int kKeys = 64;      // keys of a tile
-constexpr int kRows = 128;     // query rows of a workgroup
 constexpr int kRope = 64;
 constexpr float kSlack = 8.f;  // exp2 units a row maximum may rise before O is rescaled
 
@@ -34,9 +38,78 @@ struct ExpandedArgs {
   int64_t o_st, o_sh;
   const int32_t* cu_q;
   const int32_t* cu_k;
-  int32_t total_q, total_k, causal;
+  int32_t total_q, total_k, causal, batch, heads;
   float scale_log2;
+  // Balanced schedule (runs > 0): parts of cut units, and each sequence's first tile within a head's.
+  int32_t runs;
+  float* part_o;      // [runs][2][128][DN] unnormalised rows
+  float* part_ml;     // [runs][2][128][2] their (m, l), m in exp2 units
+  int32_t* seq_tile;  // [B + 1]
 };
+
+constexpr int kRows = 128;  // query rows of a workgroup
+constexpr int kXcds = 8;
+
+// A sequence's extent, within the tensors whatever the offsets say, and its units' tiles.
+struct Seq {
+  int q0, q_len, k0, k_len, offset, blocks, shift;
+  bool causal;
+  __device__ __forceinline__ Seq(const ExpandedArgs& a, int b) {
+    q0 = min(max(a.cu_q[b], 0), a.total_q);
+    q_len = min(max(a.cu_q[b + 1], q0), a.total_q) - q0;
+    k0 = min(max(a.cu_k[b], 0), a.total_k);
+    k_len = min(max(a.cu_k[b + 1], k0), a.total_k) - k0;
+    offset = k_len - q_len;  // query i sits at key position offset + i
+    blocks = (q_len + kRows - 1) / kRows;
+    shift = (offset + (offset > 0 ? kKeys - 1 : 0)) / kKeys;  // offset / 64 rounded up
+    causal = a.causal;
+  }
+  // Keys that block qb sees: all under no mask, and to the last one for the last block.
+  __device__ __forceinline__ int key_end(int qb) const {
+    const int end = !causal || qb == blocks - 1 ? k_len : offset + kRows * (qb + 1);
+    return end > 0 ? end : 0;
+  }
+  __device__ __forceinline__ int tiles(int qb) const { return (key_end(qb) + kKeys - 1) / kKeys; }
+  // Tiles of the blocks before qb. Under the mask those of block i < blocks - 1 are 2 (i + 1) + shift, if
+  // positive.
+  __device__ __forceinline__ int before(int qb) const {
+    const int n = max(min(qb, blocks - 1), 0);
+    int sum;
+    if (causal) {
+      const int none = min(max(-shift / 2, 0), n);
+      sum = n * (n + 1 + shift) - none * (none + 1 + shift);
+    } else {
+      sum = n * ((k_len + kKeys - 1) / kKeys);
+    }
+    return qb == blocks && blocks > 0 ? sum + tiles(blocks - 1) : sum;
+  }
+};
+
+// `total` tiles cut into runs, the first `rest` of them one tile longer (32 bits; the host takes the other
+// schedule for longer lists).
+constexpr uint32_t kMinRun = 4;
+struct Runs {
+  uint32_t runs, base, rest;
+  __device__ __forceinline__ Runs(const ExpandedArgs& a, uint32_t total) {
+    runs = max(1u, min(uint32_t(a.runs), total / kMinRun));
+    base = total / runs;
+    rest = total - base * runs;
+  }
+  __device__ __forceinline__ uint32_t start(uint32_t i) const { return i * base + min(i, rest); }
+  __device__ __forceinline__ uint32_t holding(uint32_t u) const {  // the run of position u
+    const uint32_t longer = rest * (base + 1);
+    return u < longer ? u / (base + 1) : rest + (u - longer) / base;
+  }
+};
+
+__device__ __forceinline__ int wave_scan(int x, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(x, d, 64);
+    if (lane >= d) x += y;
+  }
+  return x;
+}
 
 // LDS places of 16-byte chunk c of row r: c ^ swz16(r) in rows of whole 256-byte blocks (kn and v),
 // c ^ swz8(r) in the 128-byte rows of k_r. A ds_read_b128 serves rows {0-3, 12-15} of one chunk with rows
@@ -48,7 +121,7 @@ __device__ __forceinline__ int swz8(int r) {
   return ((2 * u) & 7) ^ ((u & 4) ? 5 : 0);
 }
 
-template <int DN, typename Tag>
+template <int DN, bool BALANCED, typename Tag>
 __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(ExpandedArgs a) {
   constexpr int KN = DN / 32;               // k-steps of the unrotated part
   constexpr int NDT = DN / 16;
@@ -64,31 +137,66 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(ExpandedArgs a) 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
-  const int h = blockIdx.x, b = blockIdx.z;
 
-  // The sequence's extent, within the tensors whatever the offsets say.
-  const int q0 = min(max(a.cu_q[b], 0), a.total_q);
-  const int q_len = min(max(a.cu_q[b + 1], q0), a.total_q) - q0;
-  const int k0 = min(max(a.cu_k[b], 0), a.total_k);
-  const int k_len = min(max(a.cu_k[b + 1], k0), a.total_k) - k0;
-  const int blocks = (q_len + kRows - 1) / kRows;
-  if (int(blockIdx.y) >= blocks) return;
-  const int qb0 = (blocks - 1 - int(blockIdx.y)) * kRows;
-  const int rows = min(kRows, q_len - qb0);
-  const int offset = k_len - q_len;  // query i sits at key position offset + i
-  const int k_end = a.causal ? min(k_len, offset + qb0 + rows) : k_len;
-  const int nt = k_end > 0 ? (k_end + kKeys - 1) / kKeys : 0;
-
-  // Q operands of this wave's rows; rows behind the last repeat it and are not stored.
-  u32x4 q[2][KN + 2];
-  int limit[2];
-#pragma unroll
-  for (int rt = 0; rt < 2; ++rt) {
-    const int r = min(qb0 + wave * 32 + rt * 16 + n, q_len - 1);
-    limit[rt] = a.causal ? offset + r : k_len - 1;
-    const uint16_t* src = a.q + int64_t(q0 + r) * a.q_st + h * a.q_sh + 8 * g;
-#pragma unroll
-    for (int kk = 0; kk < KN + 2; ++kk) q[rt][kk] = load16(src + 32 * kk);
+  int h, b, qb;
+  uint32_t p = 0, start = 0, end = 1;  // the run's positions in the list, and the next one
+  int t_first = 0;                     // first tile of the next unit
+  uint32_t run = 0;
+  if constexpr (BALANCED) {
+    int per_head = 0, nt = 0, incl = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+      nt = 0;
+      if (b0 + lane < a.batch) {
+        const Seq s(a, b0 + lane);
+        nt = s.before(s.blocks);
+      }
+      incl = wave_scan(nt, lane);
+      if (blockIdx.x == 0 && wave == 0 && b0 + lane < a.batch) a.seq_tile[b0 + lane] = per_head + incl - nt;
+      per_head += __builtin_amdgcn_readlane(incl, 63);
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.seq_tile[a.batch] = per_head;
+    const uint32_t total = uint32_t(per_head) * a.heads;
+    const Runs runs(a, total);
+    run = blockIdx.x;
+    if (run >= runs.runs || total == 0) return;
+    if (runs.runs % kXcds == 0) run = run % kXcds * (runs.runs / kXcds) + run / kXcds;
+    start = p = runs.start(run);
+    end = runs.start(run + 1);
+    h = int(p / uint32_t(per_head));
+    int rel = int(p - uint32_t(h) * per_head);
+    b = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+      if (a.batch > 64) {
+        nt = 0;
+        if (b0 + lane < a.batch) {
+          const Seq s(a, b0 + lane);
+          nt = s.before(s.blocks);
+        }
+        incl = wave_scan(nt, lane);
+      }
+      const int sum = __builtin_amdgcn_readlane(incl, 63);
+      if (sum > rel) {
+        const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(incl > rel));
+        b = b0 + l;
+        rel -= __builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(nt, l);
+        break;
+      }
+      rel -= sum;
+    }
+    const Seq s(a, b);
+    int lo = 0, hi = s.blocks - 1;  // the first block whose end lies behind rel
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (s.before(mid + 1) > rel) hi = mid;
+      else lo = mid + 1;
+    }
+    qb = lo;
+    t_first = rel - s.before(qb);
+  } else {
+    h = blockIdx.x;
+    b = blockIdx.z;
+    qb = Seq(a, b).blocks - 1 - int(blockIdx.y);
+    if (qb < 0) return;
   }
 
   // Byte offsets of this lane's loads within a tile.
@@ -103,137 +211,234 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(ExpandedArgs a) 
     const int f = (wave * NKR + i) * 64 + lane, r = f >> 3;
     kr_at[i] = uint32_t(r) * uint32_t(a.kr_st * 2) + 16 * ((f & 7) ^ swz8(r));
   }
-  auto issue = [&](int t, int stage) {
-    const int valid = min(kKeys, k_end - t * kKeys);  // keys past it read as zero
-    const uint16_t* kv = a.kv + int64_t(k0 + t * kKeys) * a.kv_st + h * a.kv_sh;
-    const uint16_t* kr = a.kr + int64_t(k0 + t * kKeys) * a.kr_st;
-    const u32x4 rkv = rsrc_words(kv, uint32_t(valid - 1) * uint32_t(a.kv_st * 2) + ROW * 2);
-    const u32x4 rkr = rsrc_words(kr, uint32_t(valid - 1) * uint32_t(a.kr_st * 2) + kRope * 2);
-    uint16_t* to = s_tile + stage * kStage;
-#pragma unroll
-    for (int i = 0; i < NKV; ++i) load_lds16(rkv, kv_at[i], to + (wave * NKV + i) * 512);
-#pragma unroll
-    for (int i = 0; i < NKR; ++i) load_lds16(rkr, kr_at[i], to + kKeys * ROW + (wave * NKR + i) * 512);
-  };
+  // Operand reads of row n (K) and of row 4 g + n / 4 (V), elements: those of k-step kk and column tile dt are
+  // at these with the bits of kk and dt flipped, which the rows' places leave alone.
+  const int k_at = n * ROW + 8 * (g ^ swz16(n));
+  const int r_at = kKeys * ROW + n * kRope + 8 * (g ^ swz8(n));
+  const int v_row = 4 * g + (n >> 2);
+  const int v_at = v_row * ROW + 8 * ((DN / 8 + ((lane >> 1) & 1)) ^ swz16(v_row)) + 4 * (lane & 1);
 
-  // Operand reads of row n (K) and of row 4 g + n / 4 (V), elements.
-  int k_at[KN], r_at[2], v_at[NDT];
+  while (true) {
+    const Seq sq(a, b);
+    const int tiles = sq.tiles(qb), k_end = sq.key_end(qb);
+    const int t0 = BALANCED ? t_first : 0;
+    const int t1 = BALANCED ? min(tiles, t0 + int(end - p)) : tiles;
+
+    // Q operands of this wave's rows; rows behind the last repeat it and are not stored.
+    u32x4 q[2][KN + 2];
+    int limit[2];
 #pragma unroll
-  for (int kk = 0; kk < KN; ++kk) k_at[kk] = n * ROW + 8 * ((4 * kk + g) ^ swz16(n));
+    for (int rt = 0; rt < 2; ++rt) {
+      const int r = min(qb * kRows + wave * 32 + rt * 16 + n, sq.q_len - 1);
+      limit[rt] = a.causal ? sq.offset + r : sq.k_len - 1;
+      const uint16_t* src = a.q + int64_t(sq.q0 + r) * a.q_st + h * a.q_sh + 8 * g;
 #pragma unroll
-  for (int kk = 0; kk < 2; ++kk) r_at[kk] = kKeys * ROW + n * kRope + 8 * ((4 * kk + g) ^ swz8(n));
-  {
-    const int r = 4 * g + (n >> 2);
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) {
-      v_at[dt] = r * ROW + 8 * ((DN / 8 + 2 * dt + ((lane >> 1) & 1)) ^ swz16(r)) + 4 * (lane & 1);
+      for (int kk = 0; kk < KN + 2; ++kk) q[rt][kk] = load16(src + 32 * kk);
     }
-  }
 
-  f32x4 o[NDT][2];
-  float m[2], l[2];
+    auto issue = [&](int t, int stage) {
+      const int valid = min(kKeys, k_end - t * kKeys);  // keys past it read as zero
+      const uint16_t* kv = a.kv + int64_t(sq.k0 + t * kKeys) * a.kv_st + h * a.kv_sh;
+      const uint16_t* kr = a.kr + int64_t(sq.k0 + t * kKeys) * a.kr_st;
+      const u32x4 rkv = rsrc_words(kv, uint32_t(valid - 1) * uint32_t(a.kv_st * 2) + ROW * 2);
+      const u32x4 rkr = rsrc_words(kr, uint32_t(valid - 1) * uint32_t(a.kr_st * 2) + kRope * 2);
+      uint16_t* to = s_tile + stage * kStage;
 #pragma unroll
-  for (int rt = 0; rt < 2; ++rt) {
-    m[rt] = -INFINITY;
-    l[rt] = 0.f;
+      for (int i = 0; i < NKV; ++i) load_lds16(rkv, kv_at[i], to + (wave * NKV + i) * 512);
 #pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) o[dt][rt] = f32x4{};
-  }
-  // The rows this wave has, the keys its first and its last row see.
-  const int wrow = qb0 + wave * 32;
-  const int see_first = a.causal ? offset + wrow : k_len - 1;
-  const int see_last = a.causal ? offset + min(wrow + 31, q_len - 1) : k_len - 1;
-  const bool active = wrow < q_len;
+      for (int i = 0; i < NKR; ++i) load_lds16(rkr, kr_at[i], to + kKeys * ROW + (wave * NKR + i) * 512);
+    };
 
-  __builtin_amdgcn_s_waitcnt(0);  // q has landed: the loop below has waits of its own alone
-  if (nt > 0) issue(0, 0);
-  if (nt > 1) issue(1, 1);
-  for (int t = 0; t < nt; ++t) {
-    if (t + 1 < nt) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(NL) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    const uint16_t* tile = s_tile + (t & 1) * kStage;
-    if (active && t * kKeys <= see_last) {  // uniform
-      f32x4 s[4][2];
+    f32x4 o[NDT][2];
+    float m[2], l[2];
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt) {
-        s[tt][0] = f32x4{};
-        s[tt][1] = f32x4{};
-      }
+    for (int rt = 0; rt < 2; ++rt) {
+      m[rt] = -INFINITY;
+      l[rt] = 0.f;
 #pragma unroll
-      for (int kk = 0; kk < KN + 2; ++kk) {
+      for (int dt = 0; dt < NDT; ++dt) o[dt][rt] = f32x4{};
+    }
+    // The rows this wave has, the keys its first and its last row see.
+    const int wrow = qb * kRows + wave * 32;
+    const int see_first = a.causal ? sq.offset + wrow : sq.k_len - 1;
+    const int see_last = a.causal ? sq.offset + min(wrow + 31, sq.q_len - 1) : sq.k_len - 1;
+    const bool active = wrow < sq.q_len;
+
+    __builtin_amdgcn_s_waitcnt(0);  // q has landed: the loop below has waits of its own alone
+    if (t0 < t1) issue(t0, 0);
+    if (t0 + 1 < t1) issue(t0 + 1, 1);
+    for (int t = t0; t < t1; ++t) {
+      if (t + 1 < t1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NL) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      const uint16_t* tile = s_tile + ((t - t0) & 1) * kStage;
+      if (active && t * kKeys <= see_last) {  // uniform
+        f32x4 s[4][2];
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt) {
-          const int at = kk < KN ? k_at[kk < KN ? kk : 0] + 16 * tt * ROW
-                                 : r_at[kk < KN ? 0 : kk - KN] + 16 * tt * kRope;
-          const u32x4 k = *reinterpret_cast<const u32x4*>(tile + at);
-#pragma unroll
-          for (int rt = 0; rt < 2; ++rt) s[tt][rt] = mfma16x16x32(k, q[rt][kk], s[tt][rt], Tag{});
+          s[tt][0] = f32x4{};
+          s[tt][1] = f32x4{};
         }
-      }
-      const bool whole = t * kKeys + kKeys - 1 <= see_first && (t + 1) * kKeys <= k_end;
-      u32x4 pb[2][2];
+        // The next k-step's reads go out before the products of the last one (sched_barrier: left to itself the
+        // compiler reads each operand right before its MFMAs and waits for it).
+        u32x4 k[2][4];
+        auto read_keys = [&](int kk, u32x4 (&to)[4]) {
 #pragma unroll
-      for (int rt = 0; rt < 2; ++rt) {
-        float x[16];
+          for (int tt = 0; tt < 4; ++tt) {
+            const int at = kk < KN ? (k_at ^ (32 * kk)) + 16 * tt * ROW : (r_at ^ (32 * (kk - KN))) + 16 * tt * kRope;
+            to[tt] = *reinterpret_cast<const u32x4*>(tile + at);
+          }
+        };
+        read_keys(0, k[0]);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = s[e >> 2][rt][e & 3] * a.scale_log2;
-        if (!whole) {
-          const int lim = min(limit[rt], k_end - 1) - t * kKeys - 4 * g;
+        for (int kk = 0; kk < KN + 2; ++kk) {
+          if (kk + 1 < KN + 2) read_keys(kk + 1, k[(kk + 1) & 1]);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int tt = 0; tt < 4; ++tt) {
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt) s[tt][rt] = mfma16x16x32(k[kk & 1][tt], q[rt][kk], s[tt][rt], Tag{});
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        const bool whole = t * kKeys + kKeys - 1 <= see_first && (t + 1) * kKeys <= k_end;
+        u32x4 pb[2][2];
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) {
+          float x[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[e] = s[e >> 2][rt][e & 3];
+          if (!whole) {
+            const int lim = min(limit[rt], k_end - 1) - t * kKeys - 4 * g;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              if (16 * (e >> 2) + (e & 3) > lim) x[e] = -INFINITY;
+            }
+          }
+          float top = x[0];
+#pragma unroll
+          for (int e = 1; e < 15; e += 2) top = max3(top, x[e], x[e + 1]);
+          top = row_group_max(max2(top, x[15])) * a.scale_log2;  // a scale is not negative
+          if (__builtin_amdgcn_ballot_w64(top > m[rt] + kSlack)) {  // m = -inf at first
+            const float mn = fmaxf(m[rt], top);
+            const float c = mn == -INFINITY ? 1.f : fast_exp2(m[rt] - mn);
+            m[rt] = mn;
+            l[rt] *= c;
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) o[dt][rt] *= c;
+          }
+          const float base = m[rt] == -INFINITY ? 0.f : m[rt];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            if (16 * (e >> 2) + (e & 3) > lim) x[e] = -INFINITY;
+            x[e] = fast_exp2(fmaf(x[e], a.scale_log2, -base));
+            l[rt] += x[e];
+          }
+          // P is rounded to the inputs' type for the matrix unit, as in the paged prefill: at most half a
+          // step of each weight, while l sums the unrounded ones in 32 bits.
+#pragma unroll
+          for (int e = 0; e < 8; ++e) pb[rt][e >> 2][e & 3] = pack2(x[2 * e], x[2 * e + 1], Tag{});
+        }
+#pragma unroll
+        for (int kp = 0; kp < 2; ++kp) {
+#pragma unroll
+          for (int dt = 0; dt < NDT; ++dt) {
+            const uint16_t* at = tile + (v_at ^ (16 * dt)) + 32 * kp * ROW;
+            const u32x2 lo = lds_read_tr4(at), hi = lds_read_tr4(at + 16 * ROW);
+            const u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt) o[dt][rt] = mfma16x16x32(v, pb[rt][kp], o[dt][rt], Tag{});
           }
         }
-        float top = x[0];
-#pragma unroll
-        for (int e = 1; e < 15; e += 2) top = max3(top, x[e], x[e + 1]);
-        top = row_group_max(max2(top, x[15]));
-        if (__builtin_amdgcn_ballot_w64(top > m[rt] + kSlack)) {  // m = -inf at first
-          const float mn = fmaxf(m[rt], top);
-          const float c = mn == -INFINITY ? 1.f : fast_exp2(m[rt] - mn);
-          m[rt] = mn;
-          l[rt] *= c;
-#pragma unroll
-          for (int dt = 0; dt < NDT; ++dt) o[dt][rt] *= c;
-        }
-        const float base = m[rt] == -INFINITY ? 0.f : m[rt];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          x[e] = fast_exp2(x[e] - base);
-          l[rt] += x[e];
-        }
-        // P is rounded to the inputs' type for the matrix unit, as in the paged prefill: at most half a
-        // step of each weight, while l sums the unrounded ones in 32 bits.
-#pragma unroll
-        for (int e = 0; e < 8; ++e) pb[rt][e >> 2][e & 3] = pack2(x[2 * e], x[2 * e + 1], Tag{});
       }
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the stage is read
+      if (t + 2 < t1) issue(t + 2, (t - t0) & 1);
+    }
+
+    const bool complete = t0 == 0 && t1 == tiles;
+    const int64_t part = (int64_t(run) * 2 + (p == start ? 0 : 1)) * kRows + wave * 32 + n;
 #pragma unroll
-      for (int kp = 0; kp < 2; ++kp) {
+    for (int rt = 0; rt < 2; ++rt) {
+      const int r = wrow + rt * 16 + n;
+      const float lt = row_group_sum(l[rt]);
+      if (r >= sq.q_len) continue;
+      if (!BALANCED || complete) {
+        const float inv = lt != 0.f ? 1.f / lt : 0.f;  // a row that sees nothing is zero
+        uint16_t* dst = a.out + int64_t(sq.q0 + r) * a.o_st + h * a.o_sh + 4 * g;
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) {
-          const uint16_t* at = tile + v_at[dt] + 32 * kp * ROW;
-          const u32x2 lo = lds_read_tr4(at), hi = lds_read_tr4(at + 16 * ROW);
-          const u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
-#pragma unroll
-          for (int rt = 0; rt < 2; ++rt) o[dt][rt] = mfma16x16x32(v, pb[rt][kp], o[dt][rt], Tag{});
+          const f32x4 y = o[dt][rt] * inv;
+          *reinterpret_cast<u32x2*>(dst + 16 * dt) = u32x2{pack2(y[0], y[1], Tag{}), pack2(y[2], y[3], Tag{})};
         }
+      } else {
+        float* dst = a.part_o + (part + 16 * rt) * DN + 4 * g;
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<f32x4*>(dst + 16 * dt) = o[dt][rt];
+        if (g == 0) *reinterpret_cast<float2*>(a.part_ml + (part + 16 * rt) * 2) = make_float2(m[rt], lt);
       }
     }
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the stage is read
-    if (t + 2 < nt) issue(t + 2, t & 1);
+    if constexpr (!BALANCED) return;
+    p += uint32_t(t1 - t0);
+    if (p >= end) return;
+    // The next unit that has tiles: the run holds more of them, so there is one.
+    t_first = 0;
+    do {
+      if (++qb >= Seq(a, b).blocks) {
+        qb = 0;
+        do {
+          if (++b == a.batch) {
+            b = 0;
+            ++h;
+          }
+        } while (Seq(a, b).blocks == 0);
+      }
+    } while (Seq(a, b).tiles(qb) == 0);
   }
-#pragma unroll
-  for (int rt = 0; rt < 2; ++rt) {
-    const int r = wrow + rt * 16 + n;
-    const float lt = row_group_sum(l[rt]);
-    if (r >= q_len) continue;
-    const float inv = lt != 0.f ? 1.f / lt : 0.f;  // a row that sees nothing is zero
-    uint16_t* dst = a.out + int64_t(q0 + r) * a.o_st + h * a.o_sh + 4 * g;
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) {
-      const f32x4 y = o[dt][rt] * inv;
-      *reinterpret_cast<u32x2*>(dst + 16 * dt) = u32x2{pack2(y[0], y[1], Tag{}), pack2(y[2], y[3], Tag{})};
+}
+
+// Joins the parts of units that several runs share, in the order of the runs, and writes zeros for rows that see
+// nothing: one workgroup for 16 rows of a unit.
+template <int DN, typename Tag>
+__global__ __launch_bounds__(256) void latent_prefill_merge_kernel(ExpandedArgs a) {
+  constexpr int COLS = DN / 4;          // threads of a row
+  constexpr int PAR = 256 / COLS;       // rows at a time
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int qb = int(blockIdx.x) / (kRows / 16), r0 = int(blockIdx.x) % (kRows / 16) * 16;
+  const Seq s(a, b);
+  if (qb >= s.blocks || qb * kRows + r0 >= s.q_len) return;
+  const int nt = s.tiles(qb);
+  const int col = threadIdx.x % COLS;
+  const uint32_t per_head = uint32_t(a.seq_tile[a.batch]);
+  int parts = 0;
+  int64_t row_first = 0, row_next = 0;
+  if (nt > 0) {
+    const Runs runs(a, per_head * a.heads);
+    const uint32_t u0 = uint32_t(h) * per_head + uint32_t(a.seq_tile[b] + s.before(qb));
+    const uint32_t i0 = runs.holding(u0), i1 = runs.holding(u0 + nt - 1);
+    if (i0 == i1) return;  // written by its run
+    parts = int(i1 - i0) + 1;
+    // Part i0 is that run's first one (slot 0) if the unit begins with the run, else its last (slot 1).
+    row_first = (int64_t(i0) * 2 + (runs.start(i0) == u0 ? 0 : 1)) * kRows;
+    row_next = int64_t(i0) * 2 * kRows;
+  }
+  auto part = [&](int i) { return i == 0 ? row_first : row_next + int64_t(i) * 2 * kRows; };
+  for (int k = threadIdx.x / COLS; k < 16; k += PAR) {
+    const int rr = r0 + k, r = qb * kRows + rr;
+    if (r >= s.q_len) break;
+    float top = -INFINITY;
+    for (int i = 0; i < parts; ++i) top = fmaxf(top, a.part_ml[(part(i) + rr) * 2]);
+    const float base = top == -INFINITY ? 0.f : top;
+    f32x4 o = {};
+    float l = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) {
+      const int64_t at = part(i) + rr;
+      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
+      const float c = fast_exp2(ml.x - base);
+      l += c * ml.y;
+      o += c * *reinterpret_cast<const f32x4*>(a.part_o + at * DN + 4 * col);
     }
+    o *= l != 0.f ? 1.f / l : 0.f;
+    uint16_t* dst = a.out + int64_t(s.q0 + r) * a.o_st + h * a.o_sh + 4 * col;
+    *reinterpret_cast<u32x2*>(dst) = u32x2{pack2(o[0], o[1], Tag{}), pack2(o[2], o[3], Tag{})};
   }
 }
 
@@ -241,15 +446,63 @@ bool vec_rows(const void* p, int64_t st, int64_t sh) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && st % 8 == 0 && sh % 8 == 0;
 }
 
+struct PrefillSizes {
+  int32_t runs;
+  int64_t o_floats, ml_floats, bytes;
+};
+
+// The balanced schedule's runs and workspace; 0 where the call takes one workgroup per unit. Cutting units
+// costs their parts' way through memory and a second launch, so it is for calls whose units do not fill the
+// CUs: 1,024 queries over 9,216 keys with 24 heads (192 units) 167 us against 225 per unit, but a first chunk
+// of 2,048 (384 units) 76 against 66 and 24 prompts of 17 to 700 (1,800 units) 116 against 72.
+PrefillSizes prefill_sizes(int32_t batch, int32_t total_q, int32_t total_k, int32_t heads, int32_t head_dim) {
+  PrefillSizes z{};
+  const int64_t cus = device_cu_count(), slots = 2 * cus, blocks = ceil_div(total_q, kRows);
+  const int64_t most = (blocks + batch) * (ceil_div(total_k, kKeys) + 1) * heads;  // tiles at most
+  if (blocks * heads > cus || most > INT32_MAX) return z;
+  z.runs = int32_t(slots);
+  z.o_floats = slots * 2 * kRows * head_dim;
+  z.ml_floats = slots * 2 * kRows * 2;
+  z.bytes = ((z.o_floats + z.ml_floats + batch + 1) * 4 + 15) & ~int64_t(15);
+  return z;
+}
+
+template <int DN, typename Tag>
+void launch_prefill(const ExpandedArgs& a, int64_t longest, hipStream_t s) {
+  const unsigned blocks = unsigned(ceil_div(longest, kRows));
+  const unsigned heads = unsigned(a.heads), batch = unsigned(a.batch);
+  if (a.runs == 0) {
+    hipLaunchKernelGGL((latent_prefill_kernel<DN, false, Tag>), dim3(heads, blocks, batch), dim3(256), 0, s, a);
+    return;
+  }
+  hipLaunchKernelGGL((latent_prefill_kernel<DN, true, Tag>), dim3(unsigned(a.runs)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((latent_prefill_merge_kernel<DN, Tag>), dim3(blocks * (kRows / 16), heads, batch), dim3(256), 0,
+                     s, a);
+}
+
 }  // namespace
 }  // namespace ti
+
+extern "C" int ti_latent_prefill_workspace_bytes(int32_t batch, int32_t total_q, int32_t total_k,
+                                                 int32_t num_heads, int32_t head_dim,
+                                                 int64_t* workspace_bytes_out) {
+  using namespace ti;
+  const char* who = "ti_latent_prefill_workspace_bytes";
+  if (batch < 0 || total_q < 0 || total_k < 0 || num_heads <= 0 || (head_dim != 128 && head_dim != 64)) {
+    return fail(TI_EINVAL, "%s: bad sizes batch=%d total_q=%d total_k=%d heads=%d head_dim=%d", who, batch, total_q,
+                total_k, num_heads, head_dim);
+  }
+  if (!workspace_bytes_out) return fail(TI_EINVAL, "%s: null output", who);
+  *workspace_bytes_out = batch == 0 || total_q == 0 ? 0 : prefill_sizes(batch, total_q, total_k, num_heads, head_dim).bytes;
+  return TI_OK;
+}
 
 extern "C" int ti_latent_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* kv,
                                  int64_t kv_stride_t, int64_t kv_stride_h, const void* key_rope,
                                  int64_t key_stride_t, const int32_t* cu_seqlens_q,
                                  const int32_t* cu_seqlens_k, void* out, int64_t out_stride_t,
-                                 int64_t out_stride_h, int32_t batch, int32_t total_q, int32_t total_k,
-                                 int32_t max_seqlen_q, int32_t num_heads, int32_t head_dim,
+                                 int64_t out_stride_h, void* workspace, int64_t workspace_bytes,
+                                 int32_t batch, int32_t total_q, int32_t total_k, int32_t max_seqlen_q, int32_t num_heads, int32_t head_dim,
                                  int32_t rope_dim, int32_t causal, float scale, int32_t dtype,
                                  void* stream) {
   using namespace ti;
@@ -275,6 +528,7 @@ extern "C" int ti_latent_prefill(const void* q, int64_t q_stride_t, int64_t q_st
     return fail(TI_EINVAL, "%s: rows must be 16-byte aligned", who);
   }
   // A tile's rows are reached by 32-bit offsets.
+  if (!(scale >= 0.f)) return fail(TI_EINVAL, "%s: scale %g is negative", who, double(scale));
   if (kv_stride_t < 0 || key_stride_t < 0 || kv_stride_t >= (1 << 24) || key_stride_t >= (1 << 24)) {
     return fail(TI_EINVAL, "%s: token strides %lld, %lld of kv and key_rope must be in [0, 2^24)", who,
                 static_cast<long long>(kv_stride_t), static_cast<long long>(key_stride_t));
@@ -297,17 +551,29 @@ extern "C" int ti_latent_prefill(const void* q, int64_t q_stride_t, int64_t q_st
   a.total_k = total_k;
   a.causal = causal;
   a.scale_log2 = scale * 1.4426950408889634f;
+  a.batch = batch;
+  a.heads = num_heads;
+  const PrefillSizes z = prefill_sizes(batch, total_q, total_k, num_heads, head_dim);
+  if (workspace && z.bytes > 0) {
+    if (workspace_bytes < z.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15)) {
+      return fail(TI_EINVAL, "%s: workspace %lld < %lld bytes, or not 16-byte aligned", who,
+                  static_cast<long long>(workspace_bytes), static_cast<long long>(z.bytes));
+    }
+    a.runs = z.runs;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + z.o_floats;
+    a.seq_tile = reinterpret_cast<int32_t*>(a.part_ml + z.ml_floats);
+  }
   const int64_t longest = max_seqlen_q < total_q ? max_seqlen_q : total_q;
-  const dim3 grid(unsigned(num_heads), unsigned(ceil_div(longest, kRows)), unsigned(batch));
-  if (grid.y > 65535) return fail(TI_EINVAL, "%s: max_seqlen_q %d too long", who, max_seqlen_q);
+  if (ceil_div(longest, kRows) > 65535) return fail(TI_EINVAL, "%s: max_seqlen_q %d too long", who, max_seqlen_q);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool bf16 = dtype == TI_DTYPE_BF16;
   if (head_dim == 128) {
-    if (bf16) hipLaunchKernelGGL((latent_prefill_kernel<128, Bf16>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((latent_prefill_kernel<128, F16>), grid, dim3(256), 0, s, a);
+    if (bf16) launch_prefill<128, Bf16>(a, longest, s);
+    else launch_prefill<128, F16>(a, longest, s);
   } else {
-    if (bf16) hipLaunchKernelGGL((latent_prefill_kernel<64, Bf16>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((latent_prefill_kernel<64, F16>), grid, dim3(256), 0, s, a);
+    if (bf16) launch_prefill<64, Bf16>(a, longest, s);
+    else launch_prefill<64, F16>(a, longest, s);
   }
   return check_launch(who);
 }

@@ -216,6 +216,15 @@ def _paged_args(block_table, seqlen_kv, cache, page_size, b, dev):
     return block_table, seqlen_kv.contiguous(), rows, page_size
 
 
+@functools.lru_cache(maxsize=256)
+def _prefill_workspace(batch: int, total_q: int, total_k: int, heads: int, d: int, device: int) -> int:
+    """Bytes for these sizes on this GPU (its number of CUs counts)."""
+    nbytes = ctypes.c_int64(0)
+    _lib.check(_lib.load().ti_latent_prefill_workspace_bytes(batch, total_q, total_k, heads, d,
+                                                             ctypes.byref(nbytes)))
+    return nbytes.value
+
+
 def latent_prefill_fn(q: torch.Tensor, kv: torch.Tensor, key_rope: torch.Tensor,
                       cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor, max_seqlen_q: int, *,
                       causal: bool = True, scale: float | None = None,
@@ -266,6 +275,9 @@ def latent_prefill_fn(q: torch.Tensor, kv: torch.Tensor, key_rope: torch.Tensor,
     max_seqlen_q = int(max_seqlen_q)
     if max_seqlen_q < 0:
         raise ValueError(f"max_seqlen_q {max_seqlen_q} is negative")
+    scale = row ** -0.5 if scale is None else float(scale)
+    if not scale >= 0:
+        raise ValueError(f"scale {scale} is negative")
     if out is None:
         out = torch.empty((total_q, h, d), dtype=dt, device=dev)
     elif out.shape != (total_q, h, d) or out.dtype != dt or out.device != dev or not _vec_rows(out):
@@ -274,12 +286,14 @@ def latent_prefill_fn(q: torch.Tensor, kv: torch.Tensor, key_rope: torch.Tensor,
     if total_q == 0 or b == 0:
         return out
     q, kv, key_rope = _as_rows(q), _as_rows(kv), _as_rows(key_rope)
-    scale = row ** -0.5 if scale is None else float(scale)
     with _lib.on(dev):
+        nbytes = _prefill_workspace(b, total_q, total_k, h, d, torch.cuda.current_device())
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         _lib.check(_lib.load().ti_latent_prefill(
             q.data_ptr(), q.stride(0), q.stride(1), kv.data_ptr(), kv.stride(0), kv.stride(1),
             key_rope.data_ptr(), key_rope.stride(0), cu_seqlens_q.contiguous().data_ptr(),
-            cu_seqlens_k.contiguous().data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), b,
-            total_q, total_k, max_seqlen_q, h, d, ROPE_DIM, int(bool(causal)), scale, code,
+            cu_seqlens_k.contiguous().data_ptr(), out.data_ptr(), out.stride(0), out.stride(1),
+            None if ws is None else ws.data_ptr(), nbytes, b, total_q,
+            total_k, max_seqlen_q, h, d, ROPE_DIM, int(bool(causal)), scale, code,
             _lib.stream_handle(dev)))
     return out
