@@ -45,18 +45,11 @@ __device__ __forceinline__ u32x2 lds_read_tr4(const uint16_t* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p));
 }
 
-// Maxima without the quieting of NaN operands that fmaxf's other spellings cost (v_max returns the
-// other operand for a quiet NaN, as fmaxf does).
-__device__ __forceinline__ float max2(float x, float y) {
-  float r;
-  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(x), "v"(y));
-  return r;
-}
-__device__ __forceinline__ float max3(float x, float y, float z) {
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
-  return r;
-}
+// Maxima without the quieting of NaN operands that fmaxf costs (v_maximum3 gives a NaN for one). Not as assembly:
+// an accumulator must be some wait states old when an instruction outside the matrix unit reads it, and the
+// compiler counts them only up to instructions that it knows.
+__device__ __forceinline__ float max2(float x, float y) { return __builtin_elementwise_maximum(x, y); }
+__device__ __forceinline__ float max3(float x, float y, float z) { return max2(max2(x, y), z); }
 
 // Max over the four 16-lane rows of the wave (lanes n, n+16, n+32, n+48).
 __device__ __forceinline__ float row_group_max(float x) {
