@@ -12,7 +12,9 @@
 //     beside each workgroup's (max, sum) of every row; a second kernel joins those and adds the weights.
 //     K is read once.
 //   More rows (a window of queries): scores would outweigh K, so they are computed twice: once for the
-//     (max, sum) of every wave and row, joined by a small kernel, and once for the weights.
+//     (max, sum) of every workgroup and row, joined by a small kernel, and once for the weights. A
+//     workgroup's K rows stay in registers while the queries come 32 rows at a time through LDS, the next
+//     ones on their way, so that a wave reads each operand once for all its tokens.
 #include "lds_tiles.h"
 
 namespace ti {
@@ -28,7 +30,7 @@ struct MassArgs {
   float* mass;  // [B, hkv, >= max_blocks * page_size]
   int64_t m_sb, m_sh;
   float* scores;  // [B, hkv, rows][tokens]  (up to 16 rows)
-  float* part;    // [B, hkv][parts][rows][2]  (max, sum) of a part, max in exp2 units
+  float* part;    // [B, hkv][parts][rows][2]  (max, sum) of a workgroup's tokens, max in exp2 units
   float* stats;   // [B, hkv][rows][2]  (max, 1 / sum)  (more than 16 rows)
   int32_t new_tokens, hkv, group, rows, num_blocks32, page_size, max_blocks;
   int32_t parts;   // parts of a sequence of the greatest length
@@ -106,33 +108,31 @@ __device__ __forceinline__ void score_rows(const MassArgs& a, int b, int h, int 
   }
 }
 
-// (max, sum) of each row over the wave's tokens.
+// (max, sum) of each row over the wave's tokens, of scores s * scale (a scale is positive).
 template <int TT>
-__device__ __forceinline__ void row_stats(const float (&s)[TT][4], float& m, float& l) {
-  m = -INFINITY;
+__device__ __forceinline__ void row_stats(const float (&s)[TT][4], float scale, float& m, float& l) {
+  float top = max2(max3(s[0][0], s[0][1], s[0][2]), s[0][3]);
 #pragma unroll
-  for (int tt = 0; tt < TT; ++tt) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) m = max2(m, s[tt][e]);
-  }
-  m = row_group_max(m);
+  for (int tt = 1; tt < TT; ++tt) top = max3(max3(top, s[tt][0], s[tt][1]), s[tt][2], s[tt][3]);
+  top = row_group_max(top);
+  m = top == -INFINITY ? -INFINITY : top * scale;  // nothing seen, whatever the scale
   const float base = m == -INFINITY ? 0.f : m;
-  l = 0.f;
+  float part[4] = {};
 #pragma unroll
   for (int tt = 0; tt < TT; ++tt) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) l += fast_exp2(s[tt][e] - base);
+    for (int e = 0; e < 4; ++e) part[e] += fast_exp2(fmaf(s[tt][e], scale, -base));
   }
-  l = row_group_sum(l);
+  l = row_group_sum((part[0] + part[1]) + (part[2] + part[3]));
 }
 
 // Up to 16 rows: scores of 64 TT tokens a workgroup, and its (max, sum) of every row.
 template <int D, int TT, typename Tag>
 __global__ __launch_bounds__(256) void mass_scores_kernel(MassArgs a) {
   __shared__ float s_ml[4][16][2];
-  const int b = blockIdx.z, h = blockIdx.y;
+  const int b = blockIdx.y, chunk = int(blockIdx.x / unsigned(a.hkv)), h = int(blockIdx.x) - chunk * a.hkv;
   const int len = mass_len(a, b);
-  const int wg0 = int(blockIdx.x) * 64 * TT;
+  const int wg0 = chunk * 64 * TT;
   if (wg0 >= len) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int n = lane & 15, g = lane >> 4;
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(256) void mass_scores_kernel(MassArgs a) {
       }
     }
   }
-  row_stats<TT>(s, m, l);
+  row_stats<TT>(s, 1.f, m, l);
   if (g == 0) {
     s_ml[wave][n][0] = m;
     s_ml[wave][n][1] = l;
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(256) void mass_scores_kernel(MassArgs a) {
     for (int w = 0; w < 4; ++w) top = fmaxf(top, s_ml[w][threadIdx.x][0]);
     const float base = top == -INFINITY ? 0.f : top;
     for (int w = 0; w < 4; ++w) sum += s_ml[w][threadIdx.x][1] * fast_exp2(s_ml[w][threadIdx.x][0] - base);
-    float* dst = a.part + (((int64_t(b) * a.hkv + h) * a.parts + blockIdx.x) * a.rows + threadIdx.x) * 2;
+    float* dst = a.part + (((int64_t(b) * a.hkv + h) * a.parts + chunk) * a.rows + threadIdx.x) * 2;
     dst[0] = top;
     dst[1] = sum;
   }
@@ -227,28 +227,198 @@ __global__ __launch_bounds__(256) void mass_add_kernel(MassArgs a, int part_toke
   }
 }
 
-// More than 16 rows, first pass: (max, sum) of every wave and row.
-template <int D, int TT, typename Tag>
-__global__ __launch_bounds__(256) void mass_stats_kernel(MassArgs a) {
-  const int b = blockIdx.z, h = blockIdx.y;
-  const int len = mass_len(a, b);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int part = int(blockIdx.x) * 4 + wave;
-  const int t0 = part * 16 * TT;
-  if (t0 >= len) return;
-  KeyTile<D, TT> x;
-  load_keys<D, TT>(a, b, h, len, t0, x);
-  float* dst = a.part + ((int64_t(b) * a.hkv + h) * a.parts + part) * a.rows * 2;
-  for (int r0 = 0; r0 < a.rows; r0 += 16) {
-    float s[TT][4], m, l;
-    score_rows<D, TT, Tag>(a, b, h, len, t0, r0, x, s);
-    row_stats<TT>(s, m, l);
-    const int r = r0 + (lane & 15);
-    if (lane < 16 && r < a.rows) {
-      dst[2 * r] = m;
-      dst[2 * r + 1] = l;
+// More than 16 rows: queries through LDS, kQRows at a time in two or three stages. Place of 16-byte chunk c of row r: c ^
+// its swizzle, so that the operand reads (16 rows of a chunk and its neighbour) hit every bank quad once;
+// rows of whole 256-byte blocks start on the same bank, the others 32 banks apart.
+constexpr int kQRows = 32;
+
+template <int D>
+__device__ __forceinline__ int q_place(int r) {
+  if constexpr (D % 128 == 0) return ((2 * r) & 15) ^ ((r & 8) ? 9 : 0);
+  const int u = (r >> 1) & 7;
+  return ((2 * u) & 7) ^ ((u & 4) ? 5 : 0);
+}
+
+// STATS: the rows' (max, 1 / sum) come too, behind the queries, a copy for each wave.
+template <int D, bool STATS>
+struct QueryStages {
+  static constexpr int CH = D / 8, QLOADS = kQRows * CH / 256, LOADS = QLOADS + (STATS ? 1 : 0);
+  static constexpr int STAGE = kQRows * D + (STATS ? 4 * kQRows * 4 : 0);  // 16-bit elements
+  static constexpr int STAGES = D <= 320 ? 3 : 2;  // three: one barrier a block
+
+  // This lane's part of the loads, block after block: address and place in the group of its rows. They advance
+  // without a division or a product, which would take as long as the block's scores.
+  const uint16_t* at[QLOADS];
+  int head[QLOADS];
+  const uint16_t* first;
+  const float* stats;
+  int next = 0;  // first row of the block to load next
+  int64_t step, wrap;
+  int step_heads, lane, wave;
+
+  __device__ __forceinline__ QueryStages(const MassArgs& a, int b, int h)
+      : lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {
+    first = a.q + b * a.q_sb + int64_t(h) * a.group * a.q_sh;
+    stats = STATS ? a.stats + (int64_t(b) * a.hkv + h) * a.rows * 2 : nullptr;
+    const int toks = kQRows / a.group;
+    step_heads = kQRows - toks * a.group;
+    step = toks * a.q_st + step_heads * a.q_sh;
+    wrap = a.q_st - a.group * a.q_sh;
+#pragma unroll
+    for (int i = 0; i < QLOADS; ++i) {
+      const int f = (wave * QLOADS + i) * 64 + lane, row = f / CH;
+      const int tok = row / a.group;
+      head[i] = row - tok * a.group;
+      at[i] = first + tok * a.q_st + head[i] * a.q_sh + 8 * ((f % CH) ^ q_place<D>(row));
     }
   }
+
+  // The next kQRows queries of the group into a stage; in place of rows behind the last, its first one.
+  __device__ __forceinline__ void issue(const MassArgs& a, uint16_t* stage) {
+#pragma unroll
+    for (int i = 0; i < QLOADS; ++i) {
+      const int f = (wave * QLOADS + i) * 64 + lane;
+      const uint16_t* src = next + f / CH < a.rows ? at[i] : first + 8 * (f % CH);
+      const uint32_t m0 = uint32_t(reinterpret_cast<uintptr_t>((lds_ptr_t)(stage + (wave * QLOADS + i) * 512)));
+      asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(m0) : "memory");
+      head[i] += step_heads;
+      const bool over = head[i] >= a.group;
+      at[i] += step + (over ? wrap : 0);
+      head[i] -= over ? a.group : 0;
+    }
+    if constexpr (STATS) {
+      static_assert(2 * kQRows == 64);
+      const float* src = stats + min(2 * next + lane, 2 * a.rows - 1);
+      const uint32_t m0 = uint32_t(reinterpret_cast<uintptr_t>((lds_ptr_t)(stage + kQRows * D + wave * 128)));
+      asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "{m0}"(m0) : "memory");
+    }
+    next += kQRows;
+  }
+
+  // Products of the wave's tokens and rows r0 + 16 rt + n, -inf where the row does not see the token. whole: every
+  // token exists and every row sees it.
+  template <int TT, typename Tag>
+  static __device__ __forceinline__ void scores(const MassArgs& a, int len, int t0, int r0, int rt, bool whole,
+                                                const uint16_t* stage, const KeyTile<D, TT>& x,
+                                                float (&s)[TT][4]) {
+    const int lane = threadIdx.x & 63;
+    const int n = lane & 15, g = lane >> 4;
+    u32x4 q[D / 32];
+#pragma unroll
+    for (int kk = 0; kk < D / 32; ++kk) {
+      q[kk] = *reinterpret_cast<const u32x4*>(stage + (16 * rt + n) * D + 8 * ((4 * kk + g) ^ q_place<D>(n)));
+    }
+    f32x4 acc[TT];
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) acc[tt] = f32x4{};
+#pragma unroll
+    for (int kk = 0; kk < D / 32; ++kk) {
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) acc[tt] = mfma16x16x32(x.k[tt][kk], q[kk], acc[tt], Tag{});
+    }
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[tt][e] = acc[tt][e];
+    }
+    const int r = r0 + 16 * rt + n;
+    if (!whole || r0 + kQRows > a.rows) {  // uniform
+      const int last = r < a.rows ? len - a.new_tokens + r / a.group : -1;
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = 4 * g + e;
+          if (!((x.there[tt] >> j) & 1) || t0 + 16 * tt + j > last) s[tt][e] = -INFINITY;
+        }
+      }
+    }
+  }
+
+  // Calls f(i, r0, stage) for every block of queries, the next ones on their way; past(i) behind the barrier
+  // that ends block i.
+  template <typename F, typename P>
+  __device__ __forceinline__ void for_blocks(const MassArgs& a, uint16_t* stages, F f, P past) {
+    issue(a, stages);
+    if (kQRows < a.rows) issue(a, stages + STAGE);
+    // The keys (and whatever else the compiler knows of) have landed, so that it places no wait of its own,
+    // which would also wait for the stage in flight, in the loop.
+    __builtin_amdgcn_s_waitcnt(0);
+    int stage = 0;
+    const int blocks = (a.rows + kQRows - 1) / kQRows;
+    for (int i = 0; i < blocks; ++i) {
+      if (i + 1 < blocks) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (STAGES == 3 && i + 2 < blocks) {  // the stage of block i - 1 is read
+        issue(a, stages + (stage == 0 ? 2 : stage - 1) * STAGE);
+      }
+      if (i > 0) past(i - 1);
+      f(i, i * kQRows, stages + stage * STAGE);
+      if (STAGES == 2) {
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (i + 2 < blocks) issue(a, stages + stage * STAGE);
+      }
+      stage = stage == STAGES - 1 ? 0 : stage + 1;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    past(blocks - 1);
+  }
+};
+
+// Whether every token of the wave's tiles exists and every query sees it (uniform).
+template <int D, int TT>
+__device__ __forceinline__ bool all_seen(const MassArgs& a, int len, int t0, const KeyTile<D, TT>& x) {
+  uint32_t all = 0xffffu;
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt) all &= x.there[tt];
+  return all == 0xffffu && t0 + 16 * TT <= len - a.new_tokens + 1;
+}
+
+// Waves of a SIMD: what the K rows leave of the registers. They are what hides a workgroup's start (its blocks'
+// ids, then its keys): 32 queries of 32/8 heads of 128 over 4 x U[2k, 16k] tokens, both passes, 92 us with
+// three of 64 tokens each, 67 with five of 32.
+constexpr int mass_waves(int d) { return d <= 128 ? 5 : d <= 256 ? 3 : 2; }
+
+// First pass: (max, sum) of every workgroup and row.
+template <int D, int TT, typename Tag>
+__global__ __launch_bounds__(256, mass_waves(D)) void mass_stats_kernel(MassArgs a) {
+  using Q = QueryStages<D, false>;
+  __shared__ __align__(16) uint16_t s_q[Q::STAGES * Q::STAGE];
+  __shared__ float2 s_ml[2][4][kQRows];
+  const int b = blockIdx.y, chunk = int(blockIdx.x / unsigned(a.hkv)), h = int(blockIdx.x) - chunk * a.hkv;
+  const int len = mass_len(a, b);
+  if (chunk * 64 * TT >= len) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t0 = (chunk * 4 + wave) * 16 * TT;
+  Q queries(a, b, h);
+  KeyTile<D, TT> x;
+  load_keys<D, TT>(a, b, h, len, t0, x);
+  const bool whole = all_seen<D, TT>(a, len, t0, x);
+  float2* dst = reinterpret_cast<float2*>(a.part) + ((int64_t(b) * a.hkv + h) * a.parts + chunk) * a.rows;
+  queries.for_blocks(
+      a, s_q,
+      [&](int i, int r0, const uint16_t* stage) {
+#pragma unroll
+        for (int rt = 0; rt < kQRows / 16; ++rt) {
+          float s[TT][4], m, l;
+          Q::template scores<TT, Tag>(a, len, t0, r0, rt, whole, stage, x, s);
+          row_stats<TT>(s, a.scale_log2, m, l);
+          if (lane < 16) s_ml[i & 1][wave][16 * rt + lane] = make_float2(m, l);
+        }
+      },
+      [&](int i) {  // the waves' parts are there
+        const int r = i * kQRows + lane;
+        if (wave != (i & 3) || lane >= kQRows || r >= a.rows) return;
+        float2 ml[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) ml[w] = s_ml[i & 1][w][lane];
+        const float top = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));
+        const float base = top == -INFINITY ? 0.f : top;
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) sum += ml[w].y * fast_exp2(ml[w].x - base);
+        dst[r] = make_float2(top, sum);
+      });
 }
 
 __global__ __launch_bounds__(256) void mass_join_kernel(MassArgs a, int part_tokens) {
@@ -268,44 +438,63 @@ __global__ __launch_bounds__(256) void mass_join_kernel(MassArgs a, int part_tok
 
 // Second pass: the weights, added to the sums.
 template <int D, int TT, typename Tag>
-__global__ __launch_bounds__(256) void mass_weights_kernel(MassArgs a) {
-  const int b = blockIdx.z, h = blockIdx.y;
+__global__ __launch_bounds__(256, mass_waves(D)) void mass_weights_kernel(MassArgs a) {
+  using Q = QueryStages<D, true>;
+  __shared__ __align__(16) uint16_t s_q[Q::STAGES * Q::STAGE];
+  const int b = blockIdx.y, chunk = int(blockIdx.x / unsigned(a.hkv)), h = int(blockIdx.x) - chunk * a.hkv;
   const int len = mass_len(a, b);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (chunk * 64 * TT >= len) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
-  const int t0 = (int(blockIdx.x) * 4 + wave) * 16 * TT;
-  if (t0 >= len) return;
+  const int t0 = (chunk * 4 + wave) * 16 * TT;
+  Q queries(a, b, h);
   KeyTile<D, TT> x;
   load_keys<D, TT>(a, b, h, len, t0, x);
-  const float* stats = a.stats + (int64_t(b) * a.hkv + h) * a.rows * 2;
+  const bool whole = all_seen<D, TT>(a, len, t0, x);
   float w[TT][4] = {};
-  for (int r0 = 0; r0 < a.rows; r0 += 16) {
-    float s[TT][4];
-    score_rows<D, TT, Tag>(a, b, h, len, t0, r0, x, s);
-    const int r = min(r0 + n, a.rows - 1);
-    const float m = stats[2 * r], inv = stats[2 * r + 1];
+  queries.for_blocks(a, s_q, [&](int, int r0, const uint16_t* stage) {
 #pragma unroll
-    for (int tt = 0; tt < TT; ++tt) {
+    for (int rt = 0; rt < kQRows / 16; ++rt) {
+      float s[TT][4];
+      Q::template scores<TT, Tag>(a, len, t0, r0, rt, whole, stage, x, s);
+      const float2 ml = reinterpret_cast<const float2*>(stage + kQRows * D + wave * 128)[16 * rt + n];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[tt][e] += fast_exp2(s[tt][e] - m) * inv;
+      for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          w[tt][e] = fmaf(fast_exp2(fmaf(s[tt][e], a.scale_log2, -ml.x)), ml.y, w[tt][e]);
+        }
+      }
+    }
+  }, [](int) {});
+  // The 16 lanes of a group hold 4 TT tokens' sums over their own rows: halves change hands until every lane has
+  // one token's (or one of 16 / (4 TT) copies of it), v[0] of token 16 (i / 4) + 4 g + i % 4, i the bits of n.
+  float v[4 * TT];
+#pragma unroll
+  for (int i = 0; i < 4 * TT; ++i) v[i] = w[i >> 2][i & 3];
+#pragma unroll
+  for (int half = 2 * TT, d = 8; d > 0; half >>= 1, d >>= 1) {
+    if (half > 0) {
+      const bool up = n & d;
+#pragma unroll
+      for (int i = 0; i < half; ++i) {
+        const float mine = up ? v[i + half] : v[i], other = up ? v[i] : v[i + half];
+        v[i] = mine + __shfl_xor(other, d, 64);
+      }
+    } else {
+      v[0] += __shfl_xor(v[0], d, 64);
     }
   }
-  float* dst = a.mass + b * a.m_sb + h * a.m_sh;
-#pragma unroll
-  for (int tt = 0; tt < TT; ++tt) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float y = w[tt][e];
-#pragma unroll
-      for (int d = 1; d < 16; d <<= 1) y += __shfl_xor(y, d, 64);
-      const int t = t0 + 16 * tt + 4 * g + e;
-      if (n == 0 && t < len) dst[t] += y;
-    }
-  }
+  const int i = n / (4 / TT);
+  const int t = t0 + 16 * (i >> 2) + 4 * g + (i & 3);
+  if (n % (4 / TT) == 0 && t < len) a.mass[b * a.m_sb + h * a.m_sh + t] += v[0];
 }
 
 // 16-token tiles of a wave: what its K rows leave of the registers.
-constexpr int tiles_of(int d) { return d <= 128 ? 4 : 2; }
+// (Few rows, us with 1 / 2 / 4: a step of 16 x U[512, 8k] tokens, 24/4 heads of 256, 43.8 / 43.5 / 46.9, one of
+// 8,000 14.7 / 14.0 / 16.0, 16 x 4,000 latent rows 30.6 / 27.3 / 27.1. 32 queries over 4 x 4,000 latent rows:
+// 89 with 1 against 134 with 2, whose query addresses no longer fit the registers.)
+constexpr int tiles_of(int d, bool few) { return few || d <= 320 ? 2 : 1; }
 
 struct MassSizes {
   int32_t part_tokens, parts;
@@ -315,7 +504,7 @@ struct MassSizes {
 MassSizes mass_sizes(int32_t batch, int32_t hkv, int32_t rows, int32_t d, int64_t tokens) {
   MassSizes s;
   const bool few = rows <= kFewRows;
-  s.part_tokens = 16 * tiles_of(d) * (few ? 4 : 1);
+  s.part_tokens = 64 * tiles_of(d, few);
   s.parts = int32_t(ceil_div(tokens, s.part_tokens));
   s.tokens = ceil_div(tokens, 4) * 4;
   const int64_t bh = int64_t(batch) * hkv;
@@ -335,7 +524,8 @@ int check_mass(const char* who, int32_t batch, int32_t new_tokens, int32_t hq, i
       int64_t(new_tokens) * (hq / hkv) > (1 << 20)) {
     return fail(TI_EINVAL, "%s: bad sizes batch=%d new_tokens=%d heads=%d/%d", who, batch, new_tokens, hq, hkv);
   }
-  if (page_size <= 0 || max_blocks < 0 || int64_t(max_blocks) * page_size > INT32_MAX - 1024) {
+  if (page_size <= 0 || max_blocks < 0 || int64_t(max_blocks) * page_size > INT32_MAX - 1024 ||
+      ceil_div(int64_t(max_blocks) * page_size, 64) * hkv > INT32_MAX) {
     return fail(TI_EINVAL, "%s: bad cache page_size=%d max_blocks_per_seq=%d", who, page_size, max_blocks);
   }
   return TI_OK;
@@ -343,15 +533,16 @@ int check_mass(const char* who, int32_t batch, int32_t new_tokens, int32_t hq, i
 
 template <int D, typename Tag>
 void launch_mass(const MassArgs& a, const MassSizes& sz, unsigned batch, hipStream_t s) {
-  constexpr int TT = tiles_of(D);
   const unsigned hkv = unsigned(a.hkv);
-  const dim3 grid(unsigned(ceil_div(a.tokens, 64 * TT)), hkv, batch);
+  // The heads of a token range follow each other: together they read whole rows of the cache.
+  const dim3 grid(unsigned(ceil_div(a.tokens, sz.part_tokens)) * hkv, batch);
   if (a.rows <= kFewRows) {
-    hipLaunchKernelGGL((mass_scores_kernel<D, TT, Tag>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((mass_scores_kernel<D, tiles_of(D, true), Tag>), grid, dim3(256), 0, s, a);
     hipLaunchKernelGGL(mass_add_kernel, dim3(unsigned(ceil_div(a.tokens, kAddTokens)), hkv, batch), dim3(256), 0,
                        s, a, sz.part_tokens);
     return;
   }
+  constexpr int TT = tiles_of(D, false);
   hipLaunchKernelGGL((mass_stats_kernel<D, TT, Tag>), grid, dim3(256), 0, s, a);
   hipLaunchKernelGGL(mass_join_kernel, dim3(unsigned(ceil_div(a.rows, 16)), hkv, batch), dim3(256), 0, s, a,
                      sz.part_tokens);
@@ -396,6 +587,7 @@ extern "C" int ti_cache_mass(const void* q, int64_t q_stride_b, int64_t q_stride
   }
   int rc = check_mass(who, batch, new_tokens, num_q_heads, num_kv_heads, head_dim, page_size, max_blocks_per_seq);
   if (rc != TI_OK) return rc;
+  if (!(scale > 0.f)) return fail(TI_EINVAL, "%s: scale %g is not positive", who, double(scale));
   if (num_blocks < 0 || num_blocks > INT32_MAX) {
     return fail(TI_EINVAL, "%s: bad cache num_blocks=%lld", who, static_cast<long long>(num_blocks));
   }
