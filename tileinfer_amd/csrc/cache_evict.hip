@@ -5,10 +5,12 @@
 //   and the head's K (and V) row of token kept[j] is copied to slot j of the sequence's new block table.
 // Heads of one sequence keep different tokens, all the same number. A bit copy; no arithmetic on values.
 //
-// Selection (one workgroup per (sequence, KV head)): masses become unsigned keys of the same order, the
-// budget-th largest key is found digit by digit (11, 11 and 10 bits, a histogram in LDS each), then each
-// wave walks a contiguous range of positions and numbers the kept ones by ballots, so the order is the
-// positions'. Bound: the latency of four passes over the masses, which stay in L2 after the first.
+// Selection (one workgroup per (sequence, KV head)): masses become unsigned keys of the same order, held in
+// registers (up to 32,768 tokens; longer sequences read theirs again for every pass), the budget-th largest
+// key is found digit by digit (11, 11 and 10 bits, a histogram in LDS each), then each wave walks a
+// contiguous range of positions and numbers the kept ones by ballots, so the order is the positions'. Summed
+// weights have few exponents and many zeros, so a histogram has four copies of each bin, for lanes of
+// different remainders. Bound: the latency of its passes, and of LDS atomics on the same bins.
 // Copy: every 16-byte vector of the new rows by one lane. Bound: HBM.
 #include "decode_common.h"
 
@@ -42,21 +44,39 @@ __device__ __forceinline__ int evict_len(const EvictArgs& a, int b) {
   return int64_t(n) > cap ? int(cap) : n;
 }
 
-// Unsigned keys in the order of the ranks: tokens always kept first, then by mass (-0 as 0), NaN last.
-__device__ __forceinline__ uint32_t rank_key(const EvictArgs& a, const float* mass, int t, int n) {
-  if (t < a.sinks || t >= n - a.recent) return 0xffffffffu;
-  const float x = mass[t] + 0.f;
+// Unsigned keys in the order of the ranks: tokens always kept first, then by mass (-0 as 0), NaN last. Zero is
+// none of them: it stands for no token.
+__device__ __forceinline__ uint32_t rank_key(const EvictArgs& a, float mass, int t, int n) {
+  const float x = mass + 0.f;
   const uint32_t u = __float_as_uint(x);
-  if (x != x) return 0u;
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  const uint32_t key = x != x ? 1u : u & 0x80000000u ? ~u : u | 0x80000000u;
+  return t < a.sinks || t >= n - a.recent ? 0xffffffffu : key;
 }
 
+constexpr int kCopies = 4;   // of every bin
+constexpr int kHeld = 32;    // keys that a thread holds in registers
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+static_assert(kCopies == 4 && kBins == 2 * kThreads);
+
+// Sum over the waves before this one.
+__device__ __forceinline__ int before_wave(const i32x4* of_waves, int wave) {
+  int sum = 0;
+#pragma unroll
+  for (int k = 0; k < kWaves / 4; ++k) {
+    const i32x4 v = of_waves[k];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum += 4 * k + e < wave ? v[e] : 0;
+  }
+  return sum;
+}
+
+template <bool HELD>
 __global__ __launch_bounds__(kThreads) void evict_select_kernel(EvictArgs a) {
-  __shared__ int s_hist[kBins];
-  __shared__ int s_wave[kWaves][2];
+  __shared__ i32x4 s_hist[kBins];
+  __shared__ i32x4 s_wave[2][kWaves / 4];
   __shared__ int s_found[2];
   const int h = blockIdx.x, b = blockIdx.y;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = evict_len(a, b);
   const int keep = min(n, a.budget);
   const int64_t row = int64_t(b) * a.hkv + h;
@@ -64,8 +84,7 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(EvictArgs a) {
   int32_t* kept = a.kept + row * a.budget;
   float* out = a.mass_out + row * a.capacity;
   if (h == 0 && threadIdx.x == 0) a.new_seqlen[b] = keep;
-  for (int j = keep + int(threadIdx.x); j < a.budget; j += kThreads) kept[j] = -1;
-  for (int64_t j = keep + int64_t(threadIdx.x); j < a.capacity; j += kThreads) out[j] = 0.f;
+  if (HELD ? n > kHeld * kThreads : n <= kHeld * kThreads) return;  // the other form's
   if (keep == n) {
     for (int t = threadIdx.x; t < n; t += kThreads) {
       kept[t] = t;
@@ -73,32 +92,69 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(EvictArgs a) {
     }
     return;
   }
+  // Wave w's tokens are [w per, (w + 1) per), 64 a round.
+  const int per = ((n + kWaves - 1) / kWaves + 63) & ~63;
+  const int w0 = min(n, wave * per), w1 = min(n, w0 + per);
+  const int rounds = (w1 - w0 + 63) >> 6;
+  uint32_t keys[HELD ? kHeld : 1];
+  if constexpr (HELD) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      if (i < rounds) {
+        keys[i] = __float_as_uint(mass[min(w0 + 64 * i + lane, n - 1)]);  // all of them in flight
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      if (i < rounds) {
+        const int t = w0 + 64 * i + lane;
+        keys[i] = t < w1 ? rank_key(a, __uint_as_float(keys[i]), t, n) : 0u;
+      }
+    }
+  }
+  // f(round, key) for the wave's tokens; lanes behind its last one have key 0.
+  auto each = [&](auto f) __attribute__((always_inline)) {
+    if constexpr (HELD) {
+      int here = rounds;
+      asm volatile("" : "+s"(here));  // compared anew: 32 conditions kept from pass to pass do not fit the registers
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        if (i < here) f(i, keys[i]);
+      }
+    } else {
+      for (int i = 0; i < rounds; ++i) {
+        const int t = w0 + 64 * i + lane;
+        f(i, t < w1 ? rank_key(a, mass[min(t, n - 1)], t, n) : 0u);
+      }
+    }
+  };
+  s_hist[threadIdx.x] = i32x4{};
+  s_hist[kThreads + threadIdx.x] = i32x4{};
+  __syncthreads();
   // The keep-th largest key: `prefix` is its digits so far, `need` how many of the keys with that prefix
-  // (and the digits to come) are still to be kept.
+  // (and the digits to come) are still to be kept. Digits of 11, 11 and 10 bits. (Lanes without a token fall
+  // into the least bin, behind every token.)
   uint32_t prefix = 0, fixed = 0;
   int need = keep;
-  for (int shift = 21; shift >= 0; shift -= shift == 21 ? 11 : 10) {
-    const uint32_t bins = shift == 0 ? 1024 : 2048;
-    // shifts 21, 10, 0: digits of 11, 11 and 10 bits
-    for (int i = threadIdx.x; i < kBins; i += kThreads) s_hist[i] = 0;
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const uint32_t mask = pass == 2 ? 1023u : 2047u;
+    int* const copy = reinterpret_cast<int*>(s_hist) + (lane & (kCopies - 1));
+    each([&](int, uint32_t key) {
+      if ((key & fixed) == prefix) atomicAdd(copy + ((key >> shift) & mask) * kCopies, 1);
+    });
     __syncthreads();
-    for (int t = threadIdx.x; t < n; t += kThreads) {
-      const uint32_t key = rank_key(a, mass, t, n);
-      if ((key & fixed) == prefix) atomicAdd(&s_hist[(key >> shift) & (bins - 1)], 1);
-    }
+    // Bins from the greatest: thread i holds bins 2 i and 2 i + 1 of that order, and clears them.
+    i32x4* const bins = s_hist + (kBins - 2 - 2 * int(threadIdx.x));
+    const i32x4 l4 = bins[0], h4 = bins[1];
+    bins[0] = i32x4{};
+    bins[1] = i32x4{};
+    const int hi = (h4[0] + h4[1]) + (h4[2] + h4[3]), lo = (l4[0] + l4[1]) + (l4[2] + l4[3]);
+    const int incl = wave_prefix_sum(hi + lo);
+    if (lane == 63) reinterpret_cast<int*>(s_wave[0])[wave] = incl;
     __syncthreads();
-    // Bins from the greatest: thread i holds bins 2 i and 2 i + 1 of that order.
-    const int hi = s_hist[kBins - 1 - 2 * int(threadIdx.x)], lo = s_hist[kBins - 2 - 2 * int(threadIdx.x)];
-    int incl = hi + lo;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int y = __shfl_up(incl, d, 64);
-      if (lane >= d) incl += y;
-    }
-    if (lane == 63) s_wave[wave][0] = incl;
-    __syncthreads();
-    int before = incl - hi - lo;
-    for (int w = 0; w < wave; ++w) before += s_wave[w][0];
+    const int before = incl - hi - lo + before_wave(s_wave[0], wave);
     if (before < need && need <= before + hi) {
       s_found[0] = kBins - 1 - 2 * int(threadIdx.x);
       s_found[1] = need - before;
@@ -108,56 +164,49 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(EvictArgs a) {
     }
     __syncthreads();
     prefix |= uint32_t(s_found[0]) << shift;
-    fixed |= (bins - 1) << shift;
+    fixed |= mask << shift;
     need = s_found[1];
-    if (shift == 0) break;
   }
-  // Kept: keys above `prefix`, and the first `need` that equal it. Each wave numbers a contiguous range.
-  const int per = ((n + kWaves - 1) / kWaves + 63) & ~63;
-  const int w0 = min(n, wave * per), w1 = min(n, w0 + per);
+  // Kept: keys above `prefix`, and the first `need` that equal it.
   int above = 0, equal = 0;
-  for (int t0 = w0; t0 < w1; t0 += 64) {
-    const int t = t0 + lane;
-    const uint32_t key = t < w1 ? rank_key(a, mass, t, n) : 0u;
-    above += __popcll(__builtin_amdgcn_ballot_w64(t < w1 && key > prefix));
-    equal += __popcll(__builtin_amdgcn_ballot_w64(t < w1 && key == prefix));
-  }
+  each([&](int, uint32_t key) {
+    above += __popcll(__builtin_amdgcn_ballot_w64(key > prefix));
+    equal += __popcll(__builtin_amdgcn_ballot_w64(key == prefix));
+  });
   __syncthreads();  // s_wave is read
   if (lane == 0) {
-    s_wave[wave][0] = above;
-    s_wave[wave][1] = equal;
+    reinterpret_cast<int*>(s_wave[0])[wave] = above;
+    reinterpret_cast<int*>(s_wave[1])[wave] = equal;
   }
   __syncthreads();
-  int seen_above = 0, seen_equal = 0;
-  for (int w = 0; w < wave; ++w) {
-    seen_above += s_wave[w][0];
-    seen_equal += s_wave[w][1];
-  }
+  int seen_above = before_wave(s_wave[0], wave), seen_equal = before_wave(s_wave[1], wave);
   const uint64_t below = (uint64_t(1) << lane) - 1;
-  for (int t0 = w0; t0 < w1; t0 += 64) {
-    const int t = t0 + lane;
-    const uint32_t key = t < w1 ? rank_key(a, mass, t, n) : 0u;
-    const bool is_above = t < w1 && key > prefix, is_equal = t < w1 && key == prefix;
-    const uint64_t ma = __builtin_amdgcn_ballot_w64(is_above), me = __builtin_amdgcn_ballot_w64(is_equal);
-    const int eq = seen_equal + __popcll(me & below);
-    if (is_above || (is_equal && eq < need)) {
-      const int j = seen_above + __popcll(ma & below) + min(eq, need);
-      kept[j] = t;
-      out[j] = mass[t];
+  each([&](int i, uint32_t key) {
+    const uint64_t ma = __builtin_amdgcn_ballot_w64(key > prefix), me = __builtin_amdgcn_ballot_w64(key == prefix);
+    if (ma | me) {  // uniform
+      const int eq = seen_equal + __popcll(me & below);
+      if (key > prefix || (key == prefix && eq < need)) {
+        const int j = seen_above + __popcll(ma & below) + min(eq, need), t = w0 + 64 * i + lane;
+        kept[j] = t;
+        out[j] = mass[t];
+      }
+      seen_above += __popcll(ma);
+      seen_equal += __popcll(me);
     }
-    seen_above += __popcll(ma);
-    seen_equal += __popcll(me);
-  }
+  });
 }
 
-// Vectors [16 bytes] of the kept rows of one (sequence, KV head), a grid of them.
+// Vectors [16 bytes] of the kept rows of one (sequence, KV head), a grid of them, and what lies behind the last.
 __global__ __launch_bounds__(256) void evict_copy_kernel(EvictArgs a) {
   const int h = blockIdx.y, b = blockIdx.z;
   const int keep = min(evict_len(a, b), a.budget);
   const int vecs = a.head_dim / 8;
   const int64_t row = int64_t(b) * a.hkv + h;
-  const int64_t total = int64_t(keep) * vecs;
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+  const int64_t total = int64_t(keep) * vecs, first = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t stride = int64_t(gridDim.x) * 256;
+  for (int64_t j = keep + first; j < a.budget; j += stride) a.kept[row * a.budget + j] = -1;
+  for (int64_t j = keep + first; j < a.capacity; j += stride) a.mass_out[row * a.capacity + j] = 0.f;
+  for (int64_t i = first; i < total; i += stride) {
     const int j = int(i / vecs), c = int(i - int64_t(j) * vecs);
     const int t = a.kept[row * a.budget + j];
     const int from = a.block_table[b * a.bt_stride + t / a.page_size];
@@ -242,11 +291,14 @@ extern "C" int ti_evict_kvcache(void* k_cache, void* v_cache, const float* mass,
   a.recent = recent;
   a.capacity = mass_capacity;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(evict_select_kernel, dim3(unsigned(num_kv_heads), unsigned(batch)), dim3(kThreads), 0, s, a);
-  if (most > 0) {
-    const int64_t blocks = ceil_div(most * (head_dim / 8), 256);
-    const dim3 grid(unsigned(blocks < 4096 ? blocks : 4096), unsigned(num_kv_heads), unsigned(batch));
-    hipLaunchKernelGGL(evict_copy_kernel, grid, dim3(256), 0, s, a);
-  }
+  const dim3 sel{unsigned(num_kv_heads), unsigned(batch)};
+  hipLaunchKernelGGL(evict_select_kernel<true>, sel, dim3(kThreads), 0, s, a);
+  if (tokens > kHeld * kThreads) hipLaunchKernelGGL(evict_select_kernel<false>, sel, dim3(kThreads), 0, s, a);
+  int64_t work = most * (head_dim / 8);
+  work = work > budget ? work : budget;
+  work = work > mass_capacity ? work : mass_capacity;
+  const int64_t blocks = ceil_div(work, 256);
+  const dim3 grid(unsigned(blocks < 4096 ? blocks : 4096), unsigned(num_kv_heads), unsigned(batch));
+  hipLaunchKernelGGL(evict_copy_kernel, grid, dim3(256), 0, s, a);
   return check_launch(who);
 }

@@ -85,15 +85,6 @@ struct Runs {
   }
 };
 
-__device__ __forceinline__ int wave_scan(int x, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d, 64);
-    if (lane >= d) x += y;
-  }
-  return x;
-}
-
 // One load of 16 bytes a lane into LDS, from base + off of each lane: lane i's land at byte lds + 16 i.
 // STREAM: with the nt bit, for bytes that are read once.
 template <bool STREAM>
@@ -161,7 +152,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void latent_decode_kernel(LatentArg
   int nt = 0, incl = 0;  // of the last 64 sequences looked at
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     nt = b0 + lane < a.batch ? (latent_len(a, b0 + lane) + kTile - 1) / kTile : 0;
-    incl = wave_scan(nt, lane);
+    incl = wave_prefix_sum(nt);
     if (blockIdx.x == 0 && wave == 0 && b0 + lane < a.batch) a.first_tile[b0 + lane] = int(total) + incl - nt;
     total += uint32_t(__builtin_amdgcn_readlane(incl, 63));
   }
@@ -175,7 +166,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void latent_decode_kernel(LatentArg
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     if (a.batch > 64) {
       nt = b0 + lane < a.batch ? (latent_len(a, b0 + lane) + kTile - 1) / kTile : 0;
-      incl = wave_scan(nt, lane);
+      incl = wave_prefix_sum(nt);
     }
     const uint32_t sum = uint32_t(__builtin_amdgcn_readlane(incl, 63));
     if (unit0 + sum * a.row_blocks > start) {
@@ -613,6 +604,7 @@ extern "C" int ti_latent_decode_paged(const void* q, int64_t q_stride_b, int64_t
   }
   int rc = check_latent(who, batch, new_tokens, num_heads, latent_dim, rope_dim);
   if (rc != TI_OK) return rc;
+  if (!(scale > 0.f)) return fail(TI_EINVAL, "%s: scale %g is not positive", who, double(scale));
   if (page_size <= 0 || num_blocks < 0 || max_blocks_per_seq < 0 ||
       num_blocks * page_size > INT32_MAX) {
     return fail(TI_EINVAL, "%s: bad cache page_size=%d num_blocks=%lld max_blocks_per_seq=%d (at most "

@@ -102,15 +102,6 @@ struct Runs {
   }
 };
 
-__device__ __forceinline__ int wave_scan(int x, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d, 64);
-    if (lane >= d) x += y;
-  }
-  return x;
-}
-
 // LDS places of 16-byte chunk c of row r: c ^ swz16(r) in rows of whole 256-byte blocks (kn and v),
 // c ^ swz8(r) in the 128-byte rows of k_r. A ds_read_b128 serves rows {0-3, 12-15} of one chunk with rows
 // {4-11} of its neighbour, a transposed read two neighbouring chunks of eight rows; either way these
@@ -150,7 +141,7 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(ExpandedArgs a) 
         const Seq s(a, b0 + lane);
         nt = s.before(s.blocks);
       }
-      incl = wave_scan(nt, lane);
+      incl = wave_prefix_sum(nt);
       if (blockIdx.x == 0 && wave == 0 && b0 + lane < a.batch) a.seq_tile[b0 + lane] = per_head + incl - nt;
       per_head += __builtin_amdgcn_readlane(incl, 63);
     }
@@ -172,7 +163,7 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(ExpandedArgs a) 
           const Seq s(a, b0 + lane);
           nt = s.before(s.blocks);
         }
-        incl = wave_scan(nt, lane);
+        incl = wave_prefix_sum(nt);
       }
       const int sum = __builtin_amdgcn_readlane(incl, 63);
       if (sum > rel) {
@@ -317,7 +308,7 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(ExpandedArgs a) 
           float top = x[0];
 #pragma unroll
           for (int e = 1; e < 15; e += 2) top = max3(top, x[e], x[e + 1]);
-          top = row_group_max(max2(top, x[15])) * a.scale_log2;  // a scale is not negative
+          top = row_group_max(max2(top, x[15])) * a.scale_log2;  // a scale is positive
           if (__builtin_amdgcn_ballot_w64(top > m[rt] + kSlack)) {  // m = -inf at first
             const float mn = fmaxf(m[rt], top);
             const float c = mn == -INFINITY ? 1.f : fast_exp2(m[rt] - mn);
@@ -528,7 +519,7 @@ extern "C" int ti_latent_prefill(const void* q, int64_t q_stride_t, int64_t q_st
     return fail(TI_EINVAL, "%s: rows must be 16-byte aligned", who);
   }
   // A tile's rows are reached by 32-bit offsets.
-  if (!(scale >= 0.f)) return fail(TI_EINVAL, "%s: scale %g is negative", who, double(scale));
+  if (!(scale > 0.f)) return fail(TI_EINVAL, "%s: scale %g is not positive", who, double(scale));
   if (kv_stride_t < 0 || key_stride_t < 0 || kv_stride_t >= (1 << 24) || key_stride_t >= (1 << 24)) {
     return fail(TI_EINVAL, "%s: token strides %lld, %lld of kv and key_rope must be in [0, 2^24)", who,
                 static_cast<long long>(kv_stride_t), static_cast<long long>(key_stride_t));

@@ -22,7 +22,7 @@ import functools
 import torch
 
 from .. import _lib
-from .latent_attention import _as_rows, _paged_args
+from .latent_attention import _as_rows, _paged_args, _scale
 
 __all__ = ["cache_attention_mass", "evict_kvcache"]
 
@@ -96,6 +96,7 @@ def cache_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, block_table: to
         raise TypeError(f"dtype mismatch: q {dt}, k_cache {k_cache.dtype}")
     block_table, seqlen_kv, rows, page_size = _paged_args(block_table, seqlen_kv, k_cache, page_size, b, dev)
     width = block_table.shape[1]
+    scale = _scale(d ** -0.5 if scale is None else scale)
     if mass is None:
         mass = torch.zeros((b, hkv, width * page_size), dtype=torch.float32, device=dev)
     else:
@@ -110,7 +111,7 @@ def cache_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, block_table: to
             q4.data_ptr(), q4.stride(0), q4.stride(1), q4.stride(2), k_cache.data_ptr(),
             block_table.data_ptr(), block_table.stride(0), seqlen_kv.data_ptr(), mass.data_ptr(),
             mass.stride(0), mass.stride(1), ws.data_ptr(), nbytes, b, new, hq, hkv, d, page_size,
-            rows // page_size, width, d ** -0.5 if scale is None else float(scale), code,
+            rows // page_size, width, scale, code,
             _lib.stream_handle(dev)))
     return mass
 

@@ -48,6 +48,13 @@ def _as_rows(t: torch.Tensor) -> torch.Tensor:
     return t if _vec_rows(t) else t.clone(memory_format=torch.contiguous_format)
 
 
+def _scale(scale: float) -> float:
+    scale = float(scale)
+    if not 0 < scale < float("inf"):
+        raise ValueError(f"scale {scale} must be positive")
+    return scale
+
+
 def latent_rope_append(q_rope: torch.Tensor | None, latent: torch.Tensor, key_rope: torch.Tensor,
                        weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
                        latent_cache: torch.Tensor, slot_mapping: torch.Tensor, eps: float = 1e-5, *,
@@ -176,6 +183,7 @@ def latent_decode_paged_fn(q: torch.Tensor, latent_cache: torch.Tensor, block_ta
         raise TypeError(f"dtype mismatch: q {dt}, latent_cache {latent_cache.dtype}")
     block_table, seqlen_kv, rows, page_size = _paged_args(block_table, seqlen_kv, latent_cache, page_size,
                                                           b, dev)
+    scale = _scale(scale)
     shape = (b, h, dim) if q.dim() == 3 else (b, new, h, dim)
     if out is None:
         out = torch.empty(shape, dtype=dt, device=dev)
@@ -192,7 +200,7 @@ def latent_decode_paged_fn(q: torch.Tensor, latent_cache: torch.Tensor, block_ta
             q4.data_ptr(), q4.stride(0), q4.stride(1), q4.stride(2), latent_cache.data_ptr(),
             block_table.data_ptr(), block_table.stride(0), seqlen_kv.data_ptr(), out.data_ptr(),
             ws.data_ptr(), nbytes, b, new, h, dim, ROPE_DIM, page_size, rows // page_size,
-            block_table.shape[1], float(scale), code, _lib.stream_handle(dev)))
+            block_table.shape[1], scale, code, _lib.stream_handle(dev)))
     return out
 
 
@@ -275,9 +283,7 @@ def latent_prefill_fn(q: torch.Tensor, kv: torch.Tensor, key_rope: torch.Tensor,
     max_seqlen_q = int(max_seqlen_q)
     if max_seqlen_q < 0:
         raise ValueError(f"max_seqlen_q {max_seqlen_q} is negative")
-    scale = row ** -0.5 if scale is None else float(scale)
-    if not scale >= 0:
-        raise ValueError(f"scale {scale} is negative")
+    scale = _scale(row ** -0.5 if scale is None else scale)
     if out is None:
         out = torch.empty((total_q, h, d), dtype=dt, device=dev)
     elif out.shape != (total_q, h, d) or out.dtype != dt or out.device != dev or not _vec_rows(out):
