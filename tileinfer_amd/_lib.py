@@ -168,7 +168,9 @@ def load(path: Path | str | None = None) -> ctypes.CDLL:
 # The library functions that _pycalls.so calls, in the order its bind() takes them.
 _BOUND = ("ti_kv_append", "ti_gqa_decode_plan", "ti_gqa_decode_paged", "ti_gqa_decode_paged_gated",
           "ti_gqa_decode_paged_append", "ti_gqa_prefill_paged", "ti_gqa_prefill_paged_gated",
-          "ti_gqa_prefill_workspace_bytes", "ti_qknorm_rope_append")
+          "ti_gqa_prefill_workspace_bytes", "ti_qknorm_rope_append", "ti_latent_rope_append",
+          "ti_latent_decode_workspace_bytes", "ti_latent_decode_paged", "ti_cache_mass_workspace_bytes",
+          "ti_cache_mass", "ti_evict_kvcache")
 _calls = None
 
 
@@ -256,3 +258,15 @@ def on(device: torch.device):
     if device.index is None or device.index == torch.cuda.current_device():
         return contextlib.nullcontext()
     return torch.cuda.device(device)
+
+
+_get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def native(t):
+    """Stream handle for ``calls()`` where ``t`` is a plain tensor on the current GPU; None: the call goes to
+    the Python form, which copies, refuses or changes the device."""
+    if type(t) is not torch.Tensor or not t.is_cuda:
+        return None
+    index = t.get_device()
+    return current_stream(index) if index == _get_device() else None

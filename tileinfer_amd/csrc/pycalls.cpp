@@ -36,6 +36,12 @@ decltype(&ti_gqa_prefill_paged) p_prefill = nullptr;
 decltype(&ti_gqa_prefill_paged_gated) p_prefill_gated = nullptr;
 decltype(&ti_gqa_prefill_workspace_bytes) p_prefill_ws = nullptr;
 decltype(&ti_qknorm_rope_append) p_qknorm_append = nullptr;
+decltype(&ti_latent_rope_append) p_latent_append = nullptr;
+decltype(&ti_latent_decode_workspace_bytes) p_latent_ws = nullptr;
+decltype(&ti_latent_decode_paged) p_latent_decode = nullptr;
+decltype(&ti_cache_mass_workspace_bytes) p_mass_ws = nullptr;
+decltype(&ti_cache_mass) p_mass = nullptr;
+decltype(&ti_evict_kvcache) p_evict = nullptr;
 
 // A plain tensor with memory of its own on a GPU, or nullptr.
 const at::Tensor* plain(PyObject* o) {
@@ -350,13 +356,266 @@ PyObject* qknorm_append(PyObject* const* a) {
   return THPVariable_Wrap(std::move(out));
 }
 
+constexpr int64_t kRope = 64;
+
+bool latent_dim(int64_t n) { return n == 256 || n == 512; }
+
+// A positive, finite float.
+bool scale_of(PyObject* o, float& out) {
+  if (!PyFloat_CheckExact(o)) return false;
+  const double x = PyFloat_AS_DOUBLE(o);
+  out = float(x);
+  return x > 0 && x < 1e30;
+}
+
+bool int_of(PyObject* o, int64_t& out) {
+  if (!PyLong_CheckExact(o)) return false;
+  out = PyLong_AsLongLong(o);
+  if (out == -1 && PyErr_Occurred()) {
+    PyErr_Clear();
+    return false;
+  }
+  return fits32(out);
+}
+
+// A layer's cache pages, its block table, lengths and page size.
+struct Pages {
+  const at::Tensor *cache, *table, *lens;
+  int64_t rows, page, width, batch;
+};
+
+bool pages(PyObject* cache, PyObject* table, PyObject* lens, PyObject* page, Pages& o) {
+  o.cache = plain(cache);
+  o.table = plain(table);
+  o.lens = plain(lens);
+  if (!o.cache || !o.table || !o.lens || !int_of(page, o.page) || o.cache->dim() != 4 || o.table->dim() != 2) return false;
+  const at::Device dev = o.cache->device();
+  o.rows = o.cache->size(0) * o.cache->size(1);
+  o.batch = o.table->size(0);
+  o.width = o.table->size(1);
+  return o.page > 0 && o.rows % o.page == 0 && o.batch > 0 && o.width > 0 && fits32(o.batch) && fits32(o.width) &&
+         o.cache->is_contiguous() && address(*o.cache) % 16 == 0 && dtype_code(*o.cache) >= 0 &&
+         o.table->scalar_type() == at::kInt && o.table->stride(1) == 1 && o.table->device() == dev &&
+         int32_vector(*o.lens, o.batch, dev);
+}
+
+// Queries [B, H, D] or [B, N, H, D] of a cache with D values a row.
+struct Queries {
+  const at::Tensor* q;
+  int64_t batch, tokens, heads, dim, st_b, st_t, st_h;
+};
+
+bool queries(PyObject* o, const Pages& p, Queries& out) {
+  out.q = plain(o);
+  if (!out.q) return false;
+  const at::Tensor& q = *out.q;
+  const int64_t n = q.dim();
+  if ((n != 3 && n != 4) || !aligned_rows(q, 8) || q.scalar_type() != p.cache->scalar_type() ||
+      q.device() != p.cache->device()) {
+    return false;
+  }
+  out.batch = q.size(0);
+  out.tokens = n == 4 ? q.size(1) : 1;
+  out.heads = q.size(n - 2);
+  out.dim = q.size(n - 1);
+  out.st_b = q.stride(0);
+  out.st_t = n == 4 ? q.stride(1) : 0;
+  out.st_h = q.stride(n - 2);
+  return out.batch == p.batch && out.tokens > 0 && out.heads > 0 && out.dim == p.cache->size(3) &&
+         fits32(out.tokens) && fits32(out.heads) && fits32(out.dim);
+}
+
+// (q_rope | None, latent, key_rope, weight, cos, sin, latent_cache, slot_mapping, eps, weight_offset, stream)
+// -> q_out, or True without queries
+PyObject* latent_append(PyObject* const* a) {
+  const at::Tensor* t[7];  // latent, key_rope, weight, cos, sin, latent_cache, slots
+  for (int i = 0; i < 7; ++i) {
+    t[i] = plain(a[i + 1]);
+    if (!t[i]) Py_RETURN_NONE;
+  }
+  const at::Tensor &c = *t[0], &k = *t[1], &w = *t[2], &cos = *t[3], &sin = *t[4], &cache = *t[5], &slots = *t[6];
+  const int code = dtype_code(c);
+  if (!PyFloat_CheckExact(a[8]) || !PyFloat_CheckExact(a[9]) || code < 0 || c.dim() != 2 || k.dim() != 2 ||
+      w.dim() != 1 || cos.dim() != 2 || cache.dim() != 2) {
+    Py_RETURN_NONE;
+  }
+  const int64_t n = c.size(0), dim = c.size(1);
+  for (int i = 0; i < 6; ++i) {
+    if (t[i]->scalar_type() != c.scalar_type() || t[i]->device() != c.device() || !aligned_rows(*t[i], 8)) {
+      Py_RETURN_NONE;
+    }
+  }
+  if (n <= 0 || !latent_dim(dim) || k.size(0) != n || k.size(1) != kRope || w.size(0) != dim || cos.size(0) != n ||
+      cos.size(1) != kRope || cos.sizes() != sin.sizes() || cos.strides() != sin.strides() ||
+      cache.size(1) != dim + kRope || cache.stride(0) < dim + kRope || !int32_vector(slots, n, c.device())) {
+    Py_RETURN_NONE;
+  }
+  const at::Tensor* q = nullptr;
+  int64_t heads = 0;
+  if (a[0] != Py_None) {
+    q = plain(a[0]);
+    if (!q || q->dim() != 3 || q->size(0) != n || q->size(1) <= 0 || q->size(2) != kRope ||
+        q->scalar_type() != c.scalar_type() || q->device() != c.device() || !aligned_rows(*q, 8)) {
+      Py_RETURN_NONE;
+    }
+    heads = q->size(1);
+  }
+  if (!fits32(n) || !fits32(heads)) Py_RETURN_NONE;
+  void* stream = stream_of(a[10]);
+  at::Tensor out;
+  int rc;
+  {
+    Unlocked unlocked;
+    if (q) out = at::empty({n, heads, kRope}, q->options());
+    rc = p_latent_append(q ? q->data_ptr() : nullptr, q ? q->stride(0) : 0, q ? q->stride(1) : 0,
+                         q ? out.data_ptr() : nullptr, heads * kRope, kRope, c.data_ptr(), c.stride(0), k.data_ptr(),
+                         k.stride(0), w.data_ptr(), float(PyFloat_AS_DOUBLE(a[9])), cos.data_ptr(), sin.data_ptr(),
+                         n == 1 ? 0 : cos.stride(0), cache.data_ptr(), cache.stride(0), cache.size(0),
+                         static_cast<const int32_t*>(slots.data_ptr()), int32_t(n), int32_t(heads), int32_t(dim),
+                         int32_t(kRope), float(PyFloat_AS_DOUBLE(a[8])), code, stream);
+  }
+  if (rc != TI_OK) return PyLong_FromLong(rc);
+  if (!q) Py_RETURN_TRUE;
+  return THPVariable_Wrap(std::move(out));
+}
+
+// (q, latent_cache, block_table, seqlen, page_size, scale, stream)
+PyObject* latent_decode(PyObject* const* a) {
+  Pages p;
+  Queries q;
+  float scale;
+  if (!pages(a[1], a[2], a[3], a[4], p) || !queries(a[0], p, q) || !scale_of(a[5], scale) || p.cache->size(2) != 1 ||
+      !latent_dim(q.dim - kRope)) {
+    Py_RETURN_NONE;
+  }
+  const int64_t dim = q.dim - kRope;
+  void* stream = stream_of(a[6]);
+  at::Tensor out;
+  int rc;
+  {
+    Unlocked unlocked;
+    int64_t ws_bytes = 0;
+    rc = p_latent_ws(int32_t(p.batch), int32_t(q.tokens), int32_t(q.heads), int32_t(dim), &ws_bytes);
+    if (rc == TI_OK) {
+      out = q.q->dim() == 3 ? at::empty({p.batch, q.heads, dim}, q.q->options())
+                            : at::empty({p.batch, q.tokens, q.heads, dim}, q.q->options());
+      at::Tensor ws = bytes_on(*q.q, ws_bytes);
+      rc = p_latent_decode(q.q->data_ptr(), q.st_b, q.st_t, q.st_h, p.cache->data_ptr(),
+                           static_cast<const int32_t*>(p.table->data_ptr()), p.table->stride(0),
+                           static_cast<const int32_t*>(p.lens->data_ptr()), out.data_ptr(), ws.data_ptr(), ws_bytes,
+                           int32_t(p.batch), int32_t(q.tokens), int32_t(q.heads), int32_t(dim), int32_t(kRope),
+                           int32_t(p.page), p.rows / p.page, int32_t(p.width), scale, dtype_code(*q.q), stream);
+    }
+  }
+  if (rc != TI_OK) return PyLong_FromLong(rc);
+  return THPVariable_Wrap(std::move(out));
+}
+
+// Running sums [batch, heads, >= tokens] of a cache's tokens, rows apart.
+bool mass_rows(const at::Tensor& m, int64_t batch, int64_t heads, int64_t tokens, const at::Device& dev) {
+  return m.scalar_type() == at::kFloat && m.dim() == 3 && m.size(0) == batch && m.size(1) == heads &&
+         m.size(2) >= tokens && m.device() == dev && m.stride(2) == 1 && m.stride(1) >= m.size(2) &&
+         (batch == 1 || m.stride(0) >= heads * m.stride(1));
+}
+
+// (q, k_cache, block_table, seqlen, page_size, scale, mass | None, stream) -> mass
+PyObject* cache_mass(PyObject* const* a) {
+  Pages p;
+  Queries q;
+  float scale;
+  if (!pages(a[1], a[2], a[3], a[4], p) || !queries(a[0], p, q) || !scale_of(a[5], scale)) Py_RETURN_NONE;
+  const int64_t hkv = p.cache->size(2), tokens = p.width * p.page;
+  const bool dim_ok = q.dim == 128 || q.dim == 256 || q.dim == 320 || q.dim == 576;
+  if (!dim_ok || hkv <= 0 || q.heads % hkv != 0) Py_RETURN_NONE;
+  at::Tensor mass;
+  if (a[6] != Py_None) {
+    const at::Tensor* m = plain(a[6]);
+    if (!m || !mass_rows(*m, p.batch, hkv, tokens, q.q->device())) Py_RETURN_NONE;
+    mass = *m;
+  }
+  void* stream = stream_of(a[7]);
+  int rc;
+  {
+    Unlocked unlocked;
+    int64_t ws_bytes = 0;
+    rc = p_mass_ws(int32_t(p.batch), int32_t(q.tokens), int32_t(q.heads), int32_t(hkv), int32_t(q.dim),
+                   int32_t(p.page), int32_t(p.width), &ws_bytes);
+    if (rc == TI_OK) {
+      if (!mass.defined()) mass = at::zeros({p.batch, hkv, tokens}, q.q->options().dtype(at::kFloat));
+      at::Tensor ws = bytes_on(*q.q, ws_bytes);
+      rc = p_mass(q.q->data_ptr(), q.st_b, q.st_t, q.st_h, p.cache->data_ptr(),
+                  static_cast<const int32_t*>(p.table->data_ptr()), p.table->stride(0),
+                  static_cast<const int32_t*>(p.lens->data_ptr()), static_cast<float*>(mass.data_ptr()),
+                  mass.stride(0), mass.stride(1), ws.data_ptr(), ws_bytes, int32_t(p.batch), int32_t(q.tokens),
+                  int32_t(q.heads), int32_t(hkv), int32_t(q.dim), int32_t(p.page), p.rows / p.page,
+                  int32_t(p.width), scale, dtype_code(*q.q), stream);
+    }
+  }
+  if (rc != TI_OK) return PyLong_FromLong(rc);
+  if (a[6] != Py_None) return (Py_INCREF(a[6]), a[6]);
+  return THPVariable_Wrap(std::move(mass));
+}
+
+// (k_cache, v_cache | None, mass, block_table, seqlen, new_block_table, budget, page_size, sinks, recent, stream)
+// -> (new_seqlen, kept, new_mass)
+PyObject* evict(PyObject* const* a) {
+  Pages p;
+  const at::Tensor *mass = plain(a[2]), *into = plain(a[5]), *v = nullptr;
+  int64_t budget, sinks, recent;
+  if (!mass || !into || !pages(a[0], a[3], a[4], a[7], p) || !int_of(a[6], budget) || !int_of(a[8], sinks) ||
+      !int_of(a[9], recent)) {
+    Py_RETURN_NONE;
+  }
+  const at::Device dev = p.cache->device();
+  const int64_t hkv = p.cache->size(2), dim = p.cache->size(3), tokens = p.width * p.page;
+  if (hkv <= 0 || dim <= 0 || dim % 8 != 0 || !fits32(hkv) || !fits32(dim) || budget <= 0 || sinks + recent > budget ||
+      !mass_rows(*mass, p.batch, hkv, tokens, dev) || into->dim() != 2 || into->size(0) != p.batch ||
+      into->scalar_type() != at::kInt || into->stride(1) != 1 || into->device() != dev || !fits32(into->size(1))) {
+    Py_RETURN_NONE;
+  }
+  if (a[1] != Py_None) {
+    v = plain(a[1]);
+    if (!v || v->sizes() != p.cache->sizes() || v->scalar_type() != p.cache->scalar_type() || v->device() != dev ||
+        !v->is_contiguous() || address(*v) % 16 != 0) {
+      Py_RETURN_NONE;
+    }
+  }
+  void* stream = stream_of(a[10]);
+  at::Tensor lens, kept, sums;
+  int rc;
+  {
+    Unlocked unlocked;
+    const auto ints = p.table->options();
+    lens = at::empty({p.batch}, ints);
+    kept = at::empty({p.batch, hkv, budget}, ints);
+    sums = at::empty({p.batch, hkv, mass->size(2)}, mass->options());
+    rc = p_evict(p.cache->data_ptr(), v ? v->data_ptr() : nullptr, static_cast<const float*>(mass->data_ptr()),
+                 mass->stride(0), mass->stride(1), mass->size(2), static_cast<const int32_t*>(p.table->data_ptr()),
+                 p.table->stride(0), static_cast<const int32_t*>(p.lens->data_ptr()),
+                 static_cast<const int32_t*>(into->data_ptr()), into->stride(0),
+                 static_cast<int32_t*>(kept.data_ptr()), static_cast<int32_t*>(lens.data_ptr()),
+                 static_cast<float*>(sums.data_ptr()), int32_t(p.batch), int32_t(hkv), int32_t(dim),
+                 int32_t(p.page), p.rows / p.page, int32_t(p.width), int32_t(into->size(1)), int32_t(budget),
+                 int32_t(sinks), int32_t(recent), dtype_code(*p.cache), stream);
+  }
+  if (rc != TI_OK) return PyLong_FromLong(rc);
+  PyObject* r = PyTuple_New(3);
+  if (!r) return nullptr;
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(lens)));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(kept)));
+  PyTuple_SET_ITEM(r, 2, THPVariable_Wrap(std::move(sums)));
+  return r;
+}
+
 // The library's entry points by address, in the order of the list below.
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   void** slots[] = {(void**)&p_append,        (void**)&p_plan,          (void**)&p_decode,
                     (void**)&p_decode_gated,  (void**)&p_decode_append, (void**)&p_prefill,
-                    (void**)&p_prefill_gated, (void**)&p_prefill_ws,    (void**)&p_qknorm_append};
+                    (void**)&p_prefill_gated, (void**)&p_prefill_ws,    (void**)&p_qknorm_append,
+                    (void**)&p_latent_append, (void**)&p_latent_ws,     (void**)&p_latent_decode,
+                    (void**)&p_mass_ws,       (void**)&p_mass,          (void**)&p_evict};
   if (n != Py_ssize_t(sizeof(slots) / sizeof(slots[0]))) {
-    PyErr_SetString(PyExc_TypeError, "bind: nine addresses");
+    PyErr_SetString(PyExc_TypeError, "bind: one address for each entry point");
     return nullptr;
   }
   for (Py_ssize_t i = 0; i < n; ++i) {
@@ -379,6 +638,10 @@ PyMethodDef methods[] = {{"bind", (PyCFunction)(void (*)(void))bind, METH_FASTCA
                          TI_METHOD(prefill, 12),
                          TI_METHOD(append, 6),
                          TI_METHOD(qknorm_append, 12),
+                         TI_METHOD(latent_append, 11),
+                         TI_METHOD(latent_decode, 7),
+                         TI_METHOD(cache_mass, 8),
+                         TI_METHOD(evict, 11),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pycalls", nullptr, -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

@@ -90,6 +90,36 @@ def layer_views(kv_cache: torch.Tensor, layer: int):
     return k_paged.reshape(nb * bs, h * d), v_paged.reshape(nb * bs, h * d), k_paged, v_paged
 
 
+def latent_cache_shape(num_layers: int, num_blocks: int, block_size: int, latent_dim: int,
+                       rope_dim: int = 64) -> tuple[int, ...]:
+    """A latent-attention cache: one vector a token, ``[latent | rotated part]``, in the place of a KV head."""
+    return (num_layers, num_blocks, block_size, 1, latent_dim + rope_dim)
+
+
+def latent_block_bytes(block_size: int, latent_dim: int, num_layers: int, rope_dim: int = 64,
+                       dtype: torch.dtype = torch.bfloat16) -> int:
+    """Bytes one block id costs across every layer of a latent cache."""
+    return block_size * (latent_dim + rope_dim) * KV_DTYPE_BYTES[dtype] * num_layers
+
+
+def allocate_latent_cache(num_layers: int, num_blocks: int, block_size: int, latent_dim: int,
+                          rope_dim: int = 64, device: torch.device | str = "cuda",
+                          dtype: torch.dtype = torch.bfloat16, zero: bool = True) -> torch.Tensor:
+    """The slab of a latent cache (see ``latent_cache_shape``); ``copy_blocks`` and ``swap_blocks`` take it
+    as they take a KV slab."""
+    alloc = torch.zeros if zero else torch.empty
+    return alloc(latent_cache_shape(num_layers, num_blocks, block_size, latent_dim, rope_dim),
+                 dtype=dtype, device=device)
+
+
+def latent_layer_views(latent_cache: torch.Tensor, layer: int):
+    """(rows, paged) of one layer: ``[num_blocks * block_size, latent_dim + rope_dim]`` for
+    ``latent_rope_append``, ``[num_blocks, block_size, 1, latent_dim + rope_dim]`` for
+    ``latent_decode_paged_fn``, ``cache_attention_mass`` and ``evict_kvcache``."""
+    paged = latent_cache[layer]
+    return paged.reshape(-1, paged.shape[-1]), paged
+
+
 def _slot(table: list[int], pos: int, bs: int) -> int:
     return table[pos // bs] * bs + pos % bs
 

@@ -4,8 +4,8 @@
 queries of its sequence give it: those of one decode step, step after step, or of a window at the end of a
 prompt. ``evict_kvcache`` keeps the heaviest tokens of every (sequence, KV head), with the first and the most
 recent ones always among them, and copies their rows to the blocks of a new, shorter table. The old table's
-blocks are untouched, so blocks shared with other sequences (prefix caching) stay valid; the caller releases
-the old table afterwards (``PagedKVManager.begin_evict`` / ``finish_evict``).
+blocks are untouched, so blocks shared with other sequences (prefix caching) stay valid; the caller takes the
+new blocks from its block manager and releases the old table afterwards.
 
 Both take the KV cache of one attention layer, or a latent cache as its one KV head with ``v_cache=None``.
 Keys are cached after their rotation, so a token keeps its position's angle wherever its row moves; the
@@ -76,6 +76,13 @@ def cache_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, block_table: to
         query ``i`` of ``N`` seeing ``t <= seqlen_kv - N + i``. Values from ``seqlen_kv`` on are not touched.
         The same call gives the same bits.
     """
+    # The call in its common form is checked and made in native code; None: another form, or one to refuse.
+    stream = _lib.native(q)
+    if stream is not None and q.dim() > 0 and q.shape[-1] > 0:
+        r = _lib.result(_lib.calls().cache_mass(q, k_cache, block_table, seqlen_kv, page_size,
+                                                q.shape[-1] ** -0.5 if scale is None else scale, mass, stream))
+        if r is not None:
+            return r
     if q.dim() not in (3, 4):
         raise ValueError(f"q must be [B, H_q, D] or [B, N, H_q, D], got {tuple(q.shape)}")
     q4 = q.unsqueeze(1) if q.dim() == 3 else q
@@ -140,6 +147,13 @@ def evict_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor | None, mass: tor
         ``(seqlen, kept, mass)``: the new lengths ``[B]`` int32, the kept positions ``[B, H_kv, budget]`` int32
         (ascending, -1 behind the last) and their masses ``[B, H_kv, capacity]`` (0 behind the last).
     """
+    # The call in its common form is checked and made in native code; None: another form, or one to refuse.
+    stream = _lib.native(k_cache)
+    if stream is not None:
+        r = _lib.result(_lib.calls().evict(k_cache, v_cache, mass, block_table, seqlen_kv, new_block_table, budget,
+                                           page_size, sinks, recent, stream))
+        if r is not None:
+            return r
     _cache_ok("k_cache", k_cache)
     dev, dt = k_cache.device, k_cache.dtype
     code = _lib.dtype_code(dt)

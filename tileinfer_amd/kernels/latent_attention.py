@@ -70,6 +70,13 @@ def latent_rope_append(q_rope: torch.Tensor | None, latent: torch.Tensor, key_ro
     whole factor. ``q_out`` ``[T, H, 64]`` receives the rotated parts, for instance the last 64 columns of
     ``latent_decode_paged_fn``'s queries; it may be ``q_rope`` itself.
     """
+    # The call in its common form is checked and made in native code; None: another form, or one to refuse.
+    stream = None if q_out is not None else _lib.native(latent)
+    if stream is not None:
+        r = _lib.result(_lib.calls().latent_append(q_rope, latent, key_rope, weight, cos, sin, latent_cache,
+                                                   slot_mapping, eps, weight_offset, stream))
+        if r is not None:
+            return None if r is True else r
     if latent.dim() != 2 or key_rope.dim() != 2:
         raise ValueError("latent must be [T, L] and key_rope [T, 64]")
     t, dim = latent.shape
@@ -161,6 +168,13 @@ def latent_decode_paged_fn(q: torch.Tensor, latent_cache: torch.Tensor, block_ta
         each head's ``Wv``. Query ``i`` of ``N`` sees the keys ``j <= seqlen_kv - N + i``; one that sees
         nothing gives zeros. Block ids outside the cache below ``seqlen_kv`` are treated as absent.
     """
+    # The call in its common form is checked and made in native code; None: another form, or one to refuse.
+    stream = None if out is not None else _lib.native(q)
+    if stream is not None:
+        r = _lib.result(_lib.calls().latent_decode(q, latent_cache, block_table, seqlen_kv, page_size, scale,
+                                                   stream))
+        if r is not None:
+            return r
     if q.dim() not in (3, 4):
         raise ValueError(f"q must be [B, H, L + 64] or [B, N, H, L + 64], got {tuple(q.shape)}")
     q4 = q.unsqueeze(1) if q.dim() == 3 else q
