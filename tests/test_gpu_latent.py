@@ -166,6 +166,10 @@ PREFILLS = [
     # more units than CUs: one workgroup each
     (48, 64, BF16, [(700, 700), (1, 9), (50, 130)], True),
     (33, 128, F16, [(1100, 1100)], True),
+    # long first chunks of few units: two key groups
+    (40, 128, BF16, [(1100, 1100)], True),
+    (20, 64, F16, [(1030, 1050), (1301, 1281)], True),
+    (14, 128, F16, [(1, 1), (2500, 2499), (600, 601)], True),
     # cut units: few heads over long keys, blocks that see nothing, empty sequences between others
     (2, 128, BF16, [(300, 2500), (0, 0), (0, 40), (400, 130), (1, 1999)], True),
     (1, 64, F16, [(129, 3001)] + [(3, 70)] * 70, True),

@@ -10,7 +10,8 @@
 //   S^T[64 keys x 32 rows]  = K[64 x (DN + 64)] . Q^T        (16x16x32, Q in registers)
 //   O^T[DN x 32 rows]      += V^T[DN x 64] . P^T             (16x16x32, V by transposed reads)
 // with an accumulator's row its lane's column, as in the paged prefill. Two workgroups fit a CU, so that
-// one's softmax runs beside the other's products.
+// one's softmax runs beside the other's products. A workgroup of eight waves gives each half of a tile's keys
+// to four of them and joins the two sums through LDS at the unit's end.
 //
 // Two schedules. Per unit: one workgroup each, the last query blocks, which see the most keys, first; no
 // workspace. Balanced: the tiles of all units are one list (by head, sequence, block), cut into equal runs,
@@ -38,7 +39,7 @@ struct ExpandedArgs {
   int64_t o_st, o_sh;
   const int32_t* cu_q;
   const int32_t* cu_k;
-  int32_t total_q, total_k, causal, batch, heads;
+  int32_t total_q, total_k, causal, batch, heads, key_groups;
   float scale_log2;
   // Balanced schedule (runs > 0): parts of cut units, and each sequence's first tile within a head's.
   int32_t runs;
@@ -112,22 +113,27 @@ __device__ __forceinline__ int swz8(int r) {
   return ((2 * u) & 7) ^ ((u & 4) ? 5 : 0);
 }
 
-template <int DN, bool BALANCED, typename Tag>
-__global__ __launch_bounds__(256, 2) void latent_prefill_kernel(ExpandedArgs a) {
+// KG: key groups of four waves each; a group takes 64 / KG keys of a tile.
+template <int DN, int KG, bool BALANCED, typename Tag>
+__global__ __launch_bounds__(256 * KG, 2) void latent_prefill_kernel(ExpandedArgs a) {
+  constexpr int TT = 4 / KG, KP = 2 / KG;   // 16-key and 32-key tiles of a wave
+  constexpr int STAGES = KG == 1 ? 2 : 3;
   constexpr int KN = DN / 32;               // k-steps of the unrotated part
   constexpr int NDT = DN / 16;
   constexpr int ROW = 2 * DN;               // elements of a [kn | v] row
   constexpr int CH = ROW / 8;
-  constexpr int NKV = kKeys * CH / 256;     // loads of a wave and tile
-  constexpr int NKR = kKeys * 8 / 256;
+  constexpr int NKV = kKeys * CH / 256 / KG;  // loads of a wave and tile
+  constexpr int NKR = kKeys * 8 / 256 / KG;
   constexpr int NL = NKV + NKR;
   constexpr int kStage = kKeys * (ROW + kRope);
   static_assert(CH % 16 == 0);
-  __shared__ __align__(16) uint16_t s_tile[2 * kStage];
+  static_assert(KG == 1 || STAGES * kStage * 2 >= 4 * (2 * NDT * 1024 + 2 * 512), "the stages hold a group's sums");
+  __shared__ __align__(16) uint16_t s_tile[STAGES * kStage];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
+  const int rw = wave & 3, key0 = 32 * (wave >> 2);  // rows and keys of a tile that this wave takes
 
   int h, b, qb;
   uint32_t p = 0, start = 0, end = 1;  // the run's positions in the list, and the next one
@@ -204,10 +210,10 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(ExpandedArgs a) 
   }
   // Operand reads of row n (K) and of row 4 g + n / 4 (V), elements: those of k-step kk and column tile dt are
   // at these with the bits of kk and dt flipped, which the rows' places leave alone.
-  const int k_at = n * ROW + 8 * (g ^ swz16(n));
-  const int r_at = kKeys * ROW + n * kRope + 8 * (g ^ swz8(n));
+  const int k_at = (key0 + n) * ROW + 8 * (g ^ swz16(n));
+  const int r_at = kKeys * ROW + (key0 + n) * kRope + 8 * (g ^ swz8(n));
   const int v_row = 4 * g + (n >> 2);
-  const int v_at = v_row * ROW + 8 * ((DN / 8 + ((lane >> 1) & 1)) ^ swz16(v_row)) + 4 * (lane & 1);
+  const int v_at = (key0 + v_row) * ROW + 8 * ((DN / 8 + ((lane >> 1) & 1)) ^ swz16(v_row)) + 4 * (lane & 1);
 
   while (true) {
     const Seq sq(a, b);
@@ -220,7 +226,7 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(ExpandedArgs a) 
     int limit[2];
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
-      const int r = min(qb * kRows + wave * 32 + rt * 16 + n, sq.q_len - 1);
+      const int r = min(qb * kRows + rw * 32 + rt * 16 + n, sq.q_len - 1);
       limit[rt] = a.causal ? sq.offset + r : sq.k_len - 1;
       const uint16_t* src = a.q + int64_t(sq.q0 + r) * a.q_st + h * a.q_sh + 8 * g;
 #pragma unroll
@@ -250,31 +256,39 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(ExpandedArgs a) 
       for (int dt = 0; dt < NDT; ++dt) o[dt][rt] = f32x4{};
     }
     // The rows this wave has, the keys its first and its last row see.
-    const int wrow = qb * kRows + wave * 32;
+    const int wrow = qb * kRows + rw * 32;
     const int see_first = a.causal ? sq.offset + wrow : sq.k_len - 1;
     const int see_last = a.causal ? sq.offset + min(wrow + 31, sq.q_len - 1) : sq.k_len - 1;
     const bool active = wrow < sq.q_len;
 
     __builtin_amdgcn_s_waitcnt(0);  // q has landed: the loop below has waits of its own alone
-    if (t0 < t1) issue(t0, 0);
-    if (t0 + 1 < t1) issue(t0 + 1, 1);
+    constexpr int kAhead = 2;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (t0 + i < t1) issue(t0 + i, i);
+    }
+    int stage = 0;
     for (int t = t0; t < t1; ++t) {
       if (t + 1 < t1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NL) : "memory");
       else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      const uint16_t* tile = s_tile + ((t - t0) & 1) * kStage;
-      if (active && t * kKeys <= see_last) {  // uniform
-        f32x4 s[4][2];
+      if constexpr (STAGES == 3) {  // every wave has read tile t - 1
+        if (t + kAhead < t1) issue(t + kAhead, stage == 0 ? STAGES - 1 : stage - 1);
+      }
+      const uint16_t* tile = s_tile + stage * kStage;
+      const int first_key = t * kKeys + key0;
+      if (active && first_key <= see_last) {  // uniform
+        f32x4 s[TT][2];
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
+        for (int tt = 0; tt < TT; ++tt) {
           s[tt][0] = f32x4{};
           s[tt][1] = f32x4{};
         }
         // The next k-step's reads go out before the products of the last one (sched_barrier: left to itself the
         // compiler reads each operand right before its MFMAs and waits for it).
-        u32x4 k[2][4];
-        auto read_keys = [&](int kk, u32x4 (&to)[4]) {
+        u32x4 k[2][TT];
+        auto read_keys = [&](int kk, u32x4 (&to)[TT]) {
 #pragma unroll
-          for (int tt = 0; tt < 4; ++tt) {
+          for (int tt = 0; tt < TT; ++tt) {
             const int at = kk < KN ? (k_at ^ (32 * kk)) + 16 * tt * ROW : (r_at ^ (32 * (kk - KN))) + 16 * tt * kRope;
             to[tt] = *reinterpret_cast<const u32x4*>(tile + at);
           }
@@ -285,30 +299,30 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(ExpandedArgs a) 
           if (kk + 1 < KN + 2) read_keys(kk + 1, k[(kk + 1) & 1]);
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int tt = 0; tt < 4; ++tt) {
+          for (int tt = 0; tt < TT; ++tt) {
 #pragma unroll
             for (int rt = 0; rt < 2; ++rt) s[tt][rt] = mfma16x16x32(k[kk & 1][tt], q[rt][kk], s[tt][rt], Tag{});
           }
           __builtin_amdgcn_sched_barrier(0);
         }
-        const bool whole = t * kKeys + kKeys - 1 <= see_first && (t + 1) * kKeys <= k_end;
-        u32x4 pb[2][2];
+        const bool whole = first_key + 16 * TT - 1 <= see_first && first_key + 16 * TT <= k_end;
+        u32x4 pb[2][KP];
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt) {
-          float x[16];
+          float x[4 * TT];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) x[e] = s[e >> 2][rt][e & 3];
+          for (int e = 0; e < 4 * TT; ++e) x[e] = s[e >> 2][rt][e & 3];
           if (!whole) {
-            const int lim = min(limit[rt], k_end - 1) - t * kKeys - 4 * g;
+            const int lim = min(limit[rt], k_end - 1) - first_key - 4 * g;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
+            for (int e = 0; e < 4 * TT; ++e) {
               if (16 * (e >> 2) + (e & 3) > lim) x[e] = -INFINITY;
             }
           }
           float top = x[0];
 #pragma unroll
-          for (int e = 1; e < 15; e += 2) top = max3(top, x[e], x[e + 1]);
-          top = row_group_max(max2(top, x[15])) * a.scale_log2;  // a scale is positive
+          for (int e = 1; e < 4 * TT - 1; e += 2) top = max3(top, x[e], x[e + 1]);
+          top = row_group_max(max2(top, x[4 * TT - 1])) * a.scale_log2;  // a scale is positive
           if (__builtin_amdgcn_ballot_w64(top > m[rt] + kSlack)) {  // m = -inf at first
             const float mn = fmaxf(m[rt], top);
             const float c = mn == -INFINITY ? 1.f : fast_exp2(m[rt] - mn);
@@ -319,17 +333,17 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(ExpandedArgs a) 
           }
           const float base = m[rt] == -INFINITY ? 0.f : m[rt];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
+          for (int e = 0; e < 4 * TT; ++e) {
             x[e] = fast_exp2(fmaf(x[e], a.scale_log2, -base));
             l[rt] += x[e];
           }
           // P is rounded to the inputs' type for the matrix unit, as in the paged prefill: at most half a
           // step of each weight, while l sums the unrounded ones in 32 bits.
 #pragma unroll
-          for (int e = 0; e < 8; ++e) pb[rt][e >> 2][e & 3] = pack2(x[2 * e], x[2 * e + 1], Tag{});
+          for (int e = 0; e < 2 * TT; ++e) pb[rt][e >> 2][e & 3] = pack2(x[2 * e], x[2 * e + 1], Tag{});
         }
 #pragma unroll
-        for (int kp = 0; kp < 2; ++kp) {
+        for (int kp = 0; kp < KP; ++kp) {
 #pragma unroll
           for (int dt = 0; dt < NDT; ++dt) {
             const uint16_t* at = tile + (v_at ^ (16 * dt)) + 32 * kp * ROW;
@@ -340,17 +354,50 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(ExpandedArgs a) 
           }
         }
       }
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the stage is read
-      if (t + 2 < t1) issue(t + 2, (t - t0) & 1);
+      if constexpr (STAGES == 2) {
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the stage is read
+        if (t + kAhead < t1) issue(t + kAhead, stage);
+      }
+      stage = stage == STAGES - 1 ? 0 : stage + 1;
     }
 
+    l[0] = row_group_sum(l[0]);
+    l[1] = row_group_sum(l[1]);
+    if constexpr (KG == 2) {
+      // The second key group's sums go to the first through the stages.
+      f32x4* const s_o = reinterpret_cast<f32x4*>(s_tile) + rw * 2 * NDT * 64 + lane;
+      float2* const s_ml = reinterpret_cast<float2*>(reinterpret_cast<f32x4*>(s_tile) + 4 * 2 * NDT * 64) + rw * 128 + lane;
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the stages are read
+      if (key0 != 0) {
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) {
+#pragma unroll
+          for (int dt = 0; dt < NDT; ++dt) s_o[64 * (NDT * rt + dt)] = o[dt][rt];
+          s_ml[64 * rt] = make_float2(m[rt], l[rt]);
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (key0 == 0) {
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) {
+          const float2 other = s_ml[64 * rt];
+          const float mn = fmaxf(m[rt], other.x);
+          const float base = mn == -INFINITY ? 0.f : mn;
+          const float c0 = fast_exp2(m[rt] - base), c1 = fast_exp2(other.x - base);
+          m[rt] = mn;
+          l[rt] = l[rt] * c0 + other.y * c1;
+#pragma unroll
+          for (int dt = 0; dt < NDT; ++dt) o[dt][rt] = o[dt][rt] * c0 + s_o[64 * (NDT * rt + dt)] * c1;
+        }
+      }
+    }
     const bool complete = t0 == 0 && t1 == tiles;
-    const int64_t part = (int64_t(run) * 2 + (p == start ? 0 : 1)) * kRows + wave * 32 + n;
+    const int64_t part = (int64_t(run) * 2 + (p == start ? 0 : 1)) * kRows + rw * 32 + n;
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
       const int r = wrow + rt * 16 + n;
-      const float lt = row_group_sum(l[rt]);
-      if (r >= sq.q_len) continue;
+      const float lt = l[rt];
+      if (r >= sq.q_len || key0 != 0) continue;
       if (!BALANCED || complete) {
         const float inv = lt != 0.f ? 1.f / lt : 0.f;  // a row that sees nothing is zero
         uint16_t* dst = a.out + int64_t(sq.q0 + r) * a.o_st + h * a.o_sh + 4 * g;
@@ -369,6 +416,7 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(ExpandedArgs a) 
     if constexpr (!BALANCED) return;
     p += uint32_t(t1 - t0);
     if (p >= end) return;
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the sums are read
     // The next unit that has tiles: the run holds more of them, so there is one.
     t_first = 0;
     do {
@@ -458,15 +506,27 @@ PrefillSizes prefill_sizes(int32_t batch, int32_t total_q, int32_t total_k, int3
   return z;
 }
 
+// Key groups of a workgroup. Two share a unit's rows and halve its tiles' time, but one such workgroup fills a
+// CU, so nothing runs beside its start and end. They are for first chunks of few units, where the time is that
+// of the last, longest unit: 2,048 queries with 24 heads (384 units) 55 us against 65, 4,096 with 12 heads 91
+// against 111. Units of one length (2,048 behind 8,192) take 366 us against 316, more units (2,800 with 24
+// heads, 528) 87 against 83 and short ones (24 of 90, 20 heads) 21 against 15.
+int32_t prefill_key_groups(int32_t batch, int32_t total_q, int32_t total_k, int32_t heads, int32_t causal) {
+  const bool few = ceil_div(total_q, kRows) * heads <= 2 * device_cu_count();
+  return causal && total_q == total_k && total_q / 8 / kRows >= batch && few ? 2 : 1;
+}
+
 template <int DN, typename Tag>
 void launch_prefill(const ExpandedArgs& a, int64_t longest, hipStream_t s) {
   const unsigned blocks = unsigned(ceil_div(longest, kRows));
   const unsigned heads = unsigned(a.heads), batch = unsigned(a.batch);
   if (a.runs == 0) {
-    hipLaunchKernelGGL((latent_prefill_kernel<DN, false, Tag>), dim3(heads, blocks, batch), dim3(256), 0, s, a);
+    const dim3 grid(heads, blocks, batch);
+    if (a.key_groups == 2) hipLaunchKernelGGL((latent_prefill_kernel<DN, 2, false, Tag>), grid, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((latent_prefill_kernel<DN, 1, false, Tag>), grid, dim3(256), 0, s, a);
     return;
   }
-  hipLaunchKernelGGL((latent_prefill_kernel<DN, true, Tag>), dim3(unsigned(a.runs)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((latent_prefill_kernel<DN, 1, true, Tag>), dim3(unsigned(a.runs)), dim3(256), 0, s, a);
   hipLaunchKernelGGL((latent_prefill_merge_kernel<DN, Tag>), dim3(blocks * (kRows / 16), heads, batch), dim3(256), 0,
                      s, a);
 }
@@ -556,6 +616,7 @@ extern "C" int ti_latent_prefill(const void* q, int64_t q_stride_t, int64_t q_st
     a.seq_tile = reinterpret_cast<int32_t*>(a.part_ml + z.ml_floats);
   }
   const int64_t longest = max_seqlen_q < total_q ? max_seqlen_q : total_q;
+  a.key_groups = prefill_key_groups(batch, total_q, total_k, num_heads, causal);
   if (ceil_div(longest, kRows) > 65535) return fail(TI_EINVAL, "%s: max_seqlen_q %d too long", who, max_seqlen_q);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool bf16 = dtype == TI_DTYPE_BF16;
