@@ -32,7 +32,7 @@ struct MassArgs {
   float* scores;  // [B, hkv, rows][tokens]  (up to 16 rows)
   float* part;    // [B, hkv][parts][rows][2]  (max, sum) of a workgroup's tokens, max in exp2 units
   float* stats;   // [B, hkv][rows][2]  (max, 1 / sum)  (more than 16 rows)
-  int32_t new_tokens, hkv, group, rows, num_blocks32, page_size, max_blocks;
+  int32_t new_tokens, hkv, group, rows, num_blocks32, page_size, page_shift, max_blocks;
   int32_t parts;   // parts of a sequence of the greatest length
   int64_t tokens;  // that length, a multiple of 4
   float scale_log2;
@@ -46,6 +46,8 @@ __device__ __forceinline__ int mass_len(const MassArgs& a, int b) {
   return int64_t(n) > cap ? int(cap) : n;
 }
 
+__device__ __align__(16) uint16_t g_zero_key[576] = {};
+
 // The K operands of tokens t0 + 16 tt + (0 .. 15), as lane (n, g) holds them, and whether this lane's
 // accumulator tokens (4 g + e of each tile) exist.
 template <int D, int TT>
@@ -58,20 +60,24 @@ template <int D, int TT>
 __device__ __forceinline__ void load_keys(const MassArgs& a, int b, int h, int len, int t0, KeyTile<D, TT>& x) {
   const int lane = threadIdx.x & 63;
   const int n = lane & 15, g = lane >> 4;
+  // All ids, then all rows: no load waits for another one's, and none is conditional (a branch around each would
+  // order them). An absent token is a row of zeros, whatever the cache holds there.
+  int id[TT], in_page[TT];
 #pragma unroll
   for (int tt = 0; tt < TT; ++tt) {
-    const int t = t0 + 16 * tt + n;
-    int id = -1, in_page = 0;
-    if (t < len) {
-      const int page = t / a.page_size;
-      in_page = t - page * a.page_size;
-      id = a.block_table[b * a.bt_stride + page];
-    }
-    const bool ok = uint32_t(id) < uint32_t(a.num_blocks32);
-    x.there[tt] = uint32_t(__builtin_amdgcn_ballot_w64(ok)) & 0xffffu;
-    const uint16_t* src = a.k_cache + ((int64_t(ok ? id : 0) * a.page_size + in_page) * a.hkv + h) * D + 8 * g;
+    const int t = min(t0 + 16 * tt + n, len - 1);
+    const int page = a.page_shift >= 0 ? t >> a.page_shift : t / a.page_size;
+    in_page[tt] = t - page * a.page_size;
+    id[tt] = a.block_table[b * a.bt_stride + page];
+  }
 #pragma unroll
-    for (int kk = 0; kk < D / 32; ++kk) x.k[tt][kk] = ok ? load16(src + 32 * kk) : u32x4{};
+  for (int tt = 0; tt < TT; ++tt) {
+    const bool ok = t0 + 16 * tt + n < len && uint32_t(id[tt]) < uint32_t(a.num_blocks32);
+    x.there[tt] = uint32_t(__builtin_amdgcn_ballot_w64(ok)) & 0xffffu;
+    const uint16_t* row = a.k_cache + ((int64_t(id[tt]) * a.page_size + in_page[tt]) * a.hkv + h) * D;
+    const uint16_t* src = (ok ? row : g_zero_key) + 8 * g;
+#pragma unroll
+    for (int kk = 0; kk < D / 32; ++kk) x.k[tt][kk] = load16(src + 32 * kk);
   }
 }
 
@@ -139,6 +145,9 @@ __global__ __launch_bounds__(256) void mass_scores_kernel(MassArgs a) {
   const int t0 = wg0 + wave * 16 * TT;
   KeyTile<D, TT> x;
   load_keys<D, TT>(a, b, h, len, t0, x);
+  // All of them in flight before the first product waits (16 x U[512, 8k], D = 256: 34.5 us against 36.9); 144
+  // registers of them would leave two waves a SIMD (16 x 4,000 latent rows 27.5 us against 24.6).
+  if constexpr (D <= 320) __builtin_amdgcn_sched_barrier(0);
   float s[TT][4], m, l;
   score_rows<D, TT, Tag>(a, b, h, len, t0, 0, x, s);
   if (n < a.rows) {
@@ -172,12 +181,20 @@ __device__ __forceinline__ void join_parts(const float* part, int parts, int64_t
                                            float& inv) {
   m = -INFINITY;
   float l = 0.f;
-  for (int p = lane16; p < parts; p += 16) {
-    const float pm = part[p * stride], pl = part[p * stride + 1];
-    const float mn = fmaxf(m, pm);
-    const float base = mn == -INFINITY ? 0.f : mn;
-    l = l * fast_exp2(m - base) + pl * fast_exp2(pm - base);
-    m = mn;
+  for (int p0 = 0; p0 < parts; p0 += 64) {  // four loads in flight a lane
+    float2 ml[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      ml[k] = *reinterpret_cast<const float2*>(part + min(p0 + 16 * k + lane16, parts - 1) * stride);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float pm = p0 + 16 * k + lane16 < parts ? ml[k].x : -INFINITY;
+      const float mn = fmaxf(m, pm);
+      const float base = mn == -INFINITY ? 0.f : mn;
+      l = l * fast_exp2(m - base) + (pm == -INFINITY ? 0.f : ml[k].y) * fast_exp2(pm - base);
+      m = mn;
+    }
   }
 #pragma unroll
   for (int d = 1; d < 16; d <<= 1) {
@@ -199,6 +216,11 @@ __global__ __launch_bounds__(256) void mass_add_kernel(MassArgs a, int part_toke
   const int len = mass_len(a, b);
   const int wg0 = int(blockIdx.x) * kAddTokens;
   if (wg0 >= len) return;
+  const int t = wg0 + 4 * int(threadIdx.x);
+  float* dst = a.mass + b * a.m_sb + h * a.m_sh;
+  float before[4];  // on their way beside the scores, not one after the other behind them
+#pragma unroll
+  for (int e = 0; e < 4; ++e) before[e] = dst[min(t + e, len - 1)];
   const int64_t bh = int64_t(b) * a.hkv + h;
   const int parts = (len + part_tokens - 1) / part_tokens;
   const int row = threadIdx.x >> 4;
@@ -211,19 +233,23 @@ __global__ __launch_bounds__(256) void mass_add_kernel(MassArgs a, int part_toke
     }
   }
   __syncthreads();
-  const int t = wg0 + 4 * int(threadIdx.x);
   if (t >= len) return;
   const float* src = a.scores + bh * a.rows * a.tokens + t;
   float w[4] = {};
-  for (int r = 0; r < a.rows; ++r) {
-    const f32x4 s = *reinterpret_cast<const f32x4*>(src + r * a.tokens);
+  for (int r0 = 0; r0 < a.rows; r0 += 8) {
+    f32x4 s[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] += fast_exp2(s[e] - s_stat[r][0]) * s_stat[r][1];
+    for (int i = 0; i < 8; ++i) s[i] = *reinterpret_cast<const f32x4*>(src + min(r0 + i, a.rows - 1) * a.tokens);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (r0 + i >= a.rows) break;  // uniform
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] += fast_exp2(s[i][e] - s_stat[r0 + i][0]) * s_stat[r0 + i][1];
+    }
   }
-  float* dst = a.mass + b * a.m_sb + h * a.m_sh + t;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    if (t + e < len) dst[e] += w[e];
+    if (t + e < len) dst[t + e] = before[e] + w[e];
   }
 }
 
@@ -630,6 +656,7 @@ extern "C" int ti_cache_mass(const void* q, int64_t q_stride_b, int64_t q_stride
   a.rows = rows;
   a.num_blocks32 = int32_t(num_blocks);
   a.page_size = page_size;
+  a.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(unsigned(page_size)) : -1;
   a.max_blocks = max_blocks_per_seq;
   a.parts = sz.parts;
   a.tokens = sz.tokens;
