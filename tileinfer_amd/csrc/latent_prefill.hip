@@ -13,12 +13,15 @@
 // one's softmax runs beside the other's products. A workgroup of eight waves gives each half of a tile's keys
 // to four of them and joins the two sums through LDS at the unit's end.
 //
-// Two schedules. Per unit: one workgroup each, the last query blocks, which see the most keys, first; no
-// workspace. Balanced: the tiles of all units are one list (by head, sequence, block), cut into equal runs,
-// one for each of the workgroups that fit the GPU; a unit that lies in one run is written by it, others
-// leave (m, l, o) parts in 32 bits that a second kernel joins in the order of the runs. Under a causal mask
-// a first chunk's units differ by a factor of its length, and few heads or a short chunk are fewer units
-// than CUs. Consecutive runs go to the same XCD, whose L2 then serves a head's keys to its blocks.
+// Schedules. Per unit: one workgroup each, the last query blocks, which see the most keys, first; no workspace.
+// Balanced: the tiles of all units are one list (by head, sequence, block), cut into equal runs, one for each of
+// the workgroups that fit the GPU; a unit that lies in one run is written by it, others leave (m, l, o) parts in
+// 32 bits that a second kernel joins in the order of the runs. It is for calls whose units do not fill the CUs.
+// Consecutive runs go to the same XCD, whose L2 then serves a head's keys to its blocks.
+//
+// Bound: the matrix units and the softmax's vector work for long chunks (8,192 queries with 24 heads 470 us,
+// 1,100 TFLOP/s), the longest unit for a first chunk (2,048 queries 50 us, 650 TFLOP/s), starts of units for short
+// ones (24 of 17 to 700 68 us).
 #include "lds_tiles.h"
 
 namespace ti {

@@ -166,7 +166,9 @@ def latent_decode_paged_fn(q: torch.Tensor, latent_cache: torch.Tensor, block_ta
     Returns:
         ``[B, H, L]`` or ``[B, N, H, L]`` in q's dtype: the weighted latents, to which the caller applies
         each head's ``Wv``. Query ``i`` of ``N`` sees the keys ``j <= seqlen_kv - N + i``; one that sees
-        nothing gives zeros. Block ids outside the cache below ``seqlen_kv`` are treated as absent.
+        nothing gives zeros. Block ids outside the cache below ``seqlen_kv`` are treated as absent. A cached
+        value that is not finite also reaches the queries of ``N`` that come before its token (a weight of
+        zero times it); what lies behind ``seqlen_kv`` reaches none.
     """
     # The call in its common form is checked and made in native code; None: another form, or one to refuse.
     stream = None if out is not None else _lib.native(q)
