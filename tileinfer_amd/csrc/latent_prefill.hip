@@ -308,36 +308,59 @@ __global__ __launch_bounds__(256 * KG, 2) void latent_prefill_kernel(ExpandedArg
           }
           __builtin_amdgcn_sched_barrier(0);
         }
+        // V of the first 32 keys is read beside the softmax, the others' beside its products.
+        u32x2 v[KP][NDT][2];
+        auto read_values = [&](int kp) __attribute__((always_inline)) {
+#pragma unroll
+          for (int dt = 0; dt < NDT; ++dt) {
+            const uint16_t* at = tile + (v_at ^ (16 * dt)) + 32 * kp * ROW;
+            v[kp][dt][0] = lds_read_tr4(at);
+            v[kp][dt][1] = lds_read_tr4(at + 16 * ROW);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        };
+        read_values(0);
         const bool whole = first_key + 16 * TT - 1 <= see_first && first_key + 16 * TT <= k_end;
-        u32x4 pb[2][KP];
+        if (!whole) {
 #pragma unroll
-        for (int rt = 0; rt < 2; ++rt) {
-          float x[4 * TT];
-#pragma unroll
-          for (int e = 0; e < 4 * TT; ++e) x[e] = s[e >> 2][rt][e & 3];
-          if (!whole) {
+          for (int rt = 0; rt < 2; ++rt) {
             const int lim = min(limit[rt], k_end - 1) - first_key - 4 * g;
 #pragma unroll
             for (int e = 0; e < 4 * TT; ++e) {
-              if (16 * (e >> 2) + (e & 3) > lim) x[e] = -INFINITY;
+              if (16 * (e >> 2) + (e & 3) > lim) s[e >> 2][rt][e & 3] = -INFINITY;
             }
           }
-          float top = x[0];
+        }
+        float top[2];
 #pragma unroll
-          for (int e = 1; e < 4 * TT - 1; e += 2) top = max3(top, x[e], x[e + 1]);
-          top = row_group_max(max2(top, x[4 * TT - 1])) * a.scale_log2;  // a scale is positive
-          if (__builtin_amdgcn_ballot_w64(top > m[rt] + kSlack)) {  // m = -inf at first
-            const float mn = fmaxf(m[rt], top);
+        for (int rt = 0; rt < 2; ++rt) {
+          top[rt] = s[0][rt][0];
+#pragma unroll
+          for (int e = 1; e < 4 * TT - 1; e += 2) {
+            top[rt] = max3(top[rt], s[e >> 2][rt][e & 3], s[(e + 1) >> 2][rt][(e + 1) & 3]);
+          }
+          top[rt] = row_group_max(max2(top[rt], s[TT - 1][rt][3])) * a.scale_log2;  // a scale is positive
+        }
+        // One condition for both row tiles, so that their exponentials are one block.
+        if (__builtin_amdgcn_ballot_w64(top[0] > m[0] + kSlack || top[1] > m[1] + kSlack)) {  // m = -inf at first
+#pragma unroll
+          for (int rt = 0; rt < 2; ++rt) {
+            const float mn = fmaxf(m[rt], top[rt]);
             const float c = mn == -INFINITY ? 1.f : fast_exp2(m[rt] - mn);
             m[rt] = mn;
             l[rt] *= c;
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt) o[dt][rt] *= c;
           }
+        }
+        u32x4 pb[2][KP];
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) {
           const float base = m[rt] == -INFINITY ? 0.f : m[rt];
+          float x[4 * TT];
 #pragma unroll
           for (int e = 0; e < 4 * TT; ++e) {
-            x[e] = fast_exp2(fmaf(x[e], a.scale_log2, -base));
+            x[e] = fast_exp2(fmaf(s[e >> 2][rt][e & 3], a.scale_log2, -base));
             l[rt] += x[e];
           }
           // P is rounded to the inputs' type for the matrix unit, as in the paged prefill: at most half a
@@ -347,13 +370,12 @@ __global__ __launch_bounds__(256 * KG, 2) void latent_prefill_kernel(ExpandedArg
         }
 #pragma unroll
         for (int kp = 0; kp < KP; ++kp) {
+          if (kp + 1 < KP) read_values(kp + 1);
 #pragma unroll
           for (int dt = 0; dt < NDT; ++dt) {
-            const uint16_t* at = tile + (v_at ^ (16 * dt)) + 32 * kp * ROW;
-            const u32x2 lo = lds_read_tr4(at), hi = lds_read_tr4(at + 16 * ROW);
-            const u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
+            const u32x4 vv = {v[kp][dt][0][0], v[kp][dt][0][1], v[kp][dt][1][0], v[kp][dt][1][1]};
 #pragma unroll
-            for (int rt = 0; rt < 2; ++rt) o[dt][rt] = mfma16x16x32(v, pb[rt][kp], o[dt][rt], Tag{});
+            for (int rt = 0; rt < 2; ++rt) o[dt][rt] = mfma16x16x32(vv, pb[rt][kp], o[dt][rt], Tag{});
           }
         }
       }
