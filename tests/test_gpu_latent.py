@@ -166,6 +166,9 @@ PREFILLS = [
     # more units than CUs: one workgroup each
     (48, 64, BF16, [(700, 700), (1, 9), (50, 130)], True),
     (33, 128, F16, [(1100, 1100)], True),
+    # sequences in the order of their keys, equal and empty ones among them
+    (33, 64, BF16, [(300, 1500), (0, 900), (300, 1500), (1, 3000), (130, 131), (0, 0), (200, 2100)], True),
+    (40, 128, F16, [(200, 1100), (700, 1300), (129, 1100)], False),
     # long first chunks of few units: two key groups
     (40, 128, BF16, [(1100, 1100)], True),
     (20, 64, F16, [(1030, 1050), (1301, 1281)], True),

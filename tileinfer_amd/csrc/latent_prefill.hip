@@ -42,7 +42,7 @@ struct ExpandedArgs {
   int64_t o_st, o_sh;
   const int32_t* cu_q;
   const int32_t* cu_k;
-  int32_t total_q, total_k, causal, batch, heads, key_groups;
+  int32_t total_q, total_k, causal, batch, heads, key_groups, by_length;
   float scale_log2;
   // Balanced schedule (runs > 0): parts of cut units, and each sequence's first tile within a head's.
   int32_t runs;
@@ -193,8 +193,22 @@ __global__ __launch_bounds__(256 * KG, 2) void latent_prefill_kernel(ExpandedArg
     qb = lo;
     t_first = rel - s.before(qb);
   } else {
+    // A sequence's last blocks first; its blocks stay side by side, for their keys in L2 (last blocks of all
+    // sequences first: 24 chunks of up to 300 over up to 4,000 keys 274 us against 196). Long sequences in the
+    // order of their keys, so that the last units to start are short: 12 ragged chunks over up to 4,000 keys 129 us
+    // against 148, four prompts of 500 to 3,000 104 against 115. The order costs a unit about a microsecond: prompts
+    // of 17 to 700 stay as they come (67 us against 72).
     h = blockIdx.x;
     b = blockIdx.z;
+    if (a.by_length) {
+      const int len = lane < a.batch ? Seq(a, lane).k_len : -1;
+      int rank = 0;
+      for (int i = 0; i < a.batch; ++i) {
+        const int other = __builtin_amdgcn_readlane(len, i);
+        rank += other > len || (other == len && i < lane) ? 1 : 0;
+      }
+      b = __builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < a.batch && rank == int(blockIdx.z)));
+    }
     qb = Seq(a, b).blocks - 1 - int(blockIdx.y);
     if (qb < 0) return;
   }
@@ -641,6 +655,7 @@ extern "C" int ti_latent_prefill(const void* q, int64_t q_stride_t, int64_t q_st
     a.seq_tile = reinterpret_cast<int32_t*>(a.part_ml + z.ml_floats);
   }
   const int64_t longest = max_seqlen_q < total_q ? max_seqlen_q : total_q;
+  a.by_length = batch > 1 && batch <= 64 && total_k / 1024 >= batch;
   a.key_groups = prefill_key_groups(batch, total_q, total_k, num_heads, causal);
   if (ceil_div(longest, kRows) > 65535) return fail(TI_EINVAL, "%s: max_seqlen_q %d too long", who, max_seqlen_q);
   hipStream_t s = static_cast<hipStream_t>(stream);
