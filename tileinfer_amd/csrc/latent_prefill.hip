@@ -13,7 +13,8 @@
 // one's softmax runs beside the other's products. A workgroup of eight waves gives each half of a tile's keys
 // to four of them and joins the two sums through LDS at the unit's end.
 //
-// Schedules. Per unit: one workgroup each, the last query blocks, which see the most keys, first; no workspace.
+// Schedules. Per unit: one workgroup each, the last query blocks, which see the most keys, first, and long
+// sequences in the order of their keys; no workspace.
 // Balanced: the tiles of all units are one list (by head, sequence, block), cut into equal runs, one for each of
 // the workgroups that fit the GPU; a unit that lies in one run is written by it, others leave (m, l, o) parts in
 // 32 bits that a second kernel joins in the order of the runs. It is for calls whose units do not fill the CUs.
@@ -617,8 +618,8 @@ extern "C" int ti_latent_prefill(const void* q, int64_t q_stride_t, int64_t q_st
       !vec_rows(key_rope, key_stride_t, 0) || !vec_rows(out, out_stride_t, out_stride_h)) {
     return fail(TI_EINVAL, "%s: rows must be 16-byte aligned", who);
   }
-  // A tile's rows are reached by 32-bit offsets.
   if (!(scale > 0.f)) return fail(TI_EINVAL, "%s: scale %g is not positive", who, double(scale));
+  // A tile's rows are reached by 32-bit offsets.
   if (kv_stride_t < 0 || key_stride_t < 0 || kv_stride_t >= (1 << 24) || key_stride_t >= (1 << 24)) {
     return fail(TI_EINVAL, "%s: token strides %lld, %lld of kv and key_rope must be in [0, 2^24)", who,
                 static_cast<long long>(kv_stride_t), static_cast<long long>(key_stride_t));
