@@ -308,13 +308,15 @@ def latent_prefill_fn(q: torch.Tensor, kv: torch.Tensor, key_rope: torch.Tensor,
     if total_q == 0 or b == 0:
         return out
     q, kv, key_rope = _as_rows(q), _as_rows(kv), _as_rows(key_rope)
+    # Held until the launch: a copy freed before it is handed out again, for instance to the next copy.
+    cu_seqlens_q, cu_seqlens_k = cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous()
     with _lib.on(dev):
         nbytes = _prefill_workspace(b, total_q, total_k, h, d, torch.cuda.current_device())
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         _lib.check(_lib.load().ti_latent_prefill(
             q.data_ptr(), q.stride(0), q.stride(1), kv.data_ptr(), kv.stride(0), kv.stride(1),
-            key_rope.data_ptr(), key_rope.stride(0), cu_seqlens_q.contiguous().data_ptr(),
-            cu_seqlens_k.contiguous().data_ptr(), out.data_ptr(), out.stride(0), out.stride(1),
+            key_rope.data_ptr(), key_rope.stride(0), cu_seqlens_q.data_ptr(),
+            cu_seqlens_k.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1),
             None if ws is None else ws.data_ptr(), nbytes, b, total_q,
             total_k, max_seqlen_q, h, d, ROPE_DIM, int(bool(causal)), scale, code,
             _lib.stream_handle(dev)))
