@@ -140,13 +140,15 @@ def qknorm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     q = q if _rows_ok(q) else q.contiguous()
     k = k if _rows_ok(k) else k.contiguous()
     v = v if _rows_ok(v) else v.contiguous()
+    # Held until the launch: a copy freed before it is handed out again, for instance to the next copy.
+    q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
     slot_mapping = slot_mapping.contiguous()
     if q_out is None:
         q_out = torch.empty((t, hq, d), dtype=dt, device=dev)
     _lib.check(_lib.load().ti_qknorm_rope_append(
         q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-        v.data_ptr(), v.stride(0), v.stride(1), q_weight.contiguous().data_ptr(),
-        k_weight.contiguous().data_ptr(), cos.data_ptr(), sin.data_ptr(), cs_stride,
+        v.data_ptr(), v.stride(0), v.stride(1), q_weight.data_ptr(),
+        k_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), cs_stride,
         q_out.data_ptr(), q_out.stride(0), q_out.stride(1), k_cache.data_ptr(),
         v_cache.data_ptr(), k_cache.stride(0), slot_mapping.data_ptr(), k_cache.shape[0], t, hq,
         hkv, d, rd, float(eps), code, _lib.stream_handle(dev)))
