@@ -4,7 +4,8 @@ import pytest
 import torch
 
 from helpers import bits, say
-from tileinfer_amd.kernels import latent_prefill_fn
+from oracle import ref_latent as ref
+from tileinfer_amd.kernels import latent_decode_paged_fn, latent_prefill_fn
 
 pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
@@ -25,3 +26,52 @@ def test_prefill_offsets_as_columns_of_one_table(heads, dev):
     for _ in range(3):
         got = latent_prefill_fn(q, kv, kr, both[:, 0], both[:, 1], 40, out=torch.zeros_like(want))
         assert torch.equal(bits(got), bits(want))
+
+
+def _right(got, exact, limit):
+    got = got.double().cpu()
+    assert torch.isfinite(got).all() and ((got - exact).abs() <= limit).all()
+
+
+@pytest.mark.parametrize("heads,q_len,k_len,at", [
+    (2, 200, 240, 70), (2, 200, 240, 130), (2, 200, 205, 191), (150, 200, 240, 130),  # cut units; one workgroup a unit
+    (16, 2500, 2500, 70), (16, 2500, 2500, 2431)])                                    # two key groups
+@pytest.mark.parametrize("what", ["inf", "nan"])
+def test_prefill_reach_of_a_value_that_is_not_finite(heads, q_len, k_len, at, what, dev):
+    """Queries whose 32 see no key of the value's 64 are right; a key that is not finite reaches only those that see it."""
+    say(f"latent prefill, {what} at {at}, H={heads} {q_len}/{k_len}")
+    q, kv, kr = _randn(dev, q_len, heads, 128), _randn(dev, k_len, heads, 128, seed=1), _randn(dev, k_len, 64, seed=2)
+    cu_q, cu_k = (torch.tensor([0, n], dtype=torch.int32, device=dev) for n in (q_len, k_len))
+    offset = k_len - q_len
+    group = next(g for g in range(q_len) if offset + min(32 * g + 31, q_len - 1) >= at // 64 * 64)
+    n = min(32 * group, 96)  # rows compared
+    exact, limit = ref.latent_prefill(q[:n].cpu(), kv.cpu(), kr.cpu(), [0, n], [0, offset + n], 128 ** -0.5)
+    bad = kv.clone()
+    bad[at, :, 64:] = float(what)
+    out = latent_prefill_fn(q, bad, kr, cu_q, cu_k, q_len)
+    assert torch.isfinite(out[:32 * group]).all()
+    _right(out[:n], exact, limit)
+    assert not torch.isfinite(out[max(0, at - offset):]).any()
+    plain = latent_prefill_fn(q, kv, kr, cu_q, cu_k, q_len)
+    bad = kv.clone()
+    bad[at, :, :64] = float("nan")
+    out = latent_prefill_fn(q, bad, kr, cu_q, cu_k, q_len)
+    first = max(0, at - offset)
+    assert torch.equal(bits(out[:first]), bits(plain[:first])) and torch.isnan(out[first:]).all()
+
+
+def test_decode_reach_of_a_row_that_is_not_finite(dev):
+    """It stays in its sequence; its rotated part reaches only the queries that see it."""
+    say("latent decode, rows that are not finite")
+    cache = _randn(dev, 12, 16, 1, 320)
+    table = torch.arange(12, dtype=torch.int32, device=dev).view(3, 4)
+    lens = torch.tensor([40, 50, 64], dtype=torch.int32, device=dev)
+    q = _randn(dev, 3, 3, 24, 320, seed=1)
+    plain = latent_decode_paged_fn(q, cache, table, lens, scale=0.05)
+    for part in (slice(0, 256), slice(256, 320)):
+        bad = cache.clone()
+        bad[7, 1, 0, part] = float("nan")  # token 49 of sequence 1, its last one
+        out = latent_decode_paged_fn(q, bad, table, lens, scale=0.05)
+        assert torch.equal(bits(out[[0, 2]]), bits(plain[[0, 2]])) and torch.isnan(out[1, 2]).all()
+        if part.start:
+            assert torch.equal(bits(out[1, :2]), bits(plain[1, :2]))

@@ -267,8 +267,10 @@ def latent_prefill_fn(q: torch.Tensor, kv: torch.Tensor, key_rope: torch.Tensor,
         scale: factor of the scores, ``(D + 64) ** -0.5`` by default
     Returns:
         ``[total_q, H, D]`` in q's dtype; rows that see no key are zero, rows of no sequence are not
-        written. A value that is not finite reaches, besides the queries that see its key, those before it
-        in the same sequence whose keys end in the same 64 (a weight of zero times it).
+        written. A value (kv's second half) that is not finite can reach queries that do not see its key (a
+        weight of zero times it): those that share their 32 queries, counted from the chunk's start, with one
+        that sees any of its 64 keys, counted from the sequence's start. Keys that are not finite and not
+        seen reach none.
     """
     if q.dim() != 3 or kv.dim() != 3 or key_rope.dim() != 2:
         raise ValueError("q and kv must be [tokens, H, dims] and key_rope [tokens, 64]")
