@@ -546,14 +546,21 @@ PrefillSizes prefill_sizes(int32_t batch, int32_t total_q, int32_t total_k, int3
   return z;
 }
 
-// Key groups of a workgroup. Two share a unit's rows and halve its tiles' time, but one such workgroup fills a
-// CU, so nothing runs beside its start and end. They are for first chunks of few units, where the time is that
-// of the last, longest unit: 2,048 queries with 24 heads (384 units) 55 us against 65, 4,096 with 12 heads 91
-// against 111. Units of one length (2,048 behind 8,192) take 366 us against 316, more units (2,800 with 24
-// heads, 528) 87 against 83 and short ones (24 of 90, 20 heads) 21 against 15.
-int32_t prefill_key_groups(int32_t batch, int32_t total_q, int32_t total_k, int32_t heads, int32_t causal) {
+// Key groups of a workgroup. Two share a unit's rows and halve its tiles' time. They are for first chunks of few
+// units, where the time is that of the last, longest unit. At head_dim 128 such a workgroup fills a CU, at 64 two
+// fit; us with one group against two:
+//   head_dim 128: one of 2,048 with 24 heads (384 units) 60 / 50, one of 4,096 with 12 108 / 90, one of 1,100 with 40
+//     36 / 34, two of 2,048 with 16 77 / 61, two of 1,024 with 24 37 / 37; but four of 2,048 with 8 76 / 85, three of
+//     1,600 with 12 56 / 66, four of 1,024 with 16 45 / 51;
+//   head_dim 64: 45 / 42, 79 / 73 and 26 / 25 for the first three; but two of 2,048 55 / 58, two of 1,024 26 / 30, four
+//     of 2,048 55 / 58, four of 1,024 32 / 34.
+// More units gain nothing or lose (2,800 with 24 heads, 528 units: 82 / 85, 59 / 58; 8,192 with 24: 461 / 551, 311 /
+// 336), nor do units of one length (2,048 behind 8,192: 316 / 366) and short ones (24 of 90, 20 heads: 15 / 20).
+int32_t prefill_key_groups(int32_t batch, int32_t total_q, int32_t total_k, int32_t heads, int32_t head_dim,
+                           int32_t causal) {
   const bool few = ceil_div(total_q, kRows) * heads <= 2 * device_cu_count();
-  return causal && total_q == total_k && total_q / 8 / kRows >= batch && few ? 2 : 1;
+  const bool long_ones = total_q / 8 / kRows >= batch && batch <= (head_dim == 128 ? 2 : 1);
+  return causal && total_q == total_k && long_ones && few ? 2 : 1;
 }
 
 template <int DN, typename Tag>
@@ -657,7 +664,7 @@ extern "C" int ti_latent_prefill(const void* q, int64_t q_stride_t, int64_t q_st
   }
   const int64_t longest = max_seqlen_q < total_q ? max_seqlen_q : total_q;
   a.by_length = batch > 1 && batch <= 64 && total_k / 1024 >= batch;
-  a.key_groups = prefill_key_groups(batch, total_q, total_k, num_heads, causal);
+  a.key_groups = prefill_key_groups(batch, total_q, total_k, num_heads, head_dim, causal);
   if (ceil_div(longest, kRows) > 65535) return fail(TI_EINVAL, "%s: max_seqlen_q %d too long", who, max_seqlen_q);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool bf16 = dtype == TI_DTYPE_BF16;
