@@ -5,7 +5,8 @@ import torch
 
 from helpers import bits, say
 from oracle import ref_latent as ref
-from tileinfer_amd.kernels import latent_decode_paged_fn, latent_prefill_fn
+from tileinfer_amd.kernels import (evict_kvcache, gqa_prefill_paged_fn, latent_decode_paged_fn,
+                                   latent_prefill_fn)
 
 pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
@@ -75,3 +76,24 @@ def test_decode_reach_of_a_row_that_is_not_finite(dev):
         assert torch.equal(bits(out[[0, 2]]), bits(plain[[0, 2]])) and torch.isnan(out[1, 2]).all()
         if part.start:
             assert torch.equal(bits(out[1, :2]), bits(plain[1, :2]))
+
+
+def test_host_numbers_beyond_32_bits(dev):
+    """A bound on the chunks' length may be any number; a budget that does not fit the call is refused."""
+    say("host numbers beyond 32 bits")
+    cu = torch.tensor([0, 40, 90], dtype=torch.int32, device=dev)
+    q, kv, kr = _randn(dev, 90, 3, 192), _randn(dev, 90, 3, 256, seed=1), _randn(dev, 90, 64, seed=2)
+    want = latent_prefill_fn(q, kv, kr, cu, cu, 50)
+    for bound in (2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 33 + 7, 2 ** 70):
+        assert torch.equal(bits(latent_prefill_fn(q, kv, kr, cu, cu, bound, out=torch.zeros_like(want))), bits(want))
+    k, v = _randn(dev, 8, 16, 2, 128), _randn(dev, 8, 16, 2, 128, seed=1)
+    table = torch.arange(8, dtype=torch.int32, device=dev).view(2, 4)
+    q, lens = _randn(dev, 90, 4, 128), torch.tensor([40, 60], dtype=torch.int32, device=dev)
+    want = gqa_prefill_paged_fn(q, k, v, table, cu, lens, 50)
+    for bound in (2 ** 31, 2 ** 32, 2 ** 70):
+        got = gqa_prefill_paged_fn(q, k, v, table, cu, lens, bound, out=torch.zeros_like(want))
+        assert torch.equal(bits(got), bits(want))
+    mass = torch.rand(2, 2, 32, device=dev)
+    for budget in (2 ** 31, 2 ** 32 + 16, 2 ** 70):
+        with pytest.raises(ValueError, match="budget"):
+            evict_kvcache(k, v, mass, table[:, :2], lens, table[:, 2:], budget, 16)

@@ -34,6 +34,7 @@ TI_DECODE_SCALAR = 2
 TI_DECODE_REUSE_KV = 0x10
 TI_DECODE_STREAM_KV = 0x20
 ABI_VERSION = 8
+INT32_MAX = 2 ** 31 - 1  # ctypes cuts larger host ints to 32 bits without an error
 
 # Every symbol declared in include/tileinfer_amd.h, with its ctypes signature.
 _c_i32, _c_i64, _c_vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p

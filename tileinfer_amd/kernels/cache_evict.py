@@ -142,7 +142,7 @@ def evict_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor | None, mass: tor
         new_block_table: ``[B, W2]`` int32 with room for ``min(budget, W * page_size)`` tokens where a
             sequence has them (-1 beyond a sequence's kept tokens). Its blocks must be fresh: in no table
             that is still used, this call's ``block_table`` among them.
-        budget, sinks, recent: host ints, ``sinks + recent <= budget``
+        budget, sinks, recent: host ints, ``sinks + recent <= budget < 2^31``
     Returns:
         ``(seqlen, kept, mass)``: the new lengths ``[B]`` int32, the kept positions ``[B, H_kv, budget]`` int32
         (ascending, -1 behind the last) and their masses ``[B, H_kv, capacity]`` (0 behind the last).
@@ -167,8 +167,8 @@ def evict_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor | None, mass: tor
         if v_cache.shape != k_cache.shape or v_cache.dtype != dt or v_cache.device != dev:
             raise ValueError("v_cache must have k_cache's shape, dtype and device")
     budget, sinks, recent = int(budget), int(sinks), int(recent)
-    if budget <= 0 or sinks < 0 or recent < 0 or sinks + recent > budget:
-        raise ValueError(f"budget {budget} must be positive and hold sinks {sinks} and recent {recent}")
+    if not 0 < budget <= _lib.INT32_MAX or sinks < 0 or recent < 0 or sinks + recent > budget:
+        raise ValueError(f"budget {budget} must be positive, below 2^31 and hold sinks {sinks} and recent {recent}")
     if block_table.dim() != 2:
         raise ValueError(f"block_table must be [B, W], got {tuple(block_table.shape)}")
     b = block_table.shape[0]

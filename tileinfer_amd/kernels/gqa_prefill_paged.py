@@ -231,6 +231,7 @@ def gqa_prefill_paged_fn(
     max_seqlen_q = int(max_seqlen_q)
     if max_seqlen_q < 0:
         raise ValueError(f"max_seqlen_q must be >= 0, got {max_seqlen_q}")
+    max_seqlen_q = min(max_seqlen_q, _lib.INT32_MAX)  # no chunk is longer
     if not _aligned_rows(q):
         q = q.contiguous()
     if out is None:

@@ -301,6 +301,7 @@ def latent_prefill_fn(q: torch.Tensor, kv: torch.Tensor, key_rope: torch.Tensor,
     max_seqlen_q = int(max_seqlen_q)
     if max_seqlen_q < 0:
         raise ValueError(f"max_seqlen_q {max_seqlen_q} is negative")
+    max_seqlen_q = min(max_seqlen_q, _lib.INT32_MAX)  # no chunk is longer
     scale = _scale(row ** -0.5 if scale is None else scale)
     if out is None:
         out = torch.empty((total_q, h, d), dtype=dt, device=dev)
