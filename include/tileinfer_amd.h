@@ -448,7 +448,7 @@ int64_t ti_gqa_decode_scratch_bytes(void);
  * (cos, sin [n_tokens, >= 32] at cs_stride_t, 0 for one row; columns from 32 on are not read). 32-bit
  * arithmetic, each value rounded once. Slots that are negative or >= num_slots are skipped; duplicate
  * slots within a call are unsupported. q_out may be q_rope itself (same strides). All rows 16-byte
- * aligned, strides multiples of 8 elements.
+ * aligned, strides multiples of 8 elements. At most 2^24 workgroups: about 2^29 rotated rows a call.
  */
 int ti_latent_rope_append(const void* q_rope, int64_t q_stride_t, int64_t q_stride_h, void* q_out,
                           int64_t out_stride_t, int64_t out_stride_h, const void* latent,
@@ -473,7 +473,7 @@ int ti_latent_decode_workspace_bytes(int32_t batch, int32_t new_tokens, int32_t 
  * outside [0, num_blocks) below seqlen are absent (masked, never loaded); entries at or beyond
  * ceil(seqlen / page_size) are not read. Any page_size; scale positive.
  *   q        [batch, new_tokens, num_heads, latent_dim + rope_dim], last dim contiguous, strides multiples
- *            of 8 elements
+ *            of 8 elements; fewer than 2^24 rows in all
  *   latent_cache  contiguous rows; num_blocks * page_size < 2^31
  *   out      [batch, new_tokens, num_heads, latent_dim] contiguous
  *   workspace  ti_latent_decode_workspace_bytes bytes, 16-byte aligned, contents need no initialisation
@@ -528,6 +528,7 @@ int ti_cache_mass_workspace_bytes(int32_t batch, int32_t new_tokens, int32_t num
  *   q        [batch, new_tokens, num_q_heads, head_dim], last dim contiguous, strides multiples of 8
  *   k_cache  [num_blocks, page_size, num_kv_heads, head_dim] contiguous
  *   mass     [batch, num_kv_heads, >= max_blocks_per_seq * page_size] fp32 at mass_stride_b / _h
+ * max_blocks_per_seq * page_size * num_kv_heads is at most about 2^31 (2^30 for a window of latent rows of 576).
  * No reference counterpart (the reference never drops cached tokens).
  */
 int ti_cache_mass(const void* q, int64_t q_stride_b, int64_t q_stride_t, int64_t q_stride_h,

@@ -1,0 +1,23 @@
+"""Sizes that no launch of the latent and eviction entry points takes are refused before the first one (no GPU needed)."""
+import ctypes
+
+from test_latent_host import _addr
+from tileinfer_amd import _lib
+
+
+def test_more_work_items_than_a_launch_counts():
+    """A launch counts its work items along x in 32 bits, 2^24 workgroups of 256: where a call's second launch has more, its
+    first one must not run either, and where its first one has, the second must not add up what nothing wrote."""
+    lib, n, p = _lib.load(), ctypes.c_int64(), _addr()
+    assert lib.ti_latent_decode_workspace_bytes(1 << 14, 7, 128, 512, ctypes.byref(n)) == _lib.TI_OK
+    assert lib.ti_latent_decode_workspace_bytes(1 << 14, 8, 128, 512, ctypes.byref(n)) == _lib.TI_EINVAL
+    assert lib.ti_latent_decode_paged(p, 8 * 576, 576, 576, p, p, 4, p, p, p, 1 << 40, 1 << 14, 8, 128, 512, 64, 16, 8, 4,
+                                      0.1, 0, None) == _lib.TI_EINVAL
+    assert b"2^24" in lib.ti_last_error()
+    assert lib.ti_cache_mass_workspace_bytes(1, 1, 8, 1, 128, 16, 1 << 26, ctypes.byref(n)) == _lib.TI_OK
+    assert lib.ti_cache_mass_workspace_bytes(1, 1, 8, 8, 128, 16, 1 << 26, ctypes.byref(n)) == _lib.TI_EINVAL
+    assert lib.ti_cache_mass_workspace_bytes(1, 17, 1, 1, 576, 16, 1 << 26, ctypes.byref(n)) == _lib.TI_EINVAL
+    assert lib.ti_cache_mass(p, 1024, 1024, 128, p, p, 4, p, p, 1 << 33, 1 << 30, p, 1 << 60, 1, 1, 8, 8, 128, 16, 8, 1 << 26,
+                             0.1, 0, None) == _lib.TI_EINVAL
+    assert lib.ti_latent_rope_append(p, 192, 64, p, 192, 64, p, 512, p, 64, p, 1.0, p, p, 64, p, 576, 8, p, 1 << 25, 24, 512,
+                                     64, 1e-6, 0, None) == _lib.TI_EINVAL

@@ -550,8 +550,9 @@ int check_mass(const char* who, int32_t batch, int32_t new_tokens, int32_t hq, i
       int64_t(new_tokens) * (hq / hkv) > (1 << 20)) {
     return fail(TI_EINVAL, "%s: bad sizes batch=%d new_tokens=%d heads=%d/%d", who, batch, new_tokens, hq, hkv);
   }
+  const int part_tokens = 64 * tiles_of(d, new_tokens * (hq / hkv) <= kFewRows);
   if (page_size <= 0 || max_blocks < 0 || int64_t(max_blocks) * page_size > INT32_MAX - 1024 ||
-      ceil_div(int64_t(max_blocks) * page_size, 64) * hkv > INT32_MAX) {
+      ceil_div(int64_t(max_blocks) * page_size, part_tokens) * hkv > kMaxGridX) {
     return fail(TI_EINVAL, "%s: bad cache page_size=%d max_blocks_per_seq=%d", who, page_size, max_blocks);
   }
   return TI_OK;

@@ -564,9 +564,11 @@ int check_latent(const char* who, int32_t batch, int32_t new_tokens, int32_t hea
     return fail(TI_EUNSUPPORTED, "%s: latent_dim %d not built (256, 512)", who, latent);
   }
   if (rope != kRope) return fail(TI_EUNSUPPORTED, "%s: rope_dim %d not built (64)", who, rope);
-  if (batch < 0 || new_tokens <= 0 || heads <= 0 || int64_t(new_tokens) * heads > (1 << 24) ||
-      int64_t(batch) * new_tokens * heads > INT32_MAX) {
-    return fail(TI_EINVAL, "%s: bad sizes batch=%d new_tokens=%d heads=%d", who, batch, new_tokens, heads);
+  // The join has a workgroup for each row.
+  if (batch < 0 || new_tokens <= 0 || heads <= 0 || int64_t(new_tokens) * heads > kMaxGridX ||
+      int64_t(batch) * new_tokens * heads > kMaxGridX) {
+    return fail(TI_EINVAL, "%s: bad sizes batch=%d new_tokens=%d heads=%d (below 2^24 rows in all)", who, batch,
+                new_tokens, heads);
   }
   return TI_OK;
 }

@@ -156,6 +156,12 @@ extern "C" int ti_latent_rope_append(const void* q_rope, int64_t q_stride_t, int
                          !vec_rows(q_out, out_stride_t, out_stride_h)))) {
     return fail(TI_EINVAL, "%s: rows must be 16-byte aligned", who);
   }
+  const int64_t latent_waves = ceil_div(n_tokens, 512 / latent_dim);
+  const int64_t rope_waves = ceil_div(int64_t(n_tokens) * (num_heads + 1), 8);
+  const int64_t blocks = ceil_div(latent_waves + rope_waves, 4);
+  if (blocks > kMaxGridX) {
+    return fail(TI_EINVAL, "%s: %d tokens of %d heads are more than one call takes", who, n_tokens, num_heads);
+  }
   LatentInArgs a{};
   a.q = static_cast<const uint16_t*>(q_rope);
   a.q_st = q_stride_t;
@@ -179,11 +185,9 @@ extern "C" int ti_latent_rope_append(const void* q_rope, int64_t q_stride_t, int
   a.heads = num_heads;
   a.offset = weight_offset;
   a.eps = eps;
-  a.latent_waves = ceil_div(n_tokens, 512 / latent_dim);
-  const int64_t rope_waves = ceil_div(int64_t(n_tokens) * (num_heads + 1), 8);
-  const unsigned blocks = unsigned(ceil_div(a.latent_waves + rope_waves, 4));
+  a.latent_waves = latent_waves;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == TI_DTYPE_BF16) launch_latent_in<Bf16>(a, latent_dim, blocks, s);
-  else launch_latent_in<F16>(a, latent_dim, blocks, s);
+  if (dtype == TI_DTYPE_BF16) launch_latent_in<Bf16>(a, latent_dim, unsigned(blocks), s);
+  else launch_latent_in<F16>(a, latent_dim, unsigned(blocks), s);
   return check_launch(who);
 }

@@ -17,6 +17,9 @@ int check_launch(const char* what);
 // Number of compute units of the current device (cached per device id).
 int device_cu_count();
 
+// Workgroups of at most 256 threads that a launch takes along x: its work items there are counted in 32 bits.
+constexpr int64_t kMaxGridX = (int64_t(1) << 24) - 1;
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // 4 x 32-bit registers: one 16-byte global access, or the 8 x 16-bit operand of a

@@ -156,7 +156,7 @@ def latent_decode_paged_fn(q: torch.Tensor, latent_cache: torch.Tensor, block_ta
 
     Args:
         q: ``[B, H, L + 64]`` for one new token a sequence, or ``[B, N, H, L + 64]`` for its last ``N``
-            (drafted tokens, a short chunk): ``[q_nope @ Wk^T | rotated part]``
+            (drafted tokens, a short chunk): ``[q_nope @ Wk^T | rotated part]``; B N H below 2^24
         latent_cache: ``[num_blocks, block_size, 1, L + 64]``, contiguous; the new tokens' rows are in it
         block_table: ``[B, W]`` int32 (-1 padding allowed past each sequence)
         seqlen_kv: ``[B]`` int32 context lengths, the new tokens included
