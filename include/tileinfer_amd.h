@@ -497,7 +497,8 @@ int ti_latent_prefill_workspace_bytes(int32_t batch, int32_t total_q, int32_t to
  *   out[i, h] = softmax_j( scale * (q[i, h, :head_dim] . kn[j, h] + q[i, h, head_dim:] . key_rope[j]) ) @ v[j, h]
  * with the causal mask aligned to the last key (query i sees keys j <= k_len - q_len + i), or without it.
  * A query that sees nothing gives zeros. max_seqlen_q is at least the longest chunk; rows of longer ones
- * are not all written. Offsets beyond total_q / total_k are cut off. head_dim 128 or 64, rope_dim 64;
+ * are not all written. Offsets beyond total_q / total_k are cut off, a sequence whose end lies before its start is
+ * empty. head_dim 128 or 64, rope_dim 64;
  * rows 16-byte aligned, strides multiples of 8 elements, token strides of kv and key_rope below 2^24, scale
  * positive. With a workspace of ti_latent_prefill_workspace_bytes (16-byte aligned, contents need no
  * initialisation) units of 128 query rows may be cut between workgroups and joined; with NULL every unit is

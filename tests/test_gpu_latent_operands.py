@@ -97,3 +97,19 @@ def test_host_numbers_beyond_32_bits(dev):
     for budget in (2 ** 31, 2 ** 32 + 16, 2 ** 70):
         with pytest.raises(ValueError, match="budget"):
             evict_kvcache(k, v, mass, table[:, :2], lens, table[:, 2:], budget, 16)
+
+
+@pytest.mark.parametrize("heads", [2, 150])
+def test_prefill_offsets_that_go_back(heads, dev):
+    """A sequence whose end lies before its start is empty, one that starts inside another has its own keys; offsets stay
+    within the tensors. Rows that two sequences claim get either result."""
+    say(f"latent prefill offsets that go back, H={heads}")
+    q, kv, kr = _randn(dev, 300, heads, 128), _randn(dev, 500, heads, 128, seed=1), _randn(dev, 500, 64, seed=2)
+    i = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    out = latent_prefill_fn(q, kv, kr, i(-5, 200, 100, 2 ** 31 - 1), i(0, 320, 40, 2 ** 31 - 1), 300)
+    first = latent_prefill_fn(q[:200], kv[:320], kr[:320], i(0, 200), i(0, 320), 200, out=torch.empty_like(out[:200]))
+    last = latent_prefill_fn(q[100:], kv[40:], kr[40:], i(0, 200), i(0, 460), 200)
+    near = dict(rtol=2.0 ** -6, atol=2.0 ** -7)  # other cuts: P and the output rounded apart
+    torch.testing.assert_close(out[:100], first[:100], **near)
+    torch.testing.assert_close(out[200:], last[100:], **near)
+    assert torch.isfinite(out[100:200]).all()

@@ -21,3 +21,13 @@ def test_more_work_items_than_a_launch_counts():
                              0.1, 0, None) == _lib.TI_EINVAL
     assert lib.ti_latent_rope_append(p, 192, 64, p, 192, 64, p, 512, p, 64, p, 1.0, p, p, 64, p, 576, 8, p, 1 << 25, 24, 512,
                                      64, 1e-6, 0, None) == _lib.TI_EINVAL
+
+
+def test_a_list_of_tiles_that_offsets_could_make_too_long_is_not_cut():
+    """Cut units are counted in 32 bits; offsets that go back could give each of 65,535 sequences all 8 blocks and 1,024
+    tiles of 16 heads."""
+    lib, n = _lib.load(), ctypes.c_int64(1)
+    assert lib.ti_latent_prefill_workspace_bytes(65535, 1024, 65536, 16, 128, ctypes.byref(n)) == _lib.TI_OK
+    assert n.value == 0
+    assert lib.ti_latent_prefill_workspace_bytes(24, 2048, 400000, 16, 128, ctypes.byref(n)) == _lib.TI_OK
+    assert n.value > 0

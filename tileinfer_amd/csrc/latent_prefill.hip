@@ -537,7 +537,8 @@ struct PrefillSizes {
 PrefillSizes prefill_sizes(int32_t batch, int32_t total_q, int32_t total_k, int32_t heads, int32_t head_dim) {
   PrefillSizes z{};
   const int64_t cus = device_cu_count(), slots = 2 * cus, blocks = ceil_div(total_q, kRows);
-  const int64_t most = (blocks + batch) * (ceil_div(total_k, kKeys) + 1) * heads;  // tiles at most
+  // The list is counted in 32 bits on the device. Offsets that go back may give every sequence all blocks and keys.
+  const int64_t most = batch * blocks * ceil_div(total_k, kKeys) * heads;
   if (blocks * heads > cus || most > INT32_MAX) return z;
   z.runs = int32_t(slots);
   z.o_floats = slots * 2 * kRows * head_dim;
