@@ -415,13 +415,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void latent_decode_kernel(LatentArg
 #pragma unroll
           for (int dt = 0; dt < NDT; ++dt) o[dt] *= c;
         }
-        const float base = m == -INFINITY ? 0.f : m;
+        const float base = m == -INFINITY ? 0.f : m - weight_lift(Tag{});
         score(i + 1);
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = fast_exp2(x[e] - base);
         l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
         // P is rounded to the cache's type for the matrix unit, as in the paged decode: at most half a
-        // step of each weight, while l sums the unrounded ones in 32 bits.
+        // step of each weight (lifted in fp16, weight_lift), while l sums the unrounded ones in 32 bits.
         const u32x4 pb = {pack2(x[0], x[1], Tag{}), pack2(x[2], x[3], Tag{}), pack2(x[4], x[5], Tag{}),
                           pack2(x[6], x[7], Tag{})};
 #pragma unroll

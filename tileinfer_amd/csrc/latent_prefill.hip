@@ -371,7 +371,7 @@ __global__ __launch_bounds__(256 * KG, 2) void latent_prefill_kernel(ExpandedArg
         u32x4 pb[2][KP];
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt) {
-          const float base = m[rt] == -INFINITY ? 0.f : m[rt];
+          const float base = m[rt] == -INFINITY ? 0.f : m[rt] - weight_lift(Tag{});
           float x[4 * TT];
 #pragma unroll
           for (int e = 0; e < 4 * TT; ++e) {
@@ -379,7 +379,7 @@ __global__ __launch_bounds__(256 * KG, 2) void latent_prefill_kernel(ExpandedArg
             l[rt] += x[e];
           }
           // P is rounded to the inputs' type for the matrix unit, as in the paged prefill: at most half a
-          // step of each weight, while l sums the unrounded ones in 32 bits.
+          // step of each weight (lifted in fp16, weight_lift), while l sums the unrounded ones in 32 bits.
 #pragma unroll
           for (int e = 0; e < 2 * TT; ++e) pb[rt][e >> 2][e & 3] = pack2(x[2 * e], x[2 * e + 1], Tag{});
         }

@@ -65,4 +65,12 @@ __device__ __forceinline__ float row_group_sum(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// Exp2 units by which softmax weights are lifted before they are rounded to 16 bits; the sums carry the same factor, which
+// the division by l takes out. An fp16 weight has steps of 2^-24 at least, so that 60,000 of 2^-25.6 of their row's
+// greatest (the tail behind a first token that takes most of the attention) would all round to zero, while l counts
+// them. Seven, and the eight by which a maximum may rise before it is taken over, stay below fp16's 2^16. bf16 has the
+// exponents of 32 bits and needs none.
+__device__ __forceinline__ constexpr float weight_lift(Bf16) { return 0.f; }
+__device__ __forceinline__ constexpr float weight_lift(F16) { return 7.f; }
+
 }  // namespace ti
