@@ -260,9 +260,7 @@ constexpr int kQRows = 32;
 
 template <int D>
 __device__ __forceinline__ int q_place(int r) {
-  if constexpr (D % 128 == 0) return ((2 * r) & 15) ^ ((r & 8) ? 9 : 0);
-  const int u = (r >> 1) & 7;
-  return ((2 * u) & 7) ^ ((u & 4) ? 5 : 0);
+  return D % 128 == 0 ? swz16(r) : swz8(r);
 }
 
 // STATS: the rows' (max, 1 / sum) come too, behind the queries, a copy for each wave.

@@ -72,21 +72,9 @@ constexpr uint32_t kStreamTiles = 2048;
 // (one sequence of 700 tokens, 24 heads: 14.3 us against 16.1 with two; four of 1,000: 16.4 against 15.6).
 constexpr uint32_t kShortTiles = 48;
 
-// The list of `total` tiles cut into runs, the first `rest` of them one tile longer. All in 32 bits (the host
-// refuses longer lists): a 64-bit division takes about half a microsecond at the start of every workgroup.
-struct Runs {
-  uint32_t runs, base, rest;
-  __device__ __forceinline__ Runs(const LatentArgs& a, uint32_t total) {
-    runs = max(1u, min(uint32_t(a.runs), total / (total <= kShortTiles ? 1u : 2u)));
-    base = total / runs;
-    rest = total - base * runs;
-  }
-  __device__ __forceinline__ uint32_t start(uint32_t i) const { return i * base + min(i, rest); }
-  __device__ __forceinline__ uint32_t holding(uint32_t u) const {  // the run of position u
-    const uint32_t longer = rest * (base + 1);
-    return u < longer ? u / (base + 1) : rest + (u - longer) / base;
-  }
-};
+__device__ __forceinline__ Runs runs_of(const LatentArgs& a, uint32_t total) {
+  return Runs(uint32_t(a.runs), total, total <= kShortTiles ? 1u : 2u);
+}
 
 // One load of 16 bytes a lane into LDS, from base + off of each lane: lane i's land at byte lds + 16 i.
 // STREAM: with the nt bit, for bytes that are read once.
@@ -107,16 +95,6 @@ __device__ __forceinline__ void load_lds16_at(uint64_t src, const uint16_t* lds)
   } else {
     asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(m0) : "memory");
   }
-}
-
-// LDS places of 16-byte chunk c of a tile's row r: c ^ swz16(r) in the latents' rows (whole 256-byte
-// blocks), c ^ swz8(r) in the 128-byte rows of the rotated parts. A ds_read_b128 serves rows {0-3, 12-15}
-// of one chunk with rows {4-11} of its neighbour, a transposed read two neighbouring chunks of eight
-// rows; either way these are 16 different bank quads.
-__device__ __forceinline__ int swz16(int r) { return ((2 * r) & 15) ^ ((r & 8) ? 9 : 0); }
-__device__ __forceinline__ int swz8(int r) {
-  const int u = (r >> 1) & 7;
-  return ((2 * u) & 7) ^ ((u & 4) ? 5 : 0);
 }
 
 template <int N>
@@ -161,7 +139,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void latent_decode_kernel(LatentArg
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) a.first_tile[a.batch] = int(total);
   total *= uint32_t(a.row_blocks);
-  const Runs runs(a, total);
+  const Runs runs = runs_of(a, total);
   if (blockIdx.x >= runs.runs || total == 0) return;
   const uint32_t start = runs.start(blockIdx.x), end = runs.start(blockIdx.x + 1);
   int b = 0;
@@ -183,7 +161,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void latent_decode_kernel(LatentArg
   }
 
   // This lane's part of a tile's loads. Row r's latent is chunks [CH r, CH (r + 1)) of the stage, its
-  // rotated part 8 chunks behind the latents; a wave's load takes 64 chunks.
+  // rotated part 8 chunks behind the latents; a wave's load takes 64 chunks. Chunk c lies at c ^ swz16(r), of a rotated
+  // part at c ^ swz8(r).
   uint32_t lat_off[NLAT];
 #pragma unroll
   for (int i = 0; i < NLAT; ++i) {
@@ -479,7 +458,7 @@ __global__ __launch_bounds__(256) void latent_merge_kernel(LatentArgs a, int rb_
     if (group == 0) *reinterpret_cast<u32x2*>(dst) = u32x2{0, 0};
     return;
   }
-  const Runs runs(a, total);
+  const Runs runs = runs_of(a, total);
   const uint32_t u0 = uint32_t(f0) * a.row_blocks + rb * nt;
   const int i0 = int(runs.holding(u0)), i1 = int(runs.holding(u0 + nt - 1));
   if (i0 == i1) return;  // written by its run

@@ -90,32 +90,7 @@ struct Seq {
   }
 };
 
-// `total` tiles cut into runs, the first `rest` of them one tile longer (32 bits; the host takes the other
-// schedule for longer lists).
-constexpr uint32_t kMinRun = 4;
-struct Runs {
-  uint32_t runs, base, rest;
-  __device__ __forceinline__ Runs(const ExpandedArgs& a, uint32_t total) {
-    runs = max(1u, min(uint32_t(a.runs), total / kMinRun));
-    base = total / runs;
-    rest = total - base * runs;
-  }
-  __device__ __forceinline__ uint32_t start(uint32_t i) const { return i * base + min(i, rest); }
-  __device__ __forceinline__ uint32_t holding(uint32_t u) const {  // the run of position u
-    const uint32_t longer = rest * (base + 1);
-    return u < longer ? u / (base + 1) : rest + (u - longer) / base;
-  }
-};
-
-// LDS places of 16-byte chunk c of row r: c ^ swz16(r) in rows of whole 256-byte blocks (kn and v),
-// c ^ swz8(r) in the 128-byte rows of k_r. A ds_read_b128 serves rows {0-3, 12-15} of one chunk with rows
-// {4-11} of its neighbour, a transposed read two neighbouring chunks of eight rows; either way these
-// are 16 different bank quads.
-__device__ __forceinline__ int swz16(int r) { return ((2 * r) & 15) ^ ((r & 8) ? 9 : 0); }
-__device__ __forceinline__ int swz8(int r) {
-  const int u = (r >> 1) & 7;
-  return ((2 * u) & 7) ^ ((u & 4) ? 5 : 0);
-}
+constexpr uint32_t kMinRun = 4;  // tiles of a run (the host takes the other schedule for lists beyond 32 bits)
 
 // KG: key groups of four waves each; a group takes 64 / KG keys of a tile.
 template <int DN, int KG, bool BALANCED, typename Tag>
@@ -157,7 +132,7 @@ __global__ __launch_bounds__(256 * KG, 2) void latent_prefill_kernel(ExpandedArg
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) a.seq_tile[a.batch] = per_head;
     const uint32_t total = uint32_t(per_head) * a.heads;
-    const Runs runs(a, total);
+    const Runs runs(uint32_t(a.runs), total, kMinRun);
     run = blockIdx.x;
     if (run >= runs.runs || total == 0) return;
     if (runs.runs % kXcds == 0) run = run % kXcds * (runs.runs / kXcds) + run / kXcds;
@@ -214,7 +189,8 @@ __global__ __launch_bounds__(256 * KG, 2) void latent_prefill_kernel(ExpandedArg
     if (qb < 0) return;
   }
 
-  // Byte offsets of this lane's loads within a tile.
+  // Byte offsets of this lane's loads within a tile: chunk c of row r lies at c ^ swz16(r) of its [kn | v], at c ^ swz8(r)
+  // of its k_r.
   uint32_t kv_at[NKV], kr_at[NKR];
 #pragma unroll
   for (int i = 0; i < NKV; ++i) {
@@ -489,7 +465,7 @@ __global__ __launch_bounds__(256) void latent_prefill_merge_kernel(ExpandedArgs 
   int parts = 0;
   int64_t row_first = 0, row_next = 0;
   if (nt > 0) {
-    const Runs runs(a, per_head * a.heads);
+    const Runs runs(uint32_t(a.runs), per_head * a.heads, kMinRun);
     const uint32_t u0 = uint32_t(h) * per_head + uint32_t(a.seq_tile[b] + s.before(qb));
     const uint32_t i0 = runs.holding(u0), i1 = runs.holding(u0 + nt - 1);
     if (i0 == i1) return;  // written by its run

@@ -65,6 +65,32 @@ __device__ __forceinline__ float row_group_sum(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// LDS places of 16-byte chunk c of row r: c ^ swz16(r) in rows of whole 256-byte blocks, c ^ swz8(r) in rows of 128
+// bytes. A ds_read_b128 serves rows {0-3, 12-15} of one chunk with rows {4-11} of its neighbour, a transposed read two
+// neighbouring chunks of eight rows; either way these are 16 different bank quads.
+__device__ __forceinline__ int swz16(int r) { return ((2 * r) & 15) ^ ((r & 8) ? 9 : 0); }
+__device__ __forceinline__ int swz8(int r) {
+  const int u = (r >> 1) & 7;
+  return ((2 * u) & 7) ^ ((u & 4) ? 5 : 0);
+}
+
+// A list of `total` tiles cut into at most `most` runs of at least `shortest`, the first `rest` of them one tile longer.
+// All in 32 bits (the host refuses or does not cut longer lists): a 64-bit division takes about half a microsecond at
+// the start of every workgroup.
+struct Runs {
+  uint32_t runs, base, rest;
+  __device__ __forceinline__ Runs(uint32_t most, uint32_t total, uint32_t shortest) {
+    runs = max(1u, min(most, total / shortest));
+    base = total / runs;
+    rest = total - base * runs;
+  }
+  __device__ __forceinline__ uint32_t start(uint32_t i) const { return i * base + min(i, rest); }
+  __device__ __forceinline__ uint32_t holding(uint32_t u) const {  // the run of position u
+    const uint32_t longer = rest * (base + 1);
+    return u < longer ? u / (base + 1) : rest + (u - longer) / base;
+  }
+};
+
 // Exp2 units by which softmax weights are lifted before they are rounded to 16 bits; the sums carry the same factor, which
 // the division by l takes out. An fp16 weight has steps of 2^-24 at least, so that 60,000 of 2^-25.6 of their row's
 // greatest (the tail behind a first token that takes most of the attention) would all round to zero, while l counts
