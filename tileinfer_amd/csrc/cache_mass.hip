@@ -400,7 +400,8 @@ __device__ __forceinline__ bool all_seen(const MassArgs& a, int len, int t0, con
 
 // Waves of a SIMD: what the K rows leave of the registers. They are what hides a workgroup's start (its blocks'
 // ids, then its keys): 32 queries of 32/8 heads of 128 over 4 x U[2k, 16k] tokens, both passes, 92 us with
-// three of 64 tokens each, 67 with five of 32.
+// three of 64 tokens each, 67 with five of 32. At D = 128 five leave the second pass one register short (one value
+// of scratch a lane, stored and read once).
 constexpr int mass_waves(int d) { return d <= 128 ? 5 : d <= 256 ? 3 : 2; }
 
 // First pass: (max, sum) of every workgroup and row.

@@ -19,7 +19,10 @@
 // take a third of the time in which the tile's 36 KB come from HBM; the next tile's scores are computed beside
 // this tile's output, with one barrier a tile. Bound: HBM for long batches (64 sequences of 16,384 tokens with 32
 // heads 196 us, 6.2 TB/s), else the start of a run, a tile's chain of reads, products and softmax (1.2 us), and
-// the join's launch (16 sequences of 512 to 8,192 tokens with 24 heads 38 us; one of 700 tokens 14 us).
+// the join's launch (16 sequences of 512 to 8,192 tokens with 24 heads 38 us; one of 700 tokens 14 us). Sequences of
+// more than 32 rows read their cache once for every 32, and not from L2, since the runs of their row blocks start
+// far apart: 64 sequences of 16,384 tokens with 128 heads fetch 4.8 GB of a cache of 1.2, in 675 us (7.2 TB/s, 433
+// TFLOP/s); with 64 heads 361 us.
 //
 // The batch's tiles (row blocks times sequences times tiles) are one list, cut into runs of equal length,
 // one for each workgroup; a unit (sequence, row block) that lies in one run is written by it, others

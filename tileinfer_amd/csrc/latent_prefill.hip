@@ -172,7 +172,7 @@ __global__ __launch_bounds__(256 * KG, 2) void latent_prefill_kernel(ExpandedArg
     // A sequence's last blocks first; its blocks stay side by side, for their keys in L2 (last blocks of all
     // sequences first: 24 chunks of up to 300 over up to 4,000 keys 274 us against 196). Long sequences in the
     // order of their keys, so that the last units to start are short: 12 ragged chunks over up to 4,000 keys 129 us
-    // against 148, four prompts of 500 to 3,000 104 against 115. The order costs a unit about a microsecond: prompts
+    // against 148 (one box; 126 to 140 over several), four prompts of 500 to 3,000 104 against 115. The order costs a unit about a microsecond: prompts
     // of 17 to 700 stay as they come (67 us against 72).
     h = blockIdx.x;
     b = blockIdx.z;
