@@ -439,7 +439,9 @@ int64_t ti_gqa_decode_scratch_bytes(void);
  * Latent attention: every cached token is one vector [c | k_r] of latent_dim + rope_dim values that all
  * heads share (c the normalised latent, k_r the rotated key part), in rows laid out as a cache of one KV
  * head, [num_blocks, page_size, 1, latent_dim + rope_dim]. latent_dim 512 or 256, rope_dim 64. The
- * reference has no latent layers; these stand beside its input side, decode and varlen prefill.
+ * reference has no latent layers; these stand beside its input side, decode and varlen prefill. Both attention
+ * forms round the softmax weights to 16 bits for the matrix unit (half a step of each); scores, statistics and
+ * sums are 32 bits.
  *
  * Input side of a latent layer in one launch. For every token t:
  *   q_out[t, h]     = rotate(q_rope[t, h])                                    h < num_heads (may be 0)

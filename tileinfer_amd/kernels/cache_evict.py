@@ -9,7 +9,10 @@ new blocks from its block manager and releases the old table afterwards.
 
 Both take the KV cache of one attention layer, or a latent cache as its one KV head with ``v_cache=None``.
 Keys are cached after their rotation, so a token keeps its position's angle wherever its row moves; the
-queries' positions go on counting the evicted tokens, the cache's length does not.
+queries' positions go on counting the evicted tokens, the cache's length does not. ``engine.Sequence`` has one
+count for both, so a cut sequence's slots, tables and lengths are the caller's to make: from the new table and
+the returned lengths, not from ``engine.kv_layout``, ``DeviceBlockTables`` or ``PagedKVManager``, and its table is
+no prefix of its token ids (never recorded in a prefix cache).
 
 All run on the current stream, allocate through torch's caching allocator only, read no device value on
 the host, and can be captured in a graph. The reference never drops cached tokens.

@@ -19,6 +19,11 @@ The cache is laid out as the paged cache of one KV head, ``[num_blocks, block_si
 ``swap_blocks`` apply to it as they are. The reference has no latent layers; these functions stand beside
 its ``store_kvcache``, ``gqa_decode_paged_fn`` and varlen prefill.
 
+Both attention forms hold scores, softmax statistics and sums in 32 bits and round the softmax weights to the
+operands' type for the matrix unit, half a step of each weight, as the paged GQA kernels do (fp16 weights are
+lifted by 2^7 first, so that those far below their row's greatest keep their bits); the result is rounded
+once more.
+
 All run on the current stream, allocate through torch's caching allocator only, read no device value on
 the host, and can be captured in a graph.
 """
@@ -66,8 +71,9 @@ def latent_rope_append(q_rope: torch.Tensor | None, latent: torch.Tensor, key_ro
     ``[T, 64]``, ``[1, 64]`` or ``[64]`` (the first 32 columns serve both halves); ``latent_cache`` the
     cache rows ``[num_slots, L + 64]``; ``slot_mapping`` ``[T]`` int32 (slots < 0 or >= num_slots are
     skipped, duplicates unsupported). The row written is ``[RMSNorm(latent) * (weight_offset + weight) |
-    rotate(key_rope)]``; ``weight_offset`` is 1 as in ``qknorm_rope``, 0 for weights that are the
-    whole factor. ``q_out`` ``[T, H, 64]`` receives the rotated parts, for instance the last 64 columns of
+    rotate(key_rope)]``, the rotation pairing ``i`` with ``i + 32`` (weights trained with neighbours ``2 i`` and
+    ``2 i + 1`` as pairs: the columns ``0, 2, .. 62, 1, 3, .. 63`` of both rotated parts' projections, once, give the
+    same scores); ``weight_offset`` is 1 as in ``qknorm_rope``, 0 for weights that are the whole factor. ``q_out`` ``[T, H, 64]`` receives the rotated parts, for instance the last 64 columns of
     ``latent_decode_paged_fn``'s queries; it may be ``q_rope`` itself.
     """
     # The call in its common form is checked and made in native code; None: another form, or one to refuse.
@@ -258,7 +264,7 @@ def latent_prefill_fn(q: torch.Tensor, kv: torch.Tensor, key_rope: torch.Tensor,
     Args:
         q: ``[total_q, H, D + 64]``, ``[q_nope | rotated part]``, D 128 or 64
         kv: ``[total_k, H, 2 D]``, ``[c @ Wk | c @ Wv]`` of every key token: a chunk's own and, for a
-            continuation, the cached ones before it
+            continuation, the cached ones before it, whose rows the caller gathers from the pages
         key_rope: ``[total_k, 64]`` the rotated key parts, shared by the heads (any row stride: for
             instance the last columns of cache rows)
         cu_seqlens_q, cu_seqlens_k: ``[B + 1]`` int32 offsets of each sequence's queries and keys
