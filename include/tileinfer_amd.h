@@ -473,7 +473,7 @@ int ti_latent_decode_workspace_bytes(int32_t batch, int32_t new_tokens, int32_t 
  * where row_b[j] is the cache row of the sequence's token j and q is given in the cache's space (q_nope
  * times the key's up-projection, then the rotated part). A query that sees nothing gives zeros. Block ids
  * outside [0, num_blocks) below seqlen are absent (masked, never loaded); entries at or beyond
- * ceil(seqlen / page_size) are not read. Any page_size; scale positive.
+ * ceil(seqlen / page_size) are not read. Any page_size; scale positive, at most 1e30.
  *   q        [batch, new_tokens, num_heads, latent_dim + rope_dim], last dim contiguous, strides multiples
  *            of 8 elements; fewer than 2^24 rows in all
  *   latent_cache  contiguous rows; num_blocks * page_size < 2^31
@@ -502,7 +502,7 @@ int ti_latent_prefill_workspace_bytes(int32_t batch, int32_t total_q, int32_t to
  * are not all written. Offsets beyond total_q / total_k are cut off, a sequence whose end lies before its start is
  * empty. head_dim 128 or 64, rope_dim 64;
  * rows 16-byte aligned, strides multiples of 8 elements, token strides of kv and key_rope below 2^24, scale
- * positive. With a workspace of ti_latent_prefill_workspace_bytes (16-byte aligned, contents need no
+ * positive, at most 1e30. With a workspace of ti_latent_prefill_workspace_bytes (16-byte aligned, contents need no
  * initialisation) units of 128 query rows may be cut between workgroups and joined; with NULL every unit is
  * one workgroup's.
  * The role of the reference's varlen kernel (kernels/gqa_varlen.py:40-185).
@@ -526,8 +526,8 @@ int ti_cache_mass_workspace_bytes(int32_t batch, int32_t new_tokens, int32_t num
  *   mass[b, g, t] += sum_{i, h in group g} softmax_t( scale * q[b, i, h] . K_b[t, g] ),
  *   query i seeing t <= seqlen[b] - new_tokens + i
  * Floats of mass at and beyond seqlen[b] are not touched. Absent blocks and queries that see nothing give
- * no weight. No atomics: the same call gives the same bits. scale positive; head_dim 128 or 256, or a latent cache's 320
- * or 576 (one KV head).
+ * no weight. No atomics: the same call gives the same bits. scale positive, at most 1e30; head_dim
+ * 128 or 256, or a latent cache's 320 or 576 (one KV head).
  *   q        [batch, new_tokens, num_q_heads, head_dim], last dim contiguous, strides multiples of 8
  *   k_cache  [num_blocks, page_size, num_kv_heads, head_dim] contiguous
  *   mass     [batch, num_kv_heads, >= max_blocks_per_seq * page_size] fp32 at mass_stride_b / _h

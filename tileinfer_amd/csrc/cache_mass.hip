@@ -613,7 +613,9 @@ extern "C" int ti_cache_mass(const void* q, int64_t q_stride_b, int64_t q_stride
   }
   int rc = check_mass(who, batch, new_tokens, num_q_heads, num_kv_heads, head_dim, page_size, max_blocks_per_seq);
   if (rc != TI_OK) return rc;
-  if (!(scale > 0.f)) return fail(TI_EINVAL, "%s: scale %g is not positive", who, double(scale));
+  if (!(scale > 0.f && scale <= kMaxScale)) {
+    return fail(TI_EINVAL, "%s: scale %g is not positive or beyond 1e30", who, double(scale));
+  }
   if (num_blocks < 0 || num_blocks > INT32_MAX) {
     return fail(TI_EINVAL, "%s: bad cache num_blocks=%lld", who, static_cast<long long>(num_blocks));
   }

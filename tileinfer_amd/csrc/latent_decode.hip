@@ -592,7 +592,9 @@ extern "C" int ti_latent_decode_paged(const void* q, int64_t q_stride_b, int64_t
   }
   int rc = check_latent(who, batch, new_tokens, num_heads, latent_dim, rope_dim);
   if (rc != TI_OK) return rc;
-  if (!(scale > 0.f)) return fail(TI_EINVAL, "%s: scale %g is not positive", who, double(scale));
+  if (!(scale > 0.f && scale <= kMaxScale)) {
+    return fail(TI_EINVAL, "%s: scale %g is not positive or beyond 1e30", who, double(scale));
+  }
   if (page_size <= 0 || num_blocks < 0 || max_blocks_per_seq < 0 ||
       num_blocks * page_size > INT32_MAX) {
     return fail(TI_EINVAL, "%s: bad cache page_size=%d num_blocks=%lld max_blocks_per_seq=%d (at most "

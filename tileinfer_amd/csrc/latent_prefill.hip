@@ -602,7 +602,9 @@ extern "C" int ti_latent_prefill(const void* q, int64_t q_stride_t, int64_t q_st
       !vec_rows(key_rope, key_stride_t, 0) || !vec_rows(out, out_stride_t, out_stride_h)) {
     return fail(TI_EINVAL, "%s: rows must be 16-byte aligned", who);
   }
-  if (!(scale > 0.f)) return fail(TI_EINVAL, "%s: scale %g is not positive", who, double(scale));
+  if (!(scale > 0.f && scale <= kMaxScale)) {
+    return fail(TI_EINVAL, "%s: scale %g is not positive or beyond 1e30", who, double(scale));
+  }
   // A tile's rows are reached by 32-bit offsets.
   if (kv_stride_t < 0 || key_stride_t < 0 || kv_stride_t >= (1 << 24) || key_stride_t >= (1 << 24)) {
     return fail(TI_EINVAL, "%s: token strides %lld, %lld of kv and key_rope must be in [0, 2^24)", who,

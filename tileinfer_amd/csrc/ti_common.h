@@ -20,6 +20,10 @@ int device_cu_count();
 // Workgroups of at most 256 threads that a launch takes along x: its work items there are counted in 32 bits.
 constexpr int64_t kMaxGridX = (int64_t(1) << 24) - 1;
 
+// Scores are scaled by scale * log2 e in 32 bits; a larger scale (or an infinite one, as a host double beyond 32 bits
+// becomes) leaves them.
+constexpr float kMaxScale = 1e30f;
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // 4 x 32-bit registers: one 16-byte global access, or the 8 x 16-bit operand of a

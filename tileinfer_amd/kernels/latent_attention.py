@@ -55,8 +55,8 @@ def _as_rows(t: torch.Tensor) -> torch.Tensor:
 
 def _scale(scale: float) -> float:
     scale = float(scale)
-    if not 0 < scale < float("inf"):
-        raise ValueError(f"scale {scale} must be positive")
+    if not 0 < scale <= 1e30:
+        raise ValueError(f"scale {scale} must be positive and at most 1e30")
     return scale
 
 
