@@ -32,6 +32,8 @@ def test_a_list_of_tiles_that_offsets_could_make_too_long_is_not_cut():
     lib, n = _lib.load(), ctypes.c_int64(1)
     assert lib.ti_latent_prefill_workspace_bytes(65535, 1024, 65536, 16, 128, ctypes.byref(n)) == _lib.TI_OK
     assert n.value == 0
+    assert lib.ti_latent_prefill_workspace_bytes(2 ** 31 - 1, 1, 2 ** 31 - 1, 2, 128, ctypes.byref(n)) == _lib.TI_OK
+    assert n.value == 0  # more sequences than a call takes
     assert lib.ti_latent_prefill_workspace_bytes(24, 2048, 400000, 16, 128, ctypes.byref(n)) == _lib.TI_OK
     assert n.value > 0
 

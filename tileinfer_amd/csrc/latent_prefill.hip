@@ -172,8 +172,8 @@ __global__ __launch_bounds__(256 * KG, 2) void latent_prefill_kernel(ExpandedArg
     // A sequence's last blocks first; its blocks stay side by side, for their keys in L2 (last blocks of all
     // sequences first: 24 chunks of up to 300 over up to 4,000 keys 274 us against 196). Long sequences in the
     // order of their keys, so that the last units to start are short: 12 ragged chunks over up to 4,000 keys 129 us
-    // against 148 (one box; 126 to 140 over several), four prompts of 500 to 3,000 104 against 115. The order costs a unit about a microsecond: prompts
-    // of 17 to 700 stay as they come (67 us against 72).
+    // against 148 (one box; 126 to 140 over several), four prompts of 500 to 3,000 104 against 115. The order costs a
+    // unit about a microsecond: prompts of 17 to 700 stay as they come (67 us against 72).
     h = blockIdx.x;
     b = blockIdx.z;
     if (a.by_length) {
@@ -513,9 +513,9 @@ struct PrefillSizes {
 PrefillSizes prefill_sizes(int32_t batch, int32_t total_q, int32_t total_k, int32_t heads, int32_t head_dim) {
   PrefillSizes z{};
   const int64_t cus = device_cu_count(), slots = 2 * cus, blocks = ceil_div(total_q, kRows);
+  if (batch > 65535 || blocks * heads > cus) return z;
   // The list is counted in 32 bits on the device. Offsets that go back may give every sequence all blocks and keys.
-  const int64_t most = batch * blocks * ceil_div(total_k, kKeys) * heads;
-  if (blocks * heads > cus || most > INT32_MAX) return z;
+  if (batch * blocks * ceil_div(total_k, kKeys) * heads > INT32_MAX) return z;
   z.runs = int32_t(slots);
   z.o_floats = slots * 2 * kRows * head_dim;
   z.ml_floats = slots * 2 * kRows * 2;

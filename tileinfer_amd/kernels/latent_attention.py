@@ -73,8 +73,9 @@ def latent_rope_append(q_rope: torch.Tensor | None, latent: torch.Tensor, key_ro
     skipped, duplicates unsupported). The row written is ``[RMSNorm(latent) * (weight_offset + weight) |
     rotate(key_rope)]``, the rotation pairing ``i`` with ``i + 32`` (weights trained with neighbours ``2 i`` and
     ``2 i + 1`` as pairs: the columns ``0, 2, .. 62, 1, 3, .. 63`` of both rotated parts' projections, once, give the
-    same scores); ``weight_offset`` is 1 as in ``qknorm_rope``, 0 for weights that are the whole factor. ``q_out`` ``[T, H, 64]`` receives the rotated parts, for instance the last 64 columns of
-    ``latent_decode_paged_fn``'s queries; it may be ``q_rope`` itself.
+    same scores); ``weight_offset`` is 1 as in ``qknorm_rope``, 0 for weights that are the whole factor. ``q_out``
+    ``[T, H, 64]`` receives the rotated parts, for instance the last 64 columns of ``latent_decode_paged_fn``'s
+    queries; it may be ``q_rope`` itself.
     """
     # The call in its common form is checked and made in native code; None: another form, or one to refuse.
     stream = None if q_out is not None else _lib.native(latent)
