@@ -17,6 +17,8 @@
  *     on the pages, expanded prefill
  *   - attention weight of cached tokens and  (no reference counterpart: fewer cached tokens)
  *     eviction by it
+ *   - positions of several axes (+ append),  (no reference counterpart: image and video tokens,
+ *     drafted trees, shaped scores            speculative steps, capped / biased / masked scores)
  *
  * Conventions shared by every entry point
  *   - All tensor pointers are DEVICE pointers owned by the caller. The library never allocates,
@@ -563,6 +565,75 @@ int ti_evict_kvcache(void* k_cache, void* v_cache, const float* mass, int64_t ma
                      int32_t batch, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
                      int64_t num_blocks, int32_t max_blocks_per_seq, int32_t new_blocks_per_seq,
                      int32_t budget, int32_t sinks, int32_t recent, int32_t dtype, void* stream);
+
+/*
+ * Input side of a step whose positions have several axes, in one launch: for every token t
+ *   x' = x * rsqrt(mean(x^2) + eps) * (weight_offset + weight)      (q and k; NULL weights: x' = x)
+ *   angle_i = positions[axis_of[i], t] * inv_freq[i], i < rotary_dim / 2, pairing i with i + rotary_dim / 2
+ * q rotated to q_out, k rotated and v as it is to the cache rows at slot_mapping[t] (slots outside
+ * [0, num_slots) are skipped, duplicates unsupported). In 32 bits, angles in 64, each value rounded once.
+ *   q, k, v, q_out   rows of head_dim (128 or 256), 16-byte aligned, strides multiples of 8 elements
+ *   positions        [num_axes (1 .. 4), n_tokens] of position_bits (32 or 64) bits, token stride 1
+ *   inv_freq, axis_of  [rotary_dim / 2]; axis_of NULL: axis 0, entries outside are clamped to the axes there are
+ *   rotary_dim       a multiple of 16 up to min(head_dim, 128); 0: no rotation
+ *   caches           rows of num_kv_heads * head_dim at cache_row_stride
+ * At most 2^26 rows (n_tokens times heads of q, k and v). No reference counterpart (its positions have one axis).
+ */
+int ti_rope_axes_append(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+                        int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
+                        int64_t v_stride_h, const void* positions, int64_t pos_stride_a,
+                        int32_t position_bits, const float* inv_freq, const int32_t* axis_of,
+                        const void* q_weight, const void* k_weight, float weight_offset, void* q_out,
+                        int64_t out_stride_t, int64_t out_stride_h, void* k_cache, void* v_cache,
+                        int64_t cache_row_stride, int64_t num_slots, const int32_t* slot_mapping,
+                        int32_t n_tokens, int32_t num_axes, int32_t num_q_heads, int32_t num_kv_heads,
+                        int32_t head_dim, int32_t rotary_dim, float eps, int32_t dtype, void* stream);
+
+/* Workspace of ti_gqa_tree_paged for these host-known sizes. */
+int ti_gqa_tree_workspace_bytes(int32_t batch, int32_t num_drafts, int32_t num_q_heads, int32_t num_kv_heads,
+                                int32_t head_dim, int64_t* workspace_bytes_out);
+
+/*
+ * Attention of every sequence's last num_drafts (1 .. 64) tokens, a drafted tree behind a context of
+ * C = seqlen[b] - num_drafts tokens, over its pages:
+ *   s_j = softcap tanh(scale q . k_j / softcap) - slope_h |p_i - p_j|,   out = softmax_j(s_j) @ v_j
+ * Draft i sees every token j < C and the draft C + j where bit j of tree_mask[b, i] is set (NULL: j <= i); bits from
+ * num_drafts on are ignored. p_j = j for j < C; draft i is at C + the number of other drafts it sees. window > 0 keeps
+ * the keys with p_i - p_j < window. softcap 0: no cap; slopes NULL: none. A draft that sees nothing gives zeros. Where
+ * seqlen[b] < num_drafts the drafts before token 0 do not exist as keys. Block ids outside [0, num_blocks) below
+ * seqlen are absent (masked, never loaded); entries at or beyond ceil(seqlen / page_size) are not read.
+ *   q          [batch, num_drafts, num_q_heads, head_dim], last dim contiguous, strides multiples of 8 elements
+ *   caches     [num_blocks, page_size, num_kv_heads, head_dim] contiguous, head_dim 128 or 256, any page_size
+ *   tree_mask  [batch, num_drafts] at mask_stride_b (0: one tree for all)
+ *   slopes     [num_q_heads] fp32
+ *   out        [batch, num_drafts, num_q_heads, head_dim] contiguous; fewer than 2^24 rows in all
+ *   workspace  ti_gqa_tree_workspace_bytes bytes, 16-byte aligned, contents need no initialisation
+ * scale positive, at most 1e30, softcap 1e-3 to 1e4. No reference counterpart (the reference drafts nothing).
+ */
+int ti_gqa_tree_paged(const void* q, int64_t q_stride_b, int64_t q_stride_t, int64_t q_stride_h,
+                      const void* k_cache, const void* v_cache, const int32_t* block_table,
+                      int64_t block_table_stride, const int32_t* seqlen, const int64_t* tree_mask,
+                      int64_t mask_stride_b, const float* slopes, void* out, void* workspace,
+                      int64_t workspace_bytes, int32_t batch, int32_t num_drafts, int32_t num_q_heads,
+                      int32_t num_kv_heads, int32_t head_dim, int32_t page_size, int64_t num_blocks,
+                      int32_t max_blocks_per_seq, float scale, float softcap, int32_t window, int32_t dtype,
+                      void* stream);
+
+/*
+ * Move the cache rows of accepted drafts behind the context, in place, in every plane (a layer's keys or values):
+ *   row(C + j) = row(C + accepted[b, j]), C = seqlen[b] - num_drafts;  new_seqlen[b] = C + accepted drafts
+ * accepted[b] lists draft indices in ascending order; it ends at its first entry that does not ascend or is outside
+ * [0, num_drafts) (-1 behind the last). Sequences with seqlen[b] < num_drafts (padding) keep their rows and length. Rows
+ * whose block is outside [0, num_blocks) are not moved.
+ *   cache     planes contiguous arrays of num_blocks * page_size rows of row_elems (a multiple of 8) 16-bit elements
+ *   accepted  [batch, accepted_width] at accepted_stride; num_drafts 1 .. 64
+ * No reference counterpart.
+ */
+int ti_keep_drafts(void* cache, const int32_t* block_table, int64_t block_table_stride,
+                   const int32_t* seqlen, const int32_t* accepted, int64_t accepted_stride,
+                   int32_t* new_seqlen, int32_t batch, int32_t num_drafts, int32_t accepted_width,
+                   int32_t planes, int64_t row_elems, int32_t page_size, int64_t num_blocks,
+                   int32_t max_blocks_per_seq, void* stream);
 
 /* Text of the last error reported on the calling thread ("" when none). */
 const char* ti_last_error(void);

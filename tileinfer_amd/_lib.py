@@ -33,7 +33,7 @@ TI_DECODE_MFMA = 1
 TI_DECODE_SCALAR = 2
 TI_DECODE_REUSE_KV = 0x10
 TI_DECODE_STREAM_KV = 0x20
-ABI_VERSION = 8
+ABI_VERSION = 9
 INT32_MAX = 2 ** 31 - 1  # ctypes cuts larger host ints to 32 bits without an error
 
 # Every symbol declared in include/tileinfer_amd.h, with its ctypes signature.
@@ -124,6 +124,18 @@ SIGNATURES = {
                                         _c_vp, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_i32, _c_i32,
                                         _c_i32, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32,
                                         _c_i32, _c_i32, _c_vp]),
+    "ti_rope_axes_append": (ctypes.c_int, [_c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp, _c_i64,
+                                           _c_i64, _c_vp, _c_i64, _c_i32, _c_vp, _c_vp, _c_vp, _c_vp,
+                                           ctypes.c_float, _c_vp, _c_i64, _c_i64, _c_vp, _c_vp, _c_i64,
+                                           _c_i64, _c_vp, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,
+                                           ctypes.c_float, _c_i32, _c_vp]),
+    "ti_gqa_tree_workspace_bytes": (ctypes.c_int, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _I64P]),
+    "ti_gqa_tree_paged": (ctypes.c_int, [_c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_vp, _c_i64, _c_vp,
+                                         _c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_i64, _c_i32, _c_i32,
+                                         _c_i32, _c_i32, _c_i32, _c_i32, _c_i64, _c_i32, ctypes.c_float,
+                                         ctypes.c_float, _c_i32, _c_i32, _c_vp]),
+    "ti_keep_drafts": (ctypes.c_int, [_c_vp, _c_vp, _c_i64, _c_vp, _c_vp, _c_i64, _c_vp, _c_i32, _c_i32,
+                                      _c_i32, _c_i32, _c_i64, _c_i32, _c_i64, _c_i32, _c_vp]),
     "ti_last_error": (ctypes.c_char_p, []),
     "ti_abi_version": (ctypes.c_int32, []),
 }
