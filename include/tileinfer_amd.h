@@ -635,6 +635,39 @@ int ti_keep_drafts(void* cache, const int32_t* block_table, int64_t block_table_
                    int32_t planes, int64_t row_elems, int32_t page_size, int64_t num_blocks,
                    int32_t max_blocks_per_seq, void* stream);
 
+/* Workspace of ti_gqa_prefill_shaped for these host-known sizes; 0: the call needs none. max_seqlen_k: a bound on
+ * every seqlen_k (max_blocks_per_seq * page_size where nothing better is known). */
+int ti_gqa_prefill_shaped_workspace_bytes(int32_t batch, int32_t total_q, int32_t max_seqlen_q,
+                                          int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                          int64_t max_seqlen_k, int64_t* workspace_bytes_out);
+
+/*
+ * ti_gqa_prefill_paged with shaped scores: query row r = cu_seqlens_q[b] + i of sequence b, at position
+ * p = seqlen_k[b] - q_len + i, sees the keys j with
+ *   max(first_key[r], 0) <= j <= last_key[r], j < seqlen_k[b], p - j < window
+ * (first_key NULL: 0; last_key NULL: p with `causal`, else the last key; window 0: none) with the scores
+ *   s = softcap tanh(scale q . k_j / softcap) - slope_h |p - j|          (softcap 0: no cap; slopes NULL: none)
+ * A query that sees nothing gives zeros. max_seqlen_q is at least the longest chunk; rows of longer ones are not all
+ * written, rows of no sequence not at all. Block ids outside [0, num_blocks) below seqlen_k are absent (masked, never
+ * loaded).
+ *   q, out     [total_q, num_q_heads, head_dim] rows 16-byte aligned, strides multiples of 8 elements
+ *   caches     [num_blocks, page_size, num_kv_heads, head_dim] contiguous, head_dim 128 or 256, any page_size
+ *   first_key, last_key  [total_q] or NULL;  slopes  [num_q_heads] fp32 or NULL
+ * With a workspace of ti_gqa_prefill_shaped_workspace_bytes (16-byte aligned, contents need no initialisation; the same
+ * max_seqlen_k) the keys of few query rows may be cut between workgroups and joined; with NULL they are not.
+ * scale positive, at most 1e30, softcap 1e-3 to 1e4. The role of the reference's varlen kernel
+ * (kernels/gqa_varlen.py:40-185) for models that shape their scores.
+ */
+int ti_gqa_prefill_shaped(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_cache,
+                          const void* v_cache, const int32_t* block_table, int64_t block_table_stride,
+                          const int32_t* cu_seqlens_q, const int32_t* seqlen_k, const int32_t* first_key,
+                          const int32_t* last_key, const float* slopes, void* out, int64_t out_stride_t,
+                          int64_t out_stride_h, void* workspace, int64_t workspace_bytes, int32_t batch,
+                          int32_t total_q, int32_t max_seqlen_q, int32_t num_q_heads, int32_t num_kv_heads,
+                          int32_t head_dim, int32_t page_size, int64_t num_blocks, int32_t max_blocks_per_seq,
+                          int64_t max_seqlen_k, int32_t causal, float scale, float softcap, int32_t window,
+                          int32_t dtype, void* stream);
+
 /* Text of the last error reported on the calling thread ("" when none). */
 const char* ti_last_error(void);
 

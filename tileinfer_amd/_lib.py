@@ -136,6 +136,13 @@ SIGNATURES = {
                                          ctypes.c_float, _c_i32, _c_i32, _c_vp]),
     "ti_keep_drafts": (ctypes.c_int, [_c_vp, _c_vp, _c_i64, _c_vp, _c_vp, _c_i64, _c_vp, _c_i32, _c_i32,
                                       _c_i32, _c_i32, _c_i64, _c_i32, _c_i64, _c_i32, _c_vp]),
+    "ti_gqa_prefill_shaped_workspace_bytes": (ctypes.c_int, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,
+                                                             _c_i64, _I64P]),
+    "ti_gqa_prefill_shaped": (ctypes.c_int, [_c_vp, _c_i64, _c_i64, _c_vp, _c_vp, _c_vp, _c_i64, _c_vp, _c_vp,
+                                             _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_vp, _c_i64,
+                                             _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i64,
+                                             _c_i32, _c_i64, _c_i32, ctypes.c_float, ctypes.c_float, _c_i32,
+                                             _c_i32, _c_vp]),
     "ti_last_error": (ctypes.c_char_p, []),
     "ti_abi_version": (ctypes.c_int32, []),
 }

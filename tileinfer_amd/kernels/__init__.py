@@ -15,3 +15,4 @@ from .latent_attention import (latent_decode_paged_fn, latent_prefill_fn,  # noq
                                latent_rope_append)
 from .qknorm_rope import fused_qknorm_rope, qknorm_rope, qknorm_rope_append  # noqa: F401
 from .rope_axes import rope_axes, rope_axes_append  # noqa: F401
+from .shaped_prefill import gqa_prefill_shaped_fn  # noqa: F401
