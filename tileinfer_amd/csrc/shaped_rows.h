@@ -1,0 +1,565 @@
+// Attention of many query rows over the paged cache with shaped scores (gfx950): the kernel behind the shaped prefill
+// (queries of packed chunks, each with an interval of keys) and behind wide trees of drafts (TREE: the last tokens of
+// every sequence, each with a mask of drafts). A row is a (token, query head) pair of one KV head:
+//   s_j = cap tanh(scale q . k_j / cap) - slope |p - p_j|,   o = sum_j softmax(s)_j v_j
+//
+// Work unit: (sequence, KV head, 128 rows). The tiles of 64 keys that any row sees are loaded straight from the pages
+// into LDS and read by all waves, each with 16 C rows (C = 1 of eight waves at D = 256, 2 of four at D = 128):
+//   S^T[64 keys x rows] = K . Q^T      (16x16x32, Q in registers)
+//   O^T[D x rows]      += V^T . P^T    (16x16x32, V by transposed reads)
+// with an accumulator's row its lane's column, so that the softmax stays in the lane. A score of the cap costs three
+// exponential-unit instructions, so that the softmax takes as many cycles as the products; it runs beside them, cut in
+// two: while the matrix unit computes the scores of tile t + 1, the vector unit turns those of tile t into weights, and
+// beside the output of tile t it caps the scores of tile t + 1. One barrier a tile; K is two tiles ahead, V one.
+#pragma once
+
+#include "lds_tiles.h"
+#include "score_shape.h"
+
+namespace ti {
+namespace {
+
+constexpr int kRows = 128;     // rows of a unit
+constexpr int kKeys = 64;      // keys of a tile
+constexpr int kIdSlots = 512;  // block ids staged at a time
+constexpr float kSlack = 8.f;  // exp2 units a row maximum may rise before O is rescaled
+constexpr int kMaxDrafts = 64;
+
+struct RowsArgs {
+  const uint16_t* q;  // [tokens, hq, D] at q_st, q_sh; TREE: [B, drafts, hq, D], q_sb too
+  int64_t q_sb, q_st, q_sh;
+  const uint16_t* k_cache;  // rows [num_blocks * page_size][hkv * D]
+  const uint16_t* v_cache;
+  const int32_t* block_table;
+  int64_t bt_stride;
+  const int32_t* seqlen;
+  const float* slopes;  // [hq] or nullptr
+  uint16_t* out;        // as q
+  int64_t o_sb, o_st, o_sh;
+  // Prefill
+  const int32_t* cu_q;
+  const int32_t* first_key;  // [total_q] or nullptr
+  const int32_t* last_key;
+  int32_t total_q, causal;
+  // TREE
+  const int64_t* mask;  // [B, drafts] at mask_sb, or nullptr: draft i sees the drafts j <= i
+  int64_t mask_sb;
+  int32_t drafts;
+  // Units in the order of (sequence, block from the last one, KV head): the first `whole` of them are a workgroup's
+  // each, the keys of the others are cut into `splits` parts, of which a second kernel joins [unit - whole][splits].
+  float* part_o;   // [units - whole][splits][128][D] unnormalised rows
+  float* part_ml;  // [units - whole][splits][128][2] their (m, l), m in exp2 units
+  int32_t units, whole, splits, blocks;
+  int32_t hq, hkv, group, num_blocks32, page_size, max_blocks, window;  // window 0: none
+  // at / page_size = mulhi(2 at, page_magic) >> page_shift for at below 2^31: page_shift = ceil(log2 page_size),
+  // page_magic = ceil(2^(31 + page_shift) / page_size)
+  uint32_t page_magic, page_shift;
+  ScoreShape shape;
+};
+
+__device__ __align__(16) uint16_t g_zero_row[256] = {};
+
+// A sequence's queries, within the tensors whatever the offsets say, and its cached tokens.
+template <bool TREE>
+struct Queries {
+  int q0, q_len, kv_len, offset;
+  __device__ __forceinline__ Queries(const RowsArgs& a, int b) {
+    if constexpr (TREE) {
+      q0 = 0;
+      q_len = a.drafts;
+    } else {
+      q0 = min(max(a.cu_q[b], 0), a.total_q);
+      q_len = min(max(a.cu_q[b + 1], q0), a.total_q) - q0;
+    }
+    const int64_t cap = int64_t(a.max_blocks) * a.page_size;
+    const int n = max(a.seqlen[b], 0);
+    kv_len = int64_t(n) > cap ? int(cap) : n;
+    offset = kv_len - q_len;  // query i's row sits at position offset + i; TREE: the context's length
+  }
+};
+
+__device__ __forceinline__ void load_lds16_at(uint64_t src, const uint16_t* lds) {
+  const uint32_t m0 = uint32_t(reinterpret_cast<uintptr_t>((lds_ptr_t)(lds)));
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(m0) : "memory");
+}
+
+__device__ __forceinline__ uint64_t drafts_seen(const RowsArgs& a, int b, int i) {
+  const uint64_t exist = a.drafts == 64 ? ~uint64_t(0) : (uint64_t(1) << a.drafts) - 1;
+  return exist & (a.mask ? uint64_t(a.mask[b * a.mask_sb + i]) : (uint64_t(2) << i) - 1);
+}
+
+template <int D>
+struct RowsShape {
+  static constexpr int C = D == 256 ? 1 : 2;  // row tiles of a wave
+  static constexpr int W = kRows / 16 / C;    // waves
+  static constexpr int THREADS = 64 * W;
+};
+
+// CAP: the scores are capped. SLOPES: they are biased.
+template <int D, bool CAP, bool SLOPES, bool TREE, typename Tag>
+__global__ __launch_bounds__(RowsShape<D>::THREADS, 2) void shaped_rows_kernel(RowsArgs a) {
+  constexpr int C = RowsShape<D>::C, W = RowsShape<D>::W;
+  constexpr int TT = kKeys / 16, KP = kKeys / 32;
+  constexpr int KK = D / 32, NDT = D / 16;
+  constexpr int CH = D / 8, RPL = 64 / CH;  // 16-byte chunks of a row, rows of a load
+  constexpr int LW = 4;                     // waves that load
+  constexpr int NLD = kKeys / RPL / LW;     // their loads of a tile, of K and of V each
+  constexpr int kTile = kKeys * D;
+  __shared__ __align__(16) uint16_t s_k[2 * kTile];
+  __shared__ __align__(16) uint16_t s_v[2 * kTile];
+  __shared__ int s_ids[kIdSlots];
+  __shared__ int s_range[W][2];
+  __shared__ __align__(16) uint64_t s_from[4][kKeys][2];  // addresses of a tile's tokens in K and in V
+  __shared__ uint64_t s_here[4];                          // and which of them exist
+  __shared__ int4 s_row[kRows];  // (first key, last key, position, slope) of every row
+  __shared__ uint64_t s_seen[TREE ? kRows : 1];
+  __shared__ int s_depth[TREE ? kMaxDrafts : 1];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  int unit = blockIdx.x, split = 0, splits = 1;
+  if (unit >= a.whole) {
+    const int rest = a.units - a.whole, i = unit - a.whole;
+    split = i / rest;
+    unit = a.whole + i - split * rest;
+    splits = a.splits;
+  }
+  const int per_seq = a.blocks * a.hkv;
+  const int b = unit / per_seq, in_seq = unit - b * per_seq;
+  const int qb = a.blocks - 1 - in_seq / a.hkv, kvh = in_seq % a.hkv;
+  const Queries<TREE> sq(a, b);
+  const int rows = sq.q_len * a.group;
+  if (qb * kRows >= rows) return;
+
+  // This lane's rows and the keys they see, which stay in LDS: only tiles that a limit or a slope touches need them.
+  const int row0 = qb * kRows + wave * 16 * C + n;
+  u32x4 q[C][KK];
+  int some_lo = INT32_MAX, some_hi = -1, all_lo = 0, all_hi = INT32_MAX;
+#pragma unroll
+  for (int rt = 0; rt < C; ++rt) {
+    const int r = min(row0 + 16 * rt, rows - 1);  // rows behind the last repeat it, not stored
+    const int tok = r / a.group, head = kvh * a.group + r - tok * a.group;
+    const uint16_t* src = a.q + (TREE ? b * a.q_sb : sq.q0 * a.q_st) + tok * a.q_st + head * a.q_sh + 8 * g;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) q[rt][kk] = load16(src + 32 * kk);
+    int pos = sq.offset + tok, lo = 0, hi;
+    if constexpr (TREE) {
+      const uint64_t seen = drafts_seen(a, b, tok);
+      pos = sq.offset + __builtin_popcountll(seen & ~(uint64_t(1) << tok));
+      hi = sq.offset - 1;  // of the context; the drafts by their bits
+      if (g == 0) s_seen[wave * 16 * C + rt * 16 + n] = seen;
+    } else {
+      if (a.first_key) lo = max(a.first_key[sq.q0 + tok], 0);
+      hi = min(a.last_key ? a.last_key[sq.q0 + tok] : a.causal ? pos : sq.kv_len - 1, sq.kv_len - 1);
+    }
+    if (a.window > 0 && pos >= a.window) lo = max(lo, pos - a.window + 1);
+    if (!TREE && lo > hi) {  // sees nothing
+      lo = INT32_MAX;
+      hi = -1;
+    }
+    const float slope = SLOPES ? a.slopes[head] * kLog2e : 0.f;
+    if (g == 0) s_row[wave * 16 * C + rt * 16 + n] = make_int4(lo, hi, pos, __float_as_int(slope));
+    some_lo = min(some_lo, lo);
+    some_hi = max(some_hi, hi);
+    all_lo = max(all_lo, lo);
+    all_hi = min(all_hi, hi);
+  }
+  if constexpr (TREE) {
+    if (int(threadIdx.x) < a.drafts) {
+      s_depth[threadIdx.x] = __builtin_popcountll(drafts_seen(a, b, threadIdx.x) & ~(uint64_t(1) << threadIdx.x));
+    }
+  }
+  // Over the wave's rows: the keys that some row sees, and those that every row sees.
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) {
+    some_lo = min(some_lo, __shfl_xor(some_lo, d, 64));
+    some_hi = max(some_hi, __shfl_xor(some_hi, d, 64));
+    all_lo = max(all_lo, __shfl_xor(all_lo, d, 64));
+    all_hi = min(all_hi, __shfl_xor(all_hi, d, 64));
+  }
+  all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+  all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+  if (lane == 0) {
+    s_range[wave][0] = some_lo;
+    s_range[wave][1] = some_hi;
+  }
+  __syncthreads();
+  int key_lo = INT32_MAX, key_hi = -1;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    key_lo = min(key_lo, s_range[w][0]);
+    key_hi = max(key_hi, s_range[w][1]);
+  }
+  if constexpr (TREE) {  // a window may leave nothing of the context
+    key_hi = sq.kv_len - 1;
+    key_lo = min(key_lo, max(sq.offset, 0));
+  }
+  key_lo = __builtin_amdgcn_readfirstlane(key_lo);
+  key_hi = __builtin_amdgcn_readfirstlane(key_hi);
+  const int tile0 = key_hi < 0 ? 0 : key_lo / kKeys, tiles = key_hi < 0 ? 0 : key_hi / kKeys + 1 - tile0;
+  const int t0 = tile0 + int(int64_t(tiles) * split / splits), t1 = tile0 + int(int64_t(tiles) * (split + 1) / splits);
+
+  // Operand reads of K row n and of V row 4 g + n / 4 (elements): those of k-step kk and column tile dt are at these with
+  // the bits of kk and dt flipped, which the rows' places leave alone.
+  const int k_at = n * D + 8 * (g ^ swz16(n));
+  const int v_row = 4 * g + (n >> 2);
+  const int v_at = v_row * D + 8 * (((lane >> 1) & 1) ^ swz16(v_row)) + 4 * (lane & 1);
+  // Load j of a wave takes the tile's rows kStep j + load_row: a lane's chunk is the same in rows 16 apart, in rows 8 apart
+  // 9 places on.
+  constexpr int kStep = LW * RPL;
+  static_assert(kStep == 16 || kStep == 8);
+  const int load_row = (wave & (LW - 1)) * RPL + lane / CH;
+  const uint32_t lane_off = 16 * ((lane % CH) ^ swz16(load_row));
+  uint64_t zero_row = reinterpret_cast<uint64_t>(g_zero_row);
+  asm("" : "+s"(zero_row));  // held, not looked up again for every tile
+
+  f32x4 o[NDT][C];
+  float m[C], l[C];
+#pragma unroll
+  for (int rt = 0; rt < C; ++rt) {
+    m[rt] = -INFINITY;
+    l[rt] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) o[dt][rt] = f32x4{};
+  }
+  // The scores x between the products are what is cheapest to make and to compare: with a slope the scores in exp2
+  // units; with a cap alone r = 1 / (1 + e^2y), of which the score is cap (1 - 2 r) and whose minimum is the
+  // maximum of the scores; else the dot products. A weight is exp2(mul x + add).
+  constexpr bool kInverse = CAP && !SLOPES;
+  constexpr float kMasked = kInverse ? INFINITY : -INFINITY;
+  const float mul = SLOPES ? 1.f : CAP ? -2.f * a.shape.cap_log2 : a.shape.scale_log2;
+  const float add = kInverse ? a.shape.cap_log2 : 0.f;
+
+  // Tiles in pieces whose block ids fit s_ids.
+  const int piece = int(min(int64_t(1) << 24, int64_t(kIdSlots - 2) * a.page_size / kKeys));
+  for (int a0 = t0; a0 < t1; a0 += piece) {
+    const int a1 = min(t1, a0 + piece);
+    const int page0 = a0 * kKeys / a.page_size;
+    const int pages = (min(a1 * kKeys, sq.kv_len) - 1) / a.page_size - page0 + 1;
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the last piece is read
+    for (int i = threadIdx.x; i < pages; i += 64 * W) s_ids[i] = a.block_table[b * a.bt_stride + page0 + i];
+    __builtin_amdgcn_s_waitcnt(0);  // q has landed too: the loop below has waits of its own alone
+    asm volatile("s_barrier" ::: "memory");
+
+    // One wave's work for a tile: the addresses of its 64 tokens' rows of this KV head, from which all loads follow (each
+    // wave by itself took 1,000 cycles a tile for its rows); absent tokens are zeros, not what the cache may hold there.
+    auto find = [&](int t) __attribute__((always_inline)) {
+      const int at = t * kKeys + lane, page = int(__umulhi(2u * uint32_t(at), a.page_magic) >> a.page_shift);
+      const int id = s_ids[min(page - page0, kIdSlots - 1)];
+      const bool ok = at < min(sq.kv_len, a1 * kKeys) && uint32_t(id) < uint32_t(a.num_blocks32);
+      const uint64_t off = uint64_t(uint32_t(id * a.page_size + at - page * a.page_size)) * (uint32_t(a.hkv) * (2 * D)) +
+                           uint32_t(kvh) * (2 * D);
+      const uint64_t here = __builtin_amdgcn_ballot_w64(ok);
+      s_from[t & 3][lane][0] = ok ? reinterpret_cast<uint64_t>(a.k_cache) + off : zero_row;
+      s_from[t & 3][lane][1] = ok ? reinterpret_cast<uint64_t>(a.v_cache) + off : zero_row;
+      if (lane == 0) s_here[t & 3] = here;
+    };
+    // Loads tile t of K (kv 0) or V (1).
+    auto issue = [&](int kv, int t, uint16_t* to) __attribute__((always_inline)) {
+      const uint64_t* const from = &s_from[t & 3][load_row][kv];
+      uint64_t at[NLD];
+#pragma unroll
+      for (int j = 0; j < NLD; ++j) at[j] = from[2 * kStep * j];
+#pragma unroll
+      for (int j = 0; j < NLD; ++j) {
+        load_lds16_at(at[j] + (kStep == 8 && (j & 1) ? lane_off ^ (16 * 9) : lane_off),
+                      to + ((wave & (LW - 1)) * RPL + j * kStep) * D);
+      }
+    };
+
+    f32x4 s[TT][C];
+    // One k-step of the scores of the tile in K stage `k_off` (its reads a step ahead of the products).
+    u32x4 k[2][TT];
+    auto read_keys = [&](int k_off, int kk) __attribute__((always_inline)) {
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) {
+        k[kk & 1][tt] = *reinterpret_cast<const u32x4*>(s_k + (k_off ^ (32 * kk)) + 16 * tt * D);
+      }
+    };
+    auto multiply_keys = [&](f32x4 (&to)[TT][C], int kk) __attribute__((always_inline)) {
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+        for (int rt = 0; rt < C; ++rt) {
+          to[tt][rt] = mfma16x16x32(k[kk & 1][tt], q[rt][kk], kk == 0 ? f32x4{} : to[tt][rt], Tag{});
+        }
+      }
+    };
+    // A dot product as the score that is kept (without its slope).
+    auto shape_of = [&](float dot) __attribute__((always_inline)) {
+      if constexpr (CAP) {
+        const float r = __builtin_amdgcn_rcpf(1.f + fast_exp2(dot * a.shape.cap_in));
+        return kInverse ? r : fmaf(-2.f * a.shape.cap_log2, r, a.shape.cap_log2);
+      } else {
+        return SLOPES ? dot * a.shape.scale_log2 : dot;
+      }
+    };
+    // The slopes and limits of tile t on its scores; the rows' maxima, and O brought to new ones.
+    auto limit = [&](int t) __attribute__((always_inline)) {
+      const int first = t * kKeys;
+      const uint64_t here = uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(s_here[t & 3]))))) |
+                            uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(s_here[t & 3] >> 32))))) << 32;
+      bool whole = here == ~uint64_t(0) && first >= all_lo && first + kKeys - 1 <= all_hi;  // uniform
+      if constexpr (SLOPES) {
+        if (!TREE || whole) {
+#pragma unroll
+          for (int rt = 0; rt < C; ++rt) {
+            const int4 row = s_row[wave * 16 * C + rt * 16 + n];
+            const float far = float(first + 4 * g - row.z), slope = __int_as_float(row.w);
+#pragma unroll
+            for (int e = 0; e < 4 * TT; ++e) {
+              s[e >> 2][rt][e & 3] = fmaf(-slope, fabsf(far + float(16 * (e >> 2) + (e & 3))), s[e >> 2][rt][e & 3]);
+            }
+          }
+        }
+      }
+      if (!whole) {
+        const uint64_t mine = here >> (4 * g);
+#pragma unroll
+        for (int rt = 0; rt < C; ++rt) {
+          const int4 row = s_row[wave * 16 * C + rt * 16 + n];
+          uint64_t seen = mine;  // bit j: key first + 4 g + j
+          if constexpr (!TREE) {
+            const int from = row.x - first - 4 * g, to = row.y - first - 4 * g;
+            seen &= from > 63 ? 0 : from > 0 ? ~uint64_t(0) << from : ~uint64_t(0);
+            seen &= to < 0 ? 0 : to < 63 ? ~uint64_t(0) >> (63 - to) : ~uint64_t(0);
+          }
+          uint64_t drafts = 0;
+          if constexpr (TREE) drafts = s_seen[wave * 16 * C + rt * 16 + n];
+#pragma unroll
+          for (int e = 0; e < 4 * TT; ++e) {
+            const int j = 16 * (e >> 2) + (e & 3);
+            bool ok = (seen >> j) & 1;
+            if constexpr (TREE) {
+              const int draft = first + 4 * g + j - sq.offset;  // negative: context
+              const int at = draft < 0 ? sq.offset + draft : sq.offset + s_depth[draft & (kMaxDrafts - 1)];
+              ok = ok && (draft < 0 || (draft < kMaxDrafts && ((drafts >> (draft & 63)) & 1))) &&
+                   (a.window == 0 || row.z - at < a.window);
+              if constexpr (SLOPES) {
+                s[e >> 2][rt][e & 3] = fmaf(-__int_as_float(row.w), float(abs(row.z - at)), s[e >> 2][rt][e & 3]);
+              }
+            }
+            if (!ok) s[e >> 2][rt][e & 3] = kMasked;
+          }
+        }
+      }
+      float top[C];
+      bool rise = false;
+#pragma unroll
+      for (int rt = 0; rt < C; ++rt) {
+        float x = kInverse ? -s[0][rt][0] : s[0][rt][0];
+#pragma unroll
+        for (int e = 1; e < 4 * TT - 1; e += 2) {
+          const float y = s[e >> 2][rt][e & 3], z = s[(e + 1) >> 2][rt][(e + 1) & 3];
+          x = kInverse ? max3(x, -y, -z) : max3(x, y, z);
+        }
+        const float y = s[TT - 1][rt][3];
+        x = row_group_max(max2(x, kInverse ? -y : y));
+        top[rt] = fmaf(kInverse ? -mul : mul, x, add);  // a scale is positive
+        rise |= top[rt] > m[rt] + kSlack;  // m = -inf at first
+      }
+      // One condition for all row tiles, so that their exponentials are one block.
+      if (__builtin_amdgcn_ballot_w64(rise)) {
+#pragma unroll
+        for (int rt = 0; rt < C; ++rt) {
+          const float mn = fmaxf(m[rt], top[rt]);
+          const float c = mn == -INFINITY ? 1.f : fast_exp2(m[rt] - mn);
+          m[rt] = mn;
+          l[rt] *= c;
+#pragma unroll
+          for (int dt = 0; dt < NDT; ++dt) o[dt][rt] *= c;
+        }
+      }
+    };
+
+    // Prologue: K of the first two tiles, V of the first; the first tile's scores.
+    if (wave < 3) find(a0 + wave);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (wave < LW) {
+      issue(0, a0, s_k + (a0 & 1) * kTile);
+      issue(1, a0, s_v + (a0 & 1) * kTile);
+      if (a0 + 1 < a1) issue(0, a0 + 1, s_k + ((a0 + 1) & 1) * kTile);
+    }
+    if (a0 + 1 < a1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * NLD) : "memory");
+    else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NLD) : "memory");
+    {
+      const int k_off = (a0 & 1) * kTile + k_at;
+      read_keys(k_off, 0);
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        if (kk + 1 < KK) read_keys(k_off, kk + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply_keys(s, kk);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int rt = 0; rt < C; ++rt) {
+#pragma unroll
+        for (int e = 0; e < 4 * TT; ++e) s[e >> 2][rt][e & 3] = shape_of(s[e >> 2][rt][e & 3]);
+      }
+      limit(a0);
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+
+    for (int t = a0; t < a1; ++t) {
+      // Here K of tile t + 1 and V of tile t are in LDS, s holds the scores of tile t; every wave is done with K of tile
+      // t and V of tile t - 1.
+      const int stage = t & 1;
+      // The oldest wave of each SIMD, which the SIMD serves first and which would wait for the others at the barrier, loads:
+      // the loads pass the CU's address unit at 64 bytes a cycle, and a wave stands still meanwhile.
+      if (wave < LW) {
+        if (t + 2 < a1) issue(0, t + 2, s_k + stage * kTile);
+        if (t + 1 < a1) issue(1, t + 1, s_v + (stage ^ 1) * kTile);
+      }
+      if (wave == W - 1) find(t + 3);
+
+      int k_off = (stage ^ 1) * kTile + k_at, v_off = stage * kTile + v_at;
+      asm("" : "+v"(k_off), "+v"(v_off));  // the places of each k-step and column tile are computed, not held
+      // The scores of tile t + 1 (behind the last tile, of what is there: they are not used) beside the weights of tile t.
+      f32x4 ns[TT][C];
+      u32x4 pb[C][KP];
+      float base[C];
+#pragma unroll
+      for (int rt = 0; rt < C; ++rt) base[rt] = add - (m[rt] == -INFINITY ? 0.f : m[rt] - weight_lift(Tag{}));
+      read_keys(k_off, 0);
+      constexpr int EK = 4 * TT / KK;  // weights of a row tile beside a k-step
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        if (kk + 1 < KK) read_keys(k_off, kk + 1);
+        multiply_keys(ns, kk);
+#pragma unroll
+        for (int rt = 0; rt < C; ++rt) {
+#pragma unroll
+          for (int i = 0; i < EK; i += 2) {
+            const int e = kk * EK + i;
+            const float x = fast_exp2(fmaf(s[e >> 2][rt][e & 3], mul, base[rt]));
+            const float y = fast_exp2(fmaf(s[e >> 2][rt][(e & 3) + 1], mul, base[rt]));
+            l[rt] += x + y;
+            // P is rounded to the inputs' type for the matrix unit, as in the paged prefill: at most half a
+            // step of each weight (lifted in fp16, weight_lift), while l sums the unrounded ones in 32 bits.
+            pb[rt][e >> 3][(e >> 1) & 3] = pack2(x, y, Tag{});
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      // The output of tile t beside the cap of tile t + 1: V in groups of VG column tiles, read a group ahead.
+      constexpr int VG = 4, GROUPS = KP * NDT / VG, EV = 4 * TT / GROUPS;
+      u32x2 v[2][VG][2];
+      auto read_values = [&](int i) __attribute__((always_inline)) {  // group i: of keys 32 (i / (NDT / VG))
+        const int kp = i / (NDT / VG), d0 = i % (NDT / VG) * VG;
+#pragma unroll
+        for (int j = 0; j < VG; ++j) {
+          const uint16_t* from = s_v + (v_off ^ (16 * (d0 + j))) + 32 * kp * D;
+          v[i & 1][j][0] = lds_read_tr4(from);
+          v[i & 1][j][1] = lds_read_tr4(from + 16 * D);
+        }
+      };
+      read_values(0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < GROUPS; ++i) {
+        const int kp = i / (NDT / VG), d0 = i % (NDT / VG) * VG;
+        if (i + 1 < GROUPS) read_values(i + 1);
+#pragma unroll
+        for (int j = 0; j < VG; ++j) {
+          const u32x4 vv = {v[i & 1][j][0][0], v[i & 1][j][0][1], v[i & 1][j][1][0], v[i & 1][j][1][1]};
+#pragma unroll
+          for (int rt = 0; rt < C; ++rt) o[d0 + j][rt] = mfma16x16x32(vv, pb[rt][kp], o[d0 + j][rt], Tag{});
+        }
+#pragma unroll
+        for (int rt = 0; rt < C; ++rt) {
+#pragma unroll
+          for (int j = 0; j < EV; ++j) {
+            const int e = i * EV + j;
+            s[e >> 2][rt][e & 3] = shape_of(ns[e >> 2][rt][e & 3]);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (t + 1 < a1) limit(t + 1);
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+  }
+
+#pragma unroll
+  for (int rt = 0; rt < C; ++rt) {
+    const float lt = row_group_sum(l[rt]);
+    const int r = row0 + 16 * rt;
+    if (r >= rows) continue;
+    if (splits == 1) {
+      const float inv = lt != 0.f ? 1.f / lt : 0.f;  // a row that sees nothing is zero
+      const int tok = r / a.group, head = kvh * a.group + r - tok * a.group;
+      uint16_t* dst = a.out + (TREE ? b * a.o_sb : sq.q0 * a.o_st) + tok * a.o_st + head * a.o_sh + 4 * g;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) {
+        const f32x4 y = o[dt][rt] * inv;
+        *reinterpret_cast<u32x2*>(dst + 16 * dt) = u32x2{pack2(y[0], y[1], Tag{}), pack2(y[2], y[3], Tag{})};
+      }
+    } else {
+      const int64_t part = (int64_t(unit - a.whole) * splits + split) * kRows + r - qb * kRows;
+      float* dst = a.part_o + part * D + 4 * g;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<f32x4*>(dst + 16 * dt) = o[dt][rt];
+      if (g == 0) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(m[rt], lt);
+    }
+  }
+}
+
+// Joins the splits of the cut units' rows in their order: one workgroup for 16 rows.
+template <int D, bool TREE, typename Tag>
+__global__ __launch_bounds__(256) void shaped_merge_kernel(RowsArgs a) {
+  constexpr int COLS = D / 4, PAR = 256 / COLS;
+  const int cut = int(blockIdx.x) / (kRows / 16), r0 = int(blockIdx.x) % (kRows / 16) * 16;
+  const int unit = a.whole + cut, per_seq = a.blocks * a.hkv;
+  const int b = unit / per_seq, in_seq = unit - b * per_seq;
+  const int qb = a.blocks - 1 - in_seq / a.hkv, kvh = in_seq % a.hkv;
+  const Queries<TREE> sq(a, b);
+  const int rows = sq.q_len * a.group;
+  const int col = threadIdx.x % COLS;
+  for (int k = threadIdx.x / COLS; k < 16; k += PAR) {
+    const int r = qb * kRows + r0 + k;
+    if (r >= rows) break;
+    const int64_t part0 = int64_t(cut) * a.splits * kRows + r0 + k;
+    float top = -INFINITY;
+    for (int i = 0; i < a.splits; ++i) top = fmaxf(top, a.part_ml[(part0 + i * kRows) * 2]);
+    const float base = top == -INFINITY ? 0.f : top;
+    f32x4 o = {};
+    float l = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < a.splits; ++i) {
+      const int64_t part = part0 + i * kRows;
+      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + part * 2);
+      const float c = fast_exp2(ml.x - base);
+      l += c * ml.y;
+      o += c * *reinterpret_cast<const f32x4*>(a.part_o + part * D + 4 * col);
+    }
+    o *= l != 0.f ? 1.f / l : 0.f;
+    const int tok = r / a.group, head = kvh * a.group + r - tok * a.group;
+    uint16_t* dst = a.out + (TREE ? b * a.o_sb : sq.q0 * a.o_st) + tok * a.o_st + head * a.o_sh + 4 * col;
+    *reinterpret_cast<u32x2*>(dst) = u32x2{pack2(o[0], o[1], Tag{}), pack2(o[2], o[3], Tag{})};
+  }
+}
+
+inline void set_page(RowsArgs& a, int32_t page_size) {
+  a.page_size = page_size;
+  a.page_shift = page_size == 1 ? 0 : 32 - uint32_t(__builtin_clz(unsigned(page_size) - 1));
+  a.page_magic = uint32_t(((uint64_t(1) << (31 + a.page_shift)) + page_size - 1) / uint64_t(page_size));
+}
+
+template <int D, bool TREE, typename Tag>
+void launch_rows(const RowsArgs& a, hipStream_t s) {
+  const dim3 grid(unsigned(a.whole + (a.units - a.whole) * a.splits)), block(RowsShape<D>::THREADS);
+  const bool cap = a.shape.cap_log2 > 0.f, slopes = a.slopes != nullptr;
+  if (cap && slopes) hipLaunchKernelGGL((shaped_rows_kernel<D, true, true, TREE, Tag>), grid, block, 0, s, a);
+  else if (cap) hipLaunchKernelGGL((shaped_rows_kernel<D, true, false, TREE, Tag>), grid, block, 0, s, a);
+  else if (slopes) hipLaunchKernelGGL((shaped_rows_kernel<D, false, true, TREE, Tag>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((shaped_rows_kernel<D, false, false, TREE, Tag>), grid, block, 0, s, a);
+  if (a.splits > 1 && a.units > a.whole) {
+    hipLaunchKernelGGL((shaped_merge_kernel<D, TREE, Tag>), dim3(unsigned(a.units - a.whole) * (kRows / 16)), dim3(256), 0,
+                       s, a);
+  }
+}
+
+}  // namespace
+}  // namespace ti
