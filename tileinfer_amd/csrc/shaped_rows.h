@@ -88,6 +88,27 @@ __device__ __forceinline__ uint64_t drafts_seen(const RowsArgs& a, int b, int i)
   return exist & (a.mask ? uint64_t(a.mask[b * a.mask_sb + i]) : (uint64_t(2) << i) - 1);
 }
 
+// Bits [0, n) of 64.
+__device__ __forceinline__ uint64_t low_bits(int n) {
+  return n <= 0 ? 0 : n > 63 ? ~uint64_t(0) : (uint64_t(1) << (n & 63)) - 1;
+}
+
+// Which of the keys from draft number `base` on (negative: context) a row sees that sees the drafts of a mask, and the
+// context from its bit `from` on. Bits, not a test for each key: a branch for each takes longer than the tile.
+__device__ __forceinline__ uint64_t tree_seen(int base, int from, uint64_t drafts) {
+  const uint64_t context = low_bits(-base) & ~low_bits(from);
+  const uint64_t shifted = base >= 0 ? drafts >> (base & 63) : drafts << (-base & 63);
+  return context | (base > 63 || base < -63 ? 0 : shifted);
+}
+
+// The drafts of a mask that a window leaves to the draft at `depth` (s_depth: that of each).
+__device__ __forceinline__ uint64_t drafts_near(uint64_t mask, const int* s_depth, int drafts, int depth, int window) {
+  for (int k = 0; k < drafts; ++k) {
+    if (depth - s_depth[k] >= window) mask &= ~(uint64_t(1) << k);
+  }
+  return mask;
+}
+
 template <int D>
 struct RowsShape {
   static constexpr int C = D == 256 ? 1 : 2;  // row tiles of a wave
@@ -132,6 +153,12 @@ __global__ __launch_bounds__(RowsShape<D>::THREADS, 2) void shaped_rows_kernel(R
   const int rows = sq.q_len * a.group;
   if (qb * kRows >= rows) return;
 
+  if constexpr (TREE) {
+    if (int(threadIdx.x) < a.drafts) {
+      s_depth[threadIdx.x] = __builtin_popcountll(drafts_seen(a, b, threadIdx.x) & ~(uint64_t(1) << threadIdx.x));
+    }
+    __syncthreads();
+  }
   // This lane's rows and the keys they see, which stay in LDS: only tiles that a limit or a slope touches need them.
   const int row0 = qb * kRows + wave * 16 * C + n;
   u32x4 q[C][KK];
@@ -145,9 +172,11 @@ __global__ __launch_bounds__(RowsShape<D>::THREADS, 2) void shaped_rows_kernel(R
     for (int kk = 0; kk < KK; ++kk) q[rt][kk] = load16(src + 32 * kk);
     int pos = sq.offset + tok, lo = 0, hi;
     if constexpr (TREE) {
-      const uint64_t seen = drafts_seen(a, b, tok);
-      pos = sq.offset + __builtin_popcountll(seen & ~(uint64_t(1) << tok));
+      uint64_t seen = drafts_seen(a, b, tok);
+      const int depth = __builtin_popcountll(seen & ~(uint64_t(1) << tok));
+      pos = sq.offset + depth;
       hi = sq.offset - 1;  // of the context; the drafts by their bits
+      if (a.window > 0) seen = drafts_near(seen, s_depth, a.drafts, depth, a.window);
       if (g == 0) s_seen[wave * 16 * C + rt * 16 + n] = seen;
     } else {
       if (a.first_key) lo = max(a.first_key[sq.q0 + tok], 0);
@@ -164,11 +193,6 @@ __global__ __launch_bounds__(RowsShape<D>::THREADS, 2) void shaped_rows_kernel(R
     some_hi = max(some_hi, hi);
     all_lo = max(all_lo, lo);
     all_hi = min(all_hi, hi);
-  }
-  if constexpr (TREE) {
-    if (int(threadIdx.x) < a.drafts) {
-      s_depth[threadIdx.x] = __builtin_popcountll(drafts_seen(a, b, threadIdx.x) & ~(uint64_t(1) << threadIdx.x));
-    }
   }
   // Over the wave's rows: the keys that some row sees, and those that every row sees.
 #pragma unroll
@@ -319,28 +343,27 @@ __global__ __launch_bounds__(RowsShape<D>::THREADS, 2) void shaped_rows_kernel(R
 #pragma unroll
         for (int rt = 0; rt < C; ++rt) {
           const int4 row = s_row[wave * 16 * C + rt * 16 + n];
-          uint64_t seen = mine;  // bit j: key first + 4 g + j
-          if constexpr (!TREE) {
-            const int from = row.x - first - 4 * g, to = row.y - first - 4 * g;
-            seen &= from > 63 ? 0 : from > 0 ? ~uint64_t(0) << from : ~uint64_t(0);
-            seen &= to < 0 ? 0 : to < 63 ? ~uint64_t(0) >> (63 - to) : ~uint64_t(0);
-          }
-          uint64_t drafts = 0;
-          if constexpr (TREE) drafts = s_seen[wave * 16 * C + rt * 16 + n];
+          const int from = row.x - first - 4 * g;
+          uint64_t seen;  // bit j: key first + 4 g + j
+          if constexpr (TREE) {
+            const int base = first + 4 * g - sq.offset;
+            seen = mine & tree_seen(base, from, s_seen[wave * 16 * C + rt * 16 + n]);
+            if constexpr (SLOPES) {
 #pragma unroll
-          for (int e = 0; e < 4 * TT; ++e) {
-            const int j = 16 * (e >> 2) + (e & 3);
-            bool ok = (seen >> j) & 1;
-            if constexpr (TREE) {
-              const int draft = first + 4 * g + j - sq.offset;  // negative: context
-              const int at = draft < 0 ? sq.offset + draft : sq.offset + s_depth[draft & (kMaxDrafts - 1)];
-              ok = ok && (draft < 0 || (draft < kMaxDrafts && ((drafts >> (draft & 63)) & 1))) &&
-                   (a.window == 0 || row.z - at < a.window);
-              if constexpr (SLOPES) {
-                s[e >> 2][rt][e & 3] = fmaf(-__int_as_float(row.w), float(abs(row.z - at)), s[e >> 2][rt][e & 3]);
+              for (int e = 0; e < 4 * TT; ++e) {
+                const int draft = base + 16 * (e >> 2) + (e & 3);
+                int depth = s_depth[min(max(draft, 0), kMaxDrafts - 1)];
+                asm("" : "+v"(depth));  // read for every lane, not in a branch of those with a draft
+                const int dist = row.z - sq.offset - (draft < 0 ? draft : depth);
+                s[e >> 2][rt][e & 3] = fmaf(-__int_as_float(row.w), float(abs(dist)), s[e >> 2][rt][e & 3]);
               }
             }
-            if (!ok) s[e >> 2][rt][e & 3] = kMasked;
+          } else {
+            seen = mine & ~low_bits(from) & low_bits(row.y - first - 4 * g + 1);
+          }
+#pragma unroll
+          for (int e = 0; e < 4 * TT; ++e) {
+            if (!((seen >> (16 * (e >> 2) + (e & 3))) & 1)) s[e >> 2][rt][e & 3] = kMasked;
           }
         }
       }

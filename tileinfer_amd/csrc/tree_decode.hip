@@ -18,8 +18,7 @@
 // run is written by it, others leave (m, l, o) parts in 32 bits that a second kernel joins in the order of the runs.
 #include <type_traits>
 
-#include "lds_tiles.h"
-#include "score_shape.h"
+#include "shaped_rows.h"
 
 namespace ti {
 namespace {
@@ -27,9 +26,6 @@ namespace {
 constexpr int kWaves = 8;
 constexpr int kKStages = 3;    // K tiles in LDS: one in use, two on their way
 constexpr int kVStages = 4;    // V is used a tile later
-constexpr int kIdSlots = 512;  // block ids staged at a time
-constexpr int kMaxDrafts = 64;
-constexpr float kSlack = 8.f;  // exp2 units a row maximum may rise before O is rescaled
 
 struct TreeArgs {
   const uint16_t* q;
@@ -51,8 +47,6 @@ struct TreeArgs {
   ScoreShape shape;
 };
 
-__device__ __align__(16) uint16_t g_zero_row[256] = {};
-
 __device__ __forceinline__ int tree_len(const TreeArgs& a, int b) {
   const int64_t cap = int64_t(a.max_blocks) * a.page_size;
   const int n = max(a.seqlen[b], 0);
@@ -67,18 +61,6 @@ __device__ __forceinline__ int tile_count(const TreeArgs& a, int len, int tile) 
 }
 
 __device__ __forceinline__ Runs runs_of(const TreeArgs& a, uint32_t total) { return Runs(uint32_t(a.runs), total, 1u); }
-
-// One load of 16 bytes a lane into LDS: lane i's land at byte lds + 16 i. STREAM: with the nt bit, for bytes that are
-// read once.
-template <bool STREAM>
-__device__ __forceinline__ void load_lds16_at(uint64_t src, const uint16_t* lds) {
-  const uint32_t m0 = uint32_t(reinterpret_cast<uintptr_t>((lds_ptr_t)(lds)));
-  if constexpr (STREAM) {
-    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(src), "{m0}"(m0) : "memory");
-  } else {
-    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(m0) : "memory");
-  }
-}
 
 template <int N>
 __device__ __forceinline__ void wait_loads_barrier() {
@@ -206,9 +188,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel(TreeArgs a)
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) q[kk] = load16(src + 32 * kk);
     }
-    const uint64_t seen = mask_of(b, tok);
+    uint64_t seen = mask_of(b, tok);
     const int context = len - a.drafts;  // may be negative: then the drafts before 0 do not exist
     const int position = context + depth_of(seen, tok);
+    if (a.window > 0) {  // uniform
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the last sequence's depths are read
+      if (int(threadIdx.x) < a.drafts) s_depth[threadIdx.x] = depth_of(mask_of(b, threadIdx.x), threadIdx.x);
+      __syncthreads();
+      seen = drafts_near(seen, s_depth, a.drafts, position - context, a.window);
+    }
     // Tiles below this one are seen whole by every row if all their tokens are there and the window reaches.
     const int reach = a.window > 0 ? context + a.drafts - a.window : 0;
     f32x4 o[NDT];
@@ -267,12 +255,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel(TreeArgs a)
         }
 #pragma unroll
         for (int j = 0; j < NLD; ++j) {  // zeros for an absent token, not what the cache may hold there
-          load_lds16_at<false>(ok[j] ? reinterpret_cast<uint64_t>(a.k_cache) + from[j] : zero_row,
+          load_lds16_at(ok[j] ? reinterpret_cast<uint64_t>(a.k_cache) + from[j] : zero_row,
                                to_k + (wave * NLD + j) * 512);
         }
 #pragma unroll
         for (int j = 0; j < NLD; ++j) {
-          load_lds16_at<false>(ok[j] ? reinterpret_cast<uint64_t>(a.v_cache) + from[j] : zero_row,
+          load_lds16_at(ok[j] ? reinterpret_cast<uint64_t>(a.v_cache) + from[j] : zero_row,
                                to_v + (wave * NLD + j) * 512);
         }
       };
@@ -365,14 +353,21 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel(TreeArgs a)
             for (int e = 0; e < 4 * TT; ++e) x[e] = fmaf(slope, far + float(16 * (e >> 2) + (e & 3)), x[e]);
           }
         } else {
+          const int base = first + 4 * g - context;  // draft number of this lane's first key; negative: context
+          if (a.slopes) {
+#pragma unroll
+            for (int e = 0; e < 4 * TT; ++e) {
+              const int draft = base + 16 * (e >> 2) + (e & 3);
+              int depth = s_depth[min(max(draft, 0), kMaxDrafts - 1)];
+              asm("" : "+v"(depth));  // read for every lane, not in a branch of those with a draft
+              x[e] = fmaf(-slope, float(abs(position - context - (draft < 0 ? draft : depth))), x[e]);
+            }
+          }
+          const int from = a.window > 0 ? position - a.window + 1 - first - 4 * g : 0;
+          const uint64_t vis = ((mask & kAll) >> (4 * g)) & tree_seen(base, from, seen);
 #pragma unroll
           for (int e = 0; e < 4 * TT; ++e) {
-            const int j = 16 * (e >> 2) + 4 * g + (e & 3);
-            const int draft = first + j - context;  // negative: context
-            const int dist = position - (draft < 0 ? first + j : context + s_depth[draft & (kMaxDrafts - 1)]);
-            const bool ok = ((mask >> j) & 1) && (draft < 0 || (draft < kMaxDrafts && ((seen >> (draft & 63)) & 1))) &&
-                            (a.window == 0 || dist < a.window);
-            x[e] = ok ? (a.slopes ? fmaf(-slope, float(abs(dist)), x[e]) : x[e]) : -INFINITY;
+            if (!((vis >> (16 * (e >> 2) + (e & 3))) & 1)) x[e] = -INFINITY;
           }
         }
         float top = x[0];
@@ -527,13 +522,31 @@ int rows_per_block(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64
 int64_t align16(int64_t x) { return (x + 15) & ~int64_t(15); }
 
 struct TreeSizes {
-  int32_t rb, row_blocks, runs;
-  int64_t o_floats, ml_floats, bytes;
+  int32_t rb, row_blocks, runs;  // few rows: of this file's kernel
+  int32_t blocks, splits;        // many rows (splits > 0): units of shaped_rows.h
+  int64_t units, o_floats, ml_floats, bytes;
 };
 
-TreeSizes tree_sizes(int32_t batch, int32_t drafts, int32_t hq, int32_t hkv, int32_t head_dim) {
-  TreeSizes s;
+// Rows of a KV head beyond which the tree goes to the kernel of shaped_rows.h, whose workgroups take 128 rows at a time.
+constexpr int kFewRows = 64;
+
+TreeSizes tree_sizes(int32_t batch, int32_t drafts, int32_t hq, int32_t hkv, int32_t head_dim, int64_t max_k) {
+  TreeSizes s{};
   const int64_t rows = int64_t(drafts) * (hq / hkv);
+  if (rows > kFewRows) {
+    s.blocks = int32_t(ceil_div(rows, kRows));
+    s.units = int64_t(batch) * s.blocks * hkv;
+    const int64_t slots = int64_t(device_cu_count()) * (head_dim == 256 ? 1 : 2);
+    const int64_t splits = ceil_div(2 * slots, s.units < 1 ? 1 : s.units), most = max_k / (4 * kKeys);
+    const int64_t n = splits > most ? most : splits;
+    s.splits = int32_t(n < 1 ? 1 : n);
+    if (s.splits > 1) {
+      s.o_floats = s.units * s.splits * kRows * head_dim;
+      s.ml_floats = s.units * s.splits * kRows * 2;
+    }
+    s.bytes = (s.o_floats + s.ml_floats) * 4;
+    return s;
+  }
   s.rb = rows_per_block(rows);
   s.row_blocks = int32_t(ceil_div(rows, s.rb));
   const int64_t lists = int64_t(hkv) * s.row_blocks;  // workgroups of a run, one a CU: its LDS
@@ -576,13 +589,18 @@ void launch_tree(const TreeArgs& a, int rb, hipStream_t s) {
 }  // namespace ti
 
 extern "C" int ti_gqa_tree_workspace_bytes(int32_t batch, int32_t num_drafts, int32_t num_q_heads, int32_t num_kv_heads,
-                                           int32_t head_dim, int64_t* workspace_bytes_out) {
+                                           int32_t head_dim, int32_t page_size, int32_t max_blocks_per_seq,
+                                           int64_t* workspace_bytes_out) {
   using namespace ti;
   const char* who = "ti_gqa_tree_workspace_bytes";
   const int rc = check_tree(who, batch, num_drafts, num_q_heads, num_kv_heads, head_dim);
   if (rc != TI_OK) return rc;
   if (!workspace_bytes_out) return fail(TI_EINVAL, "%s: null output", who);
-  *workspace_bytes_out = tree_sizes(batch, num_drafts, num_q_heads, num_kv_heads, head_dim).bytes;
+  if (page_size <= 0 || max_blocks_per_seq < 0) {
+    return fail(TI_EINVAL, "%s: bad table page_size=%d max_blocks_per_seq=%d", who, page_size, max_blocks_per_seq);
+  }
+  *workspace_bytes_out = tree_sizes(batch, num_drafts, num_q_heads, num_kv_heads, head_dim,
+                                    int64_t(max_blocks_per_seq) * page_size).bytes;
   return TI_OK;
 }
 
@@ -618,7 +636,8 @@ extern "C" int ti_gqa_tree_paged(const void* q, int64_t q_stride_b, int64_t q_st
                 max_blocks_per_seq, page_size);
   }
   if (batch == 0) return TI_OK;
-  if (!q || !seqlen || !out || !workspace || (max_blocks_per_seq > 0 && (!k_cache || !v_cache || !block_table))) {
+  const TreeSizes sz = tree_sizes(batch, num_drafts, num_q_heads, num_kv_heads, head_dim, tokens);
+  if (!q || !seqlen || !out || (sz.bytes > 0 && !workspace) || (max_blocks_per_seq > 0 && (!k_cache || !v_cache || !block_table))) {
     return fail(TI_EINVAL, "%s: null pointer", who);
   }
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) |
@@ -626,10 +645,54 @@ extern "C" int ti_gqa_tree_paged(const void* q, int64_t q_stride_b, int64_t q_st
       q_stride_b % 8 != 0 || q_stride_t % 8 != 0 || q_stride_h % 8 != 0) {
     return fail(TI_EINVAL, "%s: q, caches, out and workspace must be 16-byte aligned, q strides multiples of 8", who);
   }
-  const TreeSizes sz = tree_sizes(batch, num_drafts, num_q_heads, num_kv_heads, head_dim);
   if (workspace_bytes < sz.bytes) {
     return fail(TI_EINVAL, "%s: workspace %lld < %lld bytes", who, static_cast<long long>(workspace_bytes),
                 static_cast<long long>(sz.bytes));
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool bf16 = dtype == TI_DTYPE_BF16;
+  const int32_t near = window > tokens + kMaxDrafts ? 0 : window;  // none where it is wider than any distance
+  if (sz.splits > 0) {
+    RowsArgs a{};
+    a.q = static_cast<const uint16_t*>(q);
+    a.q_sb = q_stride_b;
+    a.q_st = q_stride_t;
+    a.q_sh = q_stride_h;
+    a.k_cache = static_cast<const uint16_t*>(k_cache);
+    a.v_cache = static_cast<const uint16_t*>(v_cache);
+    a.block_table = block_table;
+    a.bt_stride = block_table_stride;
+    a.seqlen = seqlen;
+    a.slopes = slopes;
+    a.out = static_cast<uint16_t*>(out);
+    a.o_sh = head_dim;
+    a.o_st = int64_t(num_q_heads) * head_dim;
+    a.o_sb = a.o_st * num_drafts;
+    a.mask = tree_mask;
+    a.mask_sb = mask_stride_b;
+    a.drafts = num_drafts;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + sz.o_floats;
+    a.units = int32_t(sz.units);
+    a.whole = sz.splits > 1 ? 0 : a.units;
+    a.splits = sz.splits;
+    a.blocks = sz.blocks;
+    a.hq = num_q_heads;
+    a.hkv = num_kv_heads;
+    a.group = num_q_heads / num_kv_heads;
+    a.num_blocks32 = int32_t(num_blocks);
+    set_page(a, page_size);
+    a.max_blocks = max_blocks_per_seq;
+    a.window = near;
+    a.shape = score_shape(scale, softcap);
+    if (head_dim == 256) {
+      if (bf16) launch_rows<256, true, Bf16>(a, s);
+      else launch_rows<256, true, F16>(a, s);
+    } else {
+      if (bf16) launch_rows<128, true, Bf16>(a, s);
+      else launch_rows<128, true, F16>(a, s);
+    }
+    return check_launch(who);
   }
   TreeArgs a{};
   a.q = static_cast<const uint16_t*>(q);
@@ -660,10 +723,8 @@ extern "C" int ti_gqa_tree_paged(const void* q, int64_t q_stride_b, int64_t q_st
   a.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(unsigned(page_size)) : -1;
   a.max_blocks = max_blocks_per_seq;
   a.runs = sz.runs;
-  a.window = window > tokens + kMaxDrafts ? 0 : window;  // wider than any distance
+  a.window = near;
   a.shape = score_shape(scale, softcap);
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool bf16 = dtype == TI_DTYPE_BF16;
   if (head_dim == 256) {
     if (bf16) launch_tree<256, Bf16>(a, sz.rb, s);
     else launch_tree<256, F16>(a, sz.rb, s);
