@@ -191,7 +191,8 @@ _BOUND = ("ti_kv_append", "ti_gqa_decode_plan", "ti_gqa_decode_paged", "ti_gqa_d
           "ti_gqa_decode_paged_append", "ti_gqa_prefill_paged", "ti_gqa_prefill_paged_gated",
           "ti_gqa_prefill_workspace_bytes", "ti_qknorm_rope_append", "ti_latent_rope_append",
           "ti_latent_decode_workspace_bytes", "ti_latent_decode_paged", "ti_cache_mass_workspace_bytes",
-          "ti_cache_mass", "ti_evict_kvcache")
+          "ti_cache_mass", "ti_evict_kvcache", "ti_rope_axes_append", "ti_gqa_tree_workspace_bytes",
+          "ti_gqa_tree_paged", "ti_keep_drafts", "ti_gqa_prefill_shaped_workspace_bytes", "ti_gqa_prefill_shaped")
 _calls = None
 
 

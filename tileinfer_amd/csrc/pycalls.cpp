@@ -42,6 +42,12 @@ decltype(&ti_latent_decode_paged) p_latent_decode = nullptr;
 decltype(&ti_cache_mass_workspace_bytes) p_mass_ws = nullptr;
 decltype(&ti_cache_mass) p_mass = nullptr;
 decltype(&ti_evict_kvcache) p_evict = nullptr;
+decltype(&ti_rope_axes_append) p_rope_axes = nullptr;
+decltype(&ti_gqa_tree_workspace_bytes) p_tree_ws = nullptr;
+decltype(&ti_gqa_tree_paged) p_tree = nullptr;
+decltype(&ti_keep_drafts) p_keep = nullptr;
+decltype(&ti_gqa_prefill_shaped_workspace_bytes) p_shaped_ws = nullptr;
+decltype(&ti_gqa_prefill_shaped) p_shaped = nullptr;
 
 // A plain tensor with memory of its own on a GPU, or nullptr.
 const at::Tensor* plain(PyObject* o) {
@@ -607,13 +613,246 @@ PyObject* evict(PyObject* const* a) {
   return r;
 }
 
+// An optional contiguous vector of n values of one type; false where it needs a copy or is wrong.
+bool vector_or_none(PyObject* o, at::ScalarType type, int64_t n, const at::Device& dev, const at::Tensor** out) {
+  *out = nullptr;
+  if (o == Py_None) return true;
+  const at::Tensor* t = plain(o);
+  if (!t || t->scalar_type() != type || t->dim() != 1 || t->size(0) != n || !t->is_contiguous() || t->device() != dev) {
+    return false;
+  }
+  *out = t;
+  return true;
+}
+
+// The shape of scores: softcap (None: 0) and window (None: 0).
+bool shape_of(PyObject* cap, PyObject* window, float& c, int32_t& w) {
+  c = 0.f;
+  w = 0;
+  if (cap != Py_None) {
+    if (!PyFloat_CheckExact(cap)) return false;
+    const double x = PyFloat_AS_DOUBLE(cap);
+    if (!(x >= 1e-3 && x <= 1e4)) return false;
+    c = float(x);
+  }
+  if (window != Py_None) {
+    int64_t x;
+    if (!int_of(window, x) || x < 1) return false;
+    w = x > INT32_MAX ? INT32_MAX : int32_t(x);
+  }
+  return true;
+}
+
+// A cache like another one.
+bool same_cache(const at::Tensor* v, const at::Tensor& k) {
+  return v && v->sizes() == k.sizes() && v->scalar_type() == k.scalar_type() && v->device() == k.device() &&
+         v->is_contiguous() && address(*v) % 16 == 0;
+}
+
+// (q, k, v, positions, inv_freq, axes | None, k_cache, v_cache, slots, q_weight | None, k_weight | None, eps,
+//  weight_offset, stream) -> q_out
+PyObject* rope_axes_append(PyObject* const* a) {
+  const at::Tensor* t[3];
+  for (int i = 0; i < 3; ++i) {
+    t[i] = plain(a[i]);
+    if (!t[i] || t[i]->dim() != 3 || !aligned_rows(*t[i], 8)) Py_RETURN_NONE;
+  }
+  const at::Tensor &q = *t[0], &k = *t[1], &v = *t[2];
+  const at::Tensor *pos = plain(a[3]), *inv = plain(a[4]), *kc = plain(a[6]), *vc = plain(a[7]), *slots = plain(a[8]);
+  if (!pos || !inv || !kc || !vc || !slots || !PyFloat_CheckExact(a[11]) || !PyFloat_CheckExact(a[12])) Py_RETURN_NONE;
+  const int64_t n = q.size(0), hq = q.size(1), d = q.size(2), hkv = k.size(1), half = inv->dim() == 1 ? inv->size(0) : -1;
+  const at::Device dev = q.device();
+  const int code = dtype_code(q);
+  const bool wide = pos->scalar_type() == at::kLong;
+  const int64_t axes = pos->dim() == 2 ? pos->size(0) : 1;
+  if (code < 0 || n <= 0 || hq <= 0 || hkv <= 0 || (d != 128 && d != 256) || k.sizes() != v.sizes() || k.size(0) != n ||
+      k.size(2) != d || half < 0 || half % 8 != 0 || 2 * half > 128 || inv->scalar_type() != at::kFloat ||
+      !inv->is_contiguous() || (!wide && pos->scalar_type() != at::kInt) || pos->dim() < 1 || pos->dim() > 2 ||
+      pos->size(-1) != n || pos->stride(-1) != 1 || axes < 1 || axes > 4 || !int32_vector(*slots, n, dev) ||
+      kc->dim() != 2 || vc->sizes() != kc->sizes() || vc->strides() != kc->strides() || kc->size(1) != hkv * d ||
+      kc->stride(0) < hkv * d || !aligned_rows(*kc, 8) || !aligned_rows(*vc, 8) || !fits32(n) || !fits32(hq) ||
+      !fits32(hkv)) {
+    Py_RETURN_NONE;
+  }
+  for (const at::Tensor* x : {&k, &v, kc, vc}) {
+    if (x->scalar_type() != q.scalar_type() || x->device() != dev) Py_RETURN_NONE;
+  }
+  if (pos->device() != dev || inv->device() != dev) Py_RETURN_NONE;
+  const at::Tensor *axis_of, *qw, *kw;
+  if (!vector_or_none(a[5], at::kInt, half, dev, &axis_of) || !vector_or_none(a[9], q.scalar_type(), d, dev, &qw) ||
+      !vector_or_none(a[10], q.scalar_type(), d, dev, &kw) || !qw != !kw ||
+      (qw && (address(*qw) % 16 != 0 || address(*kw) % 16 != 0))) {
+    Py_RETURN_NONE;
+  }
+  void* stream = stream_of(a[13]);
+  at::Tensor out;
+  int rc;
+  {
+    Unlocked unlocked;
+    out = at::empty({n, hq, d}, q.options());
+    rc = p_rope_axes(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+                     v.stride(0), v.stride(1), pos->data_ptr(), pos->dim() == 2 ? pos->stride(0) : 0, wide ? 64 : 32,
+                     static_cast<const float*>(inv->data_ptr()),
+                     axis_of ? static_cast<const int32_t*>(axis_of->data_ptr()) : nullptr, qw ? qw->data_ptr() : nullptr,
+                     kw ? kw->data_ptr() : nullptr, float(PyFloat_AS_DOUBLE(a[12])), out.data_ptr(), hq * d, d,
+                     kc->data_ptr(), vc->data_ptr(), kc->stride(0), kc->size(0),
+                     static_cast<const int32_t*>(slots->data_ptr()), int32_t(n), int32_t(axes), int32_t(hq), int32_t(hkv),
+                     int32_t(d), int32_t(2 * half), float(PyFloat_AS_DOUBLE(a[11])), code, stream);
+  }
+  if (rc != TI_OK) return PyLong_FromLong(rc);
+  return THPVariable_Wrap(std::move(out));
+}
+
+// (q, k_cache, v_cache, block_table, seqlen, tree_mask | None, page_size, scale, softcap | None, slopes | None,
+//  window | None, stream)
+PyObject* tree(PyObject* const* a) {
+  Pages p;
+  Queries q;
+  float scale, cap;
+  int32_t window;
+  const at::Tensor *v = plain(a[2]), *mask = nullptr, *slopes;
+  if (!pages(a[1], a[3], a[4], a[6], p) || !queries(a[0], p, q) || !scale_of(a[7], scale) ||
+      !shape_of(a[8], a[10], cap, window) || !same_cache(v, *p.cache)) {
+    Py_RETURN_NONE;
+  }
+  const at::Device dev = p.cache->device();
+  const int64_t hkv = p.cache->size(2);
+  if ((q.dim != 128 && q.dim != 256) || hkv <= 0 || q.heads % hkv != 0 || q.tokens > 64 ||
+      !vector_or_none(a[9], at::kFloat, q.heads, dev, &slopes)) {
+    Py_RETURN_NONE;
+  }
+  if (a[5] != Py_None) {
+    mask = plain(a[5]);
+    if (!mask || mask->scalar_type() != at::kLong || mask->device() != dev || mask->dim() < 1 || mask->dim() > 2 ||
+        mask->size(-1) != q.tokens || mask->stride(-1) != 1 || (mask->dim() == 2 && mask->size(0) != p.batch)) {
+      Py_RETURN_NONE;
+    }
+  }
+  void* stream = stream_of(a[11]);
+  at::Tensor out;
+  int rc;
+  {
+    Unlocked unlocked;
+    int64_t ws_bytes = 0;
+    rc = p_tree_ws(int32_t(p.batch), int32_t(q.tokens), int32_t(q.heads), int32_t(hkv), int32_t(q.dim), int32_t(p.page),
+                   int32_t(p.width), &ws_bytes);
+    if (rc == TI_OK) {
+      out = at::empty(q.q->sizes(), q.q->options());
+      at::Tensor ws;
+      if (ws_bytes > 0) ws = bytes_on(*q.q, ws_bytes);
+      rc = p_tree(q.q->data_ptr(), q.st_b, q.st_t, q.st_h, p.cache->data_ptr(), v->data_ptr(),
+                  static_cast<const int32_t*>(p.table->data_ptr()), p.table->stride(0),
+                  static_cast<const int32_t*>(p.lens->data_ptr()),
+                  mask ? static_cast<const int64_t*>(mask->data_ptr()) : nullptr,
+                  mask && mask->dim() == 2 ? mask->stride(0) : 0,
+                  slopes ? static_cast<const float*>(slopes->data_ptr()) : nullptr, out.data_ptr(),
+                  ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, int32_t(p.batch), int32_t(q.tokens),
+                  int32_t(q.heads), int32_t(hkv), int32_t(q.dim), int32_t(p.page), p.rows / p.page, int32_t(p.width),
+                  scale, cap, window, dtype_code(*q.q), stream);
+    }
+  }
+  if (rc != TI_OK) return PyLong_FromLong(rc);
+  return THPVariable_Wrap(std::move(out));
+}
+
+// (cache, block_table, seqlen, accepted, page_size, num_drafts, stream) -> new_seqlen
+PyObject* keep(PyObject* const* a) {
+  const at::Tensor *cache = plain(a[0]), *table = plain(a[1]), *lens = plain(a[2]), *accepted = plain(a[3]);
+  int64_t page, drafts;
+  if (!cache || !table || !lens || !accepted || !int_of(a[4], page) || !int_of(a[5], drafts)) Py_RETURN_NONE;
+  const at::Device dev = cache->device();
+  const int64_t n = cache->dim();
+  if (n < 4 || table->dim() != 2 || accepted->dim() != 2 || cache->numel() == 0 || !cache->is_contiguous() ||
+      address(*cache) % 16 != 0 || dtype_code(*cache) < 0 || table->scalar_type() != at::kInt || table->stride(1) != 1 ||
+      table->device() != dev || accepted->scalar_type() != at::kInt || accepted->stride(1) != 1 ||
+      accepted->device() != dev) {
+    Py_RETURN_NONE;
+  }
+  const int64_t batch = table->size(0), rows = cache->size(n - 4) * cache->size(n - 3);
+  const int64_t row = cache->size(n - 2) * cache->size(n - 1), planes = cache->numel() / (rows * row);
+  if (batch <= 0 || accepted->size(0) != batch || !int32_vector(*lens, batch, dev) || page <= 0 || rows % page != 0 ||
+      row % 8 != 0 || drafts < 1 || drafts > 64 || !fits32(batch) || !fits32(page) || !fits32(planes) ||
+      !fits32(accepted->size(1)) || !fits32(table->size(1))) {
+    Py_RETURN_NONE;
+  }
+  void* stream = stream_of(a[6]);
+  at::Tensor out;
+  int rc;
+  {
+    Unlocked unlocked;
+    out = at::empty({batch}, lens->options());
+    rc = p_keep(cache->data_ptr(), static_cast<const int32_t*>(table->data_ptr()), table->stride(0),
+                static_cast<const int32_t*>(lens->data_ptr()), static_cast<const int32_t*>(accepted->data_ptr()),
+                accepted->stride(0), static_cast<int32_t*>(out.data_ptr()), int32_t(batch), int32_t(drafts),
+                int32_t(accepted->size(1)), int32_t(planes), row, int32_t(page), rows / page, int32_t(table->size(1)),
+                stream);
+  }
+  if (rc != TI_OK) return PyLong_FromLong(rc);
+  return THPVariable_Wrap(std::move(out));
+}
+
+// (q, k_cache, v_cache, block_table, cu_seqlens_q, seqlen_k, max_seqlen_q, page_size, causal, scale, softcap | None,
+//  slopes | None, window | None, first_key | None, last_key | None, max_seqlen_k | None, stream)
+PyObject* shaped(PyObject* const* a) {
+  Pages p;
+  float scale, cap;
+  int32_t window;
+  const at::Tensor *q = plain(a[0]), *v = plain(a[2]), *cu = plain(a[4]), *slopes, *first, *last;
+  int64_t max_q, max_k = INT64_MAX;
+  if (!q || !cu || !pages(a[1], a[3], a[5], a[7], p) || !same_cache(v, *p.cache) || !int_of(a[6], max_q) ||
+      !PyBool_Check(a[8]) || !scale_of(a[9], scale) || !shape_of(a[10], a[12], cap, window) ||
+      (a[15] != Py_None && !int_of(a[15], max_k))) {
+    Py_RETURN_NONE;
+  }
+  const at::Device dev = p.cache->device();
+  if (q->dim() != 3 || !aligned_rows(*q, 8) || q->scalar_type() != p.cache->scalar_type() || q->device() != dev) {
+    Py_RETURN_NONE;
+  }
+  const int64_t n = q->size(0), hq = q->size(1), d = q->size(2), hkv = p.cache->size(2);
+  if (n <= 0 || hq <= 0 || hkv <= 0 || hq % hkv != 0 || (d != 128 && d != 256) || p.cache->size(3) != d || max_q < 0 ||
+      max_k < 0 || !int32_vector(*cu, p.batch + 1, dev) || !fits32(n) || !fits32(hq) || !fits32(p.page) ||
+      !vector_or_none(a[11], at::kFloat, hq, dev, &slopes) || !vector_or_none(a[13], at::kInt, n, dev, &first) ||
+      !vector_or_none(a[14], at::kInt, n, dev, &last)) {
+    Py_RETURN_NONE;
+  }
+  max_q = max_q < n ? max_q : n;
+  const int64_t bound = p.width * p.page;
+  max_k = max_k < bound ? max_k : bound;
+  void* stream = stream_of(a[16]);
+  at::Tensor out;
+  int rc;
+  {
+    Unlocked unlocked;
+    int64_t ws_bytes = 0;
+    rc = p_shaped_ws(int32_t(p.batch), int32_t(n), int32_t(max_q), int32_t(hq), int32_t(hkv), int32_t(d), max_k, &ws_bytes);
+    if (rc == TI_OK) {
+      out = at::empty({n, hq, d}, q->options());
+      at::Tensor ws;
+      if (ws_bytes > 0) ws = bytes_on(*q, ws_bytes);
+      rc = p_shaped(q->data_ptr(), q->stride(0), q->stride(1), p.cache->data_ptr(), v->data_ptr(),
+                    static_cast<const int32_t*>(p.table->data_ptr()), p.table->stride(0),
+                    static_cast<const int32_t*>(cu->data_ptr()), static_cast<const int32_t*>(p.lens->data_ptr()),
+                    first ? static_cast<const int32_t*>(first->data_ptr()) : nullptr,
+                    last ? static_cast<const int32_t*>(last->data_ptr()) : nullptr,
+                    slopes ? static_cast<const float*>(slopes->data_ptr()) : nullptr, out.data_ptr(), hq * d, d,
+                    ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, int32_t(p.batch), int32_t(n), int32_t(max_q),
+                    int32_t(hq), int32_t(hkv), int32_t(d), int32_t(p.page), p.rows / p.page, int32_t(p.width), max_k,
+                    a[8] == Py_True, scale, cap, window, dtype_code(*q), stream);
+    }
+  }
+  if (rc != TI_OK) return PyLong_FromLong(rc);
+  return THPVariable_Wrap(std::move(out));
+}
+
 // The library's entry points by address, in the order of the list below.
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   void** slots[] = {(void**)&p_append,        (void**)&p_plan,          (void**)&p_decode,
                     (void**)&p_decode_gated,  (void**)&p_decode_append, (void**)&p_prefill,
                     (void**)&p_prefill_gated, (void**)&p_prefill_ws,    (void**)&p_qknorm_append,
                     (void**)&p_latent_append, (void**)&p_latent_ws,     (void**)&p_latent_decode,
-                    (void**)&p_mass_ws,       (void**)&p_mass,          (void**)&p_evict};
+                    (void**)&p_mass_ws,       (void**)&p_mass,          (void**)&p_evict,
+                    (void**)&p_rope_axes,     (void**)&p_tree_ws,       (void**)&p_tree,
+                    (void**)&p_keep,          (void**)&p_shaped_ws,     (void**)&p_shaped};
   if (n != Py_ssize_t(sizeof(slots) / sizeof(slots[0]))) {
     PyErr_SetString(PyExc_TypeError, "bind: one address for each entry point");
     return nullptr;
@@ -642,6 +881,10 @@ PyMethodDef methods[] = {{"bind", (PyCFunction)(void (*)(void))bind, METH_FASTCA
                          TI_METHOD(latent_decode, 7),
                          TI_METHOD(cache_mass, 8),
                          TI_METHOD(evict, 11),
+                         TI_METHOD(rope_axes_append, 14),
+                         TI_METHOD(tree, 12),
+                         TI_METHOD(keep, 7),
+                         TI_METHOD(shaped, 17),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pycalls", nullptr, -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

@@ -107,7 +107,7 @@ extern "C" int ti_gqa_prefill_shaped(const void* q, int64_t q_stride_t, int64_t 
                 "2^31 - 1 rows)", who, page_size, static_cast<long long>(num_blocks), max_blocks_per_seq);
   }
   const int64_t tokens = int64_t(max_blocks_per_seq) * page_size;
-  if (tokens > INT32_MAX - 256) {
+  if (tokens > INT32_MAX - 1024) {  // tiles ahead of the last one are counted too
     return fail(TI_EINVAL, "%s: max_blocks_per_seq %d x page_size %d exceeds 2^31", who, max_blocks_per_seq, page_size);
   }
   if (batch == 0 || total_q == 0 || max_seqlen_q == 0) return TI_OK;

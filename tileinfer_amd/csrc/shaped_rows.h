@@ -564,7 +564,8 @@ __global__ __launch_bounds__(256) void shaped_merge_kernel(RowsArgs a) {
   }
 }
 
-inline void set_page(RowsArgs& a, int32_t page_size) {
+template <typename Args>
+void set_page(Args& a, int32_t page_size) {
   a.page_size = page_size;
   a.page_shift = page_size == 1 ? 0 : 32 - uint32_t(__builtin_clz(unsigned(page_size) - 1));
   a.page_magic = uint32_t(((uint64_t(1) << (31 + a.page_shift)) + page_size - 1) / uint64_t(page_size));

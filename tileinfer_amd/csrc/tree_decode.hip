@@ -13,9 +13,11 @@
 // a row group adds them up in the same order and keeps the same statistics; the next tile's scores are computed beside
 // this tile's output, one barrier a tile.
 //
-// The batch's tiles are one list, cut into runs of equal length; a run is taken by one workgroup for each KV head and
-// row block, side by side, so that the row blocks of a head (on one XCD) find its rows in L2. A sequence that lies in one
-// run is written by it, others leave (m, l, o) parts in 32 bits that a second kernel joins in the order of the runs.
+// The batch's tiles are one list, cut into runs of equal length; a run is taken by one workgroup for each KV head, side
+// by side, since the heads' rows of a token lie side by side in memory. A sequence that lies in one run is written by it,
+// others leave (m, l, o) parts in 32 bits that a second kernel joins in the order of the runs.
+//
+// Trees of more than 64 rows a KV head go to the kernel of shaped_rows.h.
 #include <type_traits>
 
 #include "shaped_rows.h"
@@ -39,10 +41,11 @@ struct TreeArgs {
   int64_t mask_sb;
   const float* slopes;  // [hq] or nullptr
   uint16_t* out;        // [B, N, hq, D]
-  float* part_o;        // [runs][hkv * row_blocks][2][RB][D] unnormalised rows
-  float* part_ml;       // [runs][hkv * row_blocks][2][RB][2] their (m, l), m in exp2 units
+  float* part_o;        // [runs][hkv][2][RB][D] unnormalised rows
+  float* part_ml;       // [runs][hkv][2][RB][2] their (m, l), m in exp2 units
   int32_t* first_tile;  // [B + 1] each sequence's first tile, and the total
-  int32_t batch, drafts, hq, hkv, group, rows, row_blocks, num_blocks32, page_size, page_shift, max_blocks;
+  int32_t batch, drafts, hq, hkv, group, rows, num_blocks32, page_size, max_blocks;
+  uint32_t page_magic, page_shift;  // as RowsArgs has them
   int32_t runs, window;  // window 0: none
   ScoreShape shape;
 };
@@ -60,7 +63,22 @@ __device__ __forceinline__ int tile_count(const TreeArgs& a, int len, int tile) 
   return (len + tile - 1) / tile - tile_begin(a, len, tile);
 }
 
+// Calls of at least this many 32 KiB tiles load their rows with the streaming policy; shorter ones, which the last-level
+// cache may still hold, keep the default one.
+constexpr int64_t kStreamTiles = 2400;
+
 __device__ __forceinline__ Runs runs_of(const TreeArgs& a, uint32_t total) { return Runs(uint32_t(a.runs), total, 1u); }
+
+// As load_lds16_at. STREAM: with the nt bit, for bytes that are read once.
+template <bool STREAM>
+__device__ __forceinline__ void load_lds16_as(uint64_t src, const uint16_t* lds) {
+  if constexpr (STREAM) {
+    const uint32_t m0 = uint32_t(reinterpret_cast<uintptr_t>((lds_ptr_t)(lds)));
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(src), "{m0}"(m0) : "memory");
+  } else {
+    load_lds16_at(src, lds);
+  }
+}
 
 template <int N>
 __device__ __forceinline__ void wait_loads_barrier() {
@@ -92,6 +110,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel(TreeArgs a)
   __shared__ f32x4 s_s[2][KS][RG][TT][64];  // scores of the next tile and of this one
   __shared__ int s_ids[kIdSlots];
   __shared__ int s_depth[kMaxDrafts];
+  __shared__ __align__(16) uint64_t s_from[4][T][2];  // addresses of a tile's tokens in K and in V
+  __shared__ uint64_t s_here[8];                      // and which of them exist
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -100,9 +120,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel(TreeArgs a)
   const int q_tt = wave * JW % TT, q_rest = wave * JW / TT;  // of the first
   const int q_rg = q_rest % RG, q_ks = q_rest / RG;
 
-  const int units = a.runs * a.hkv;
-  const int rb = int(blockIdx.x) / units, unit = int(blockIdx.x) - rb * units;
-  const int run = unit / a.hkv, kvh = unit - run * a.hkv;
+  const int run = int(blockIdx.x) / a.hkv, kvh = int(blockIdx.x) - run * a.hkv;
 
   // The batch's tiles, this run's share of them, and the sequence in which it starts.
   uint32_t total = 0;
@@ -136,14 +154,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel(TreeArgs a)
     unit0 += sum;
   }
 
-  // This lane's part of a tile's loads: chunk c of row r lies at c ^ swz16(r).
-  uint32_t src_off[NLD];
-  int src_row[NLD];
-#pragma unroll
-  for (int i = 0; i < NLD; ++i) {
-    src_row[i] = (wave * NLD + i) * RPL + lane / CH;
-    src_off[i] = uint32_t(kvh) * (2 * D) + 16 * ((lane % CH) ^ swz16(src_row[i]));
-  }
+  // Load j of a wave takes the tile's rows kStep j + load_row; chunk c of row r lies at c ^ swz16(r), the same in rows 16
+  // apart.
+  constexpr int kStep = kWaves * RPL;
+  static_assert(kStep % 16 == 0);
+  const int load_row = wave * RPL + lane / CH;
+  const uint32_t lane_off = 16 * ((lane % CH) ^ swz16(load_row));
   // Its operand reads (elements): of K rows 16 (q_tt + j) + n each k-step, of V row 4 g + n / 4.
   int k_at[KK], v_at[NDT];
 #pragma unroll
@@ -155,12 +171,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel(TreeArgs a)
       v_at[o] = r * D + 8 * ((2 * (dg * NDT + o) + ((lane >> 1) & 1)) ^ swz16(r)) + 4 * (lane & 1);
     }
   }
-  const uint64_t row_bytes = uint64_t(a.hkv) * (2 * D);
   uint64_t zero_row = reinterpret_cast<uint64_t>(g_zero_row);
   asm("" : "+s"(zero_row));  // held, not looked up again for every tile
 
   // This lane's row of the second product: its draft, head and slope (rows behind the last repeat it, not stored).
-  const int row = rb * RB + rg * 16 + n;
+  const int row = rg * 16 + n;
   const int tok = min(row, a.rows - 1) / a.group, head = kvh * a.group + min(row, a.rows - 1) - tok * a.group;
   const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
   const uint64_t exist = a.drafts == 64 ? ~uint64_t(0) : (uint64_t(1) << a.drafts) - 1;
@@ -182,7 +197,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel(TreeArgs a)
 
     u32x4 q[KK];
     {
-      const int r = min(rb * RB + q_rg * 16 + n, a.rows - 1);
+      const int r = min(q_rg * 16 + n, a.rows - 1);
       const int i = r / a.group, h = kvh * a.group + r - i * a.group;
       const uint16_t* src = a.q + b * a.q_sb + i * a.q_st + h * a.q_sh + 32 * KK * q_ks + 8 * g;
 #pragma unroll
@@ -199,6 +214,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel(TreeArgs a)
     }
     // Tiles below this one are seen whole by every row if all their tokens are there and the window reaches.
     const int reach = a.window > 0 ? context + a.drafts - a.window : 0;
+    // Rows that no other sequence reads are streamed (kPolicyStream). A sequence whose first block another one also starts
+    // with shares pages with it (prefix caching shares whole chains of blocks from the first on).
+    bool stream = int64_t(total) * a.hkv >= kStreamTiles;
+    if (stream) {
+      const int first = a.block_table[b * a.bt_stride];
+      for (int b0 = 0; b0 < a.batch; b0 += 64) {
+        const int other = b0 + lane;
+        if (__builtin_amdgcn_ballot_w64(other < a.batch && other != b &&
+                                        a.block_table[min(other, a.batch - 1) * a.bt_stride] == first)) {
+          stream = false;
+        }
+      }
+    }
     f32x4 o[NDT];
     float m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -220,49 +248,40 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel(TreeArgs a)
       __builtin_amdgcn_s_waitcnt(0);
       asm volatile("s_barrier" ::: "memory");
 
-      // Token lane % T of the tile to load next: position, slot of its block id, place in the block. They
-      // advance tile by tile, without a division.
-      int pos = a0 * T + (lane & (T - 1));
-      int slot = a.page_shift >= 0 ? pos >> a.page_shift : pos / a.page_size;
-      int in_page = pos - slot * a.page_size;
-      slot -= page0;
-      const int step_slots = T / a.page_size, step_rest = T % a.page_size;
-      auto read_id = [&]() { return s_ids[min(slot, kIdSlots - 1)]; };
-      uint64_t here = 0;  // the tile's tokens that exist
-      // That token's cache row given its block id (-1: absent), and on to the next tile.
-      auto row_of = [&](int id) {
-        const bool ok = pos < min(len, a1 * T) && uint32_t(id) < uint32_t(a.num_blocks32);
-        here = __builtin_amdgcn_ballot_w64(ok);
-        const int at = ok ? id * a.page_size + in_page : -1;
-        pos += T;
-        slot += step_slots;
-        in_page += step_rest;
-        const bool over = in_page >= a.page_size;
-        slot += over ? 1 : 0;
-        in_page -= over ? a.page_size : 0;
-        return at;
+      // One wave's work for a tile: the addresses of its tokens' rows of this KV head, from which all loads follow; absent
+      // tokens are zeros, not what the cache may hold there.
+      auto find = [&](int t) __attribute__((always_inline)) {
+        const int at = t * T + lane, page = int(__umulhi(2u * uint32_t(at), a.page_magic) >> a.page_shift);
+        const int id = s_ids[min(page - page0, kIdSlots - 1)];
+        const bool ok = lane < T && at < min(len, a1 * T) && uint32_t(id) < uint32_t(a.num_blocks32);
+        const uint64_t off = uint64_t(uint32_t(id * a.page_size + at - page * a.page_size)) * (uint32_t(a.hkv) * (2 * D)) +
+                             uint32_t(kvh) * (2 * D);
+        const uint64_t here = __builtin_amdgcn_ballot_w64(ok);
+        if (lane < T) {
+          s_from[t & 3][lane][0] = ok ? reinterpret_cast<uint64_t>(a.k_cache) + off : zero_row;
+          s_from[t & 3][lane][1] = ok ? reinterpret_cast<uint64_t>(a.v_cache) + off : zero_row;
+        }
+        if (lane == 0) s_here[t & 7] = here;
       };
-      auto issue = [&](int at, int i) __attribute__((always_inline)) {  // tile a0 + i
+      auto issue_as = [&](auto policy, int t) __attribute__((always_inline)) {  // tile t
+        constexpr bool STREAM = decltype(policy)::value;
+        const int i = t - a0;
         uint16_t* const to_k = s_k + int(unsigned(i) % kKStages) * kTileElems;
         uint16_t* const to_v = s_v + (i & (kVStages - 1)) * kTileElems;
-        uint64_t from[NLD];
-        bool ok[NLD];
+        uint64_t from[NLD][2];
 #pragma unroll
         for (int j = 0; j < NLD; ++j) {
-          const int r = __shfl(at, src_row[j], 64);
-          ok[j] = r >= 0;
-          from[j] = uint64_t(uint32_t(r)) * row_bytes + src_off[j];
+          from[j][0] = s_from[t & 3][load_row + j * kStep][0] + lane_off;
+          from[j][1] = s_from[t & 3][load_row + j * kStep][1] + lane_off;
         }
 #pragma unroll
-        for (int j = 0; j < NLD; ++j) {  // zeros for an absent token, not what the cache may hold there
-          load_lds16_at(ok[j] ? reinterpret_cast<uint64_t>(a.k_cache) + from[j] : zero_row,
-                               to_k + (wave * NLD + j) * 512);
-        }
+        for (int j = 0; j < NLD; ++j) load_lds16_as<STREAM>(from[j][0], to_k + (wave * RPL + j * kStep) * D);
 #pragma unroll
-        for (int j = 0; j < NLD; ++j) {
-          load_lds16_at(ok[j] ? reinterpret_cast<uint64_t>(a.v_cache) + from[j] : zero_row,
-                               to_v + (wave * NLD + j) * 512);
-        }
+        for (int j = 0; j < NLD; ++j) load_lds16_as<STREAM>(from[j][1], to_v + (wave * RPL + j * kStep) * D);
+      };
+      auto issue = [&](int t) __attribute__((always_inline)) {
+        if (stream) issue_as(std::true_type{}, t);
+        else issue_as(std::false_type{}, t);
       };
       // Waits until all but this wave's loads of the `more` newest tiles have landed, and for the others' too.
       auto landed = [&](int more) {
@@ -290,15 +309,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel(TreeArgs a)
           s_s[i & 1][q_ks][q_rg][q_tt + w][lane] = s[0] + s[1];
         }
       };
-      uint64_t there[3];  // of tiles t, t + 1 and t + 2
+      if (wave < 4) find(a0 + wave);
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
       for (int i = 0; i < 3; ++i) {
-        const int at = row_of(read_id());
-        there[i] = here;
-        if (a0 + i < a1) issue(at, i);
+        if (a0 + i < a1) issue(a0 + i);
       }
-      int next = row_of(read_id());
-      uint64_t next_there = here;
       landed(a1 - 1 - a0);
       read_keys(0);
       __builtin_amdgcn_sched_barrier(0);
@@ -307,12 +323,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel(TreeArgs a)
       for (int t = a0; t < a1; ++t) {
         // Here the scores of tile t, its V and the K of tile t + 1 are in LDS; the stages that tile t + 3 takes are free.
         const int i = t - a0;
-        if (t + 3 < a1) issue(next, i + 3);
-        const uint64_t mask = there[0];
-        there[0] = there[1];
-        there[1] = there[2];
-        there[2] = next_there;
-        const int next_id = read_id();
+        if (t + 3 < a1) issue(t + 3);
+        if (wave == (i & (kWaves - 1))) find(t + 4);
         f32x4 y[KS][TT];
 #pragma unroll
         for (int j = 0; j < KS; ++j) {
@@ -330,6 +342,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel(TreeArgs a)
             v[kp][dt][1] = lds_read_tr4(tile + v_at[dt] + (32 * kp + 16) * D);
           }
         }
+        const uint64_t mask = uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(s_here[t & 7]))))) |
+                              uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(s_here[t & 7] >> 32))))) << 32;
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 1; j < KS; ++j) {
@@ -404,8 +418,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel(TreeArgs a)
                                  Tag{});
           }
         }
-        next = row_of(next_id);
-        next_there = here;
         landed(t + 3 < a1 ? 1 : 0);  // tile t + 2, and every wave is done with tile t
       }
     }
@@ -421,7 +433,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel(TreeArgs a)
           *reinterpret_cast<u32x2*>(dst + 16 * dt) = u32x2{pack2(y[0], y[1], Tag{}), pack2(y[2], y[3], Tag{})};
         }
       } else {
-        const int64_t part = ((int64_t(run) * a.row_blocks + rb) * a.hkv + kvh) * 2 + (p == start ? 0 : 1);
+        const int64_t part = (int64_t(run) * a.hkv + kvh) * 2 + (p == start ? 0 : 1);
         float* dst = a.part_o + (part * RB + rg * 16 + n) * D + dg * NDT * 16 + 4 * g;
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<f32x4*>(dst + 16 * dt) = o[dt];
@@ -454,7 +466,6 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int rb_rows
     const int b = int(at / per_seq), rest = int(at - int64_t(b) * per_seq);
     const int tok = rest / a.hq, head = rest - tok * a.hq;
     const int kvh = head / a.group, r = tok * a.group + head - kvh * a.group;
-    const int rb = r / rb_rows, rr = r - rb * rb_rows;
     const uint32_t u0 = uint32_t(a.first_tile[b]), nt = uint32_t(a.first_tile[b + 1]) - u0;
     uint16_t* dst = a.out + at * D + 4 * col;
     if (nt == 0) {
@@ -465,8 +476,8 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int rb_rows
     if (i0 == i1) continue;  // written by its run
     const int parts = i1 - i0 + 1;
     // Part i0 is that run's first one (slot 0) if the sequence begins with the run, else its last (slot 1).
-    const int64_t step = int64_t(a.row_blocks) * a.hkv * 2 * rb_rows;
-    const int64_t row0 = i0 * step + (int64_t(rb) * a.hkv + kvh) * 2 * rb_rows + rr;
+    const int64_t step = int64_t(a.hkv) * 2 * rb_rows;
+    const int64_t row0 = i0 * step + int64_t(kvh) * 2 * rb_rows + r;
     const int64_t row_first = row0 + (runs.start(i0) == u0 ? 0 : rb_rows);
     auto part = [&](int i) { return i == 0 ? row_first : row0 + i * step; };
     float top = -INFINITY;
@@ -522,7 +533,7 @@ int rows_per_block(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64
 int64_t align16(int64_t x) { return (x + 15) & ~int64_t(15); }
 
 struct TreeSizes {
-  int32_t rb, row_blocks, runs;  // few rows: of this file's kernel
+  int32_t rb, runs;              // few rows: of this file's kernel
   int32_t blocks, splits;        // many rows (splits > 0): units of shaped_rows.h
   int64_t units, o_floats, ml_floats, bytes;
 };
@@ -548,12 +559,10 @@ TreeSizes tree_sizes(int32_t batch, int32_t drafts, int32_t hq, int32_t hkv, int
     return s;
   }
   s.rb = rows_per_block(rows);
-  s.row_blocks = int32_t(ceil_div(rows, s.rb));
-  const int64_t lists = int64_t(hkv) * s.row_blocks;  // workgroups of a run, one a CU: its LDS
-  const int64_t runs = device_cu_count() / lists;
+  const int64_t runs = device_cu_count() / hkv;  // a workgroup for each KV head, one a CU: its LDS
   s.runs = int32_t(runs < 1 ? 1 : runs > kMergeParts ? kMergeParts : runs);
-  s.o_floats = s.runs * lists * 2 * s.rb * head_dim;
-  s.ml_floats = s.runs * lists * 2 * s.rb * 2;
+  s.o_floats = int64_t(s.runs) * hkv * 2 * s.rb * head_dim;
+  s.ml_floats = int64_t(s.runs) * hkv * 2 * s.rb * 2;
   s.bytes = align16((s.o_floats + s.ml_floats) * 4 + (int64_t(batch) + 1) * 4);
   return s;
 }
@@ -575,7 +584,7 @@ int check_tree(const char* who, int32_t batch, int32_t drafts, int32_t hq, int32
 
 template <int D, typename Tag>
 void launch_tree(const TreeArgs& a, int rb, hipStream_t s) {
-  const dim3 grid(unsigned(a.runs) * unsigned(a.hkv) * unsigned(a.row_blocks)), block(64 * kWaves);
+  const dim3 grid(unsigned(a.runs) * unsigned(a.hkv)), block(64 * kWaves);
   if (rb == 16) hipLaunchKernelGGL((tree_decode_kernel<D, 1, Tag>), grid, block, 0, s, a);
   else if (rb == 32) hipLaunchKernelGGL((tree_decode_kernel<D, 2, Tag>), grid, block, 0, s, a);
   else hipLaunchKernelGGL((tree_decode_kernel<D, 4, Tag>), grid, block, 0, s, a);
@@ -628,9 +637,9 @@ extern "C" int ti_gqa_tree_paged(const void* q, int64_t q_stride_b, int64_t q_st
     return fail(TI_EINVAL, "%s: bad cache page_size=%d num_blocks=%lld max_blocks_per_seq=%d (at most "
                 "2^31 - 1 rows)", who, page_size, static_cast<long long>(num_blocks), max_blocks_per_seq);
   }
-  // A tile's end and a draft's position lie up to 64 behind the last token; differences of positions stay in 32 bits.
+  // Tiles ahead of the last one and a draft's position lie some hundred tokens behind it; all stays in 32 bits.
   const int64_t tokens = int64_t(max_blocks_per_seq) * page_size;
-  if (tokens > INT32_MAX - 2 * kMaxDrafts ||
+  if (tokens > INT32_MAX - 1024 ||
       int64_t(batch) * (ceil_div(tokens, 8192 / head_dim) + 1) > INT32_MAX) {
     return fail(TI_EINVAL, "%s: batch %d x max_blocks_per_seq %d x page_size %d is more than one call takes", who, batch,
                 max_blocks_per_seq, page_size);
@@ -717,10 +726,8 @@ extern "C" int ti_gqa_tree_paged(const void* q, int64_t q_stride_b, int64_t q_st
   a.hkv = num_kv_heads;
   a.group = num_q_heads / num_kv_heads;
   a.rows = num_drafts * a.group;
-  a.row_blocks = sz.row_blocks;
   a.num_blocks32 = int32_t(num_blocks);
-  a.page_size = page_size;
-  a.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(unsigned(page_size)) : -1;
+  set_page(a, page_size);
   a.max_blocks = max_blocks_per_seq;
   a.runs = sz.runs;
   a.window = near;

@@ -138,6 +138,13 @@ def gqa_tree_paged_fn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         keys. A cached value (V) that is not finite also reaches the drafts that do not see its token (a weight of
         zero times it); keys that are not seen, and what lies behind ``seqlen_kv``, reach none.
     """
+    # The call in its common form is checked and made in native code; None: another form, or one to refuse.
+    stream = None if out is not None else _lib.native(q)
+    if stream is not None and q.dim() > 0 and q.shape[-1] > 0:
+        r = _lib.result(_lib.calls().tree(q, k_cache, v_cache, block_table, seqlen_kv, tree_mask, page_size,
+                                          q.shape[-1] ** -0.5 if scale is None else scale, softcap, slopes, window, stream))
+        if r is not None:
+            return r
     if q.dim() not in (3, 4):
         raise ValueError(f"q must be [B, H_q, D] or [B, N, H_q, D], got {tuple(q.shape)}")
     q4 = q.unsqueeze(1) if q.dim() == 3 else q
@@ -203,6 +210,12 @@ def keep_drafts(cache: torch.Tensor, block_table: torch.Tensor, seqlen_kv: torch
         ``seqlen_kv < num_drafts`` (graph padding) keeps its rows and length. Blocks outside the cache are skipped. The
         drafts' blocks belong to one sequence each.
     """
+    # The call in its common form is checked and made in native code; None: another form, or one to refuse.
+    stream = _lib.native(cache)
+    if stream is not None:
+        r = _lib.result(_lib.calls().keep(cache, block_table, seqlen_kv, accepted, page_size, num_drafts, stream))
+        if r is not None:
+            return r
     if cache.dim() < 4:
         raise ValueError(f"cache must be [..., num_blocks, block_size, H_kv, D], got {tuple(cache.shape)}")
     dev = cache.device

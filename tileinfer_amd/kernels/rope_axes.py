@@ -73,6 +73,13 @@ def rope_axes_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, position
     Angles are formed in 64 bits: position 10^6 is as exact as position 10. Values past rotary_dim are only
     normalised.
     """
+    # The call in its common form is checked and made in native code; None: another form, or one to refuse.
+    stream = None if q_out is not None else _lib.native(q)
+    if stream is not None:
+        r = _lib.result(_lib.calls().rope_axes_append(q, k, v, positions, inv_freq, axes, k_cache, v_cache, slot_mapping,
+                                                      q_weight, k_weight, eps, weight_offset, stream))
+        if r is not None:
+            return r
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError("q, k, v must be [T, heads, D]")
     t, hq, d = q.shape

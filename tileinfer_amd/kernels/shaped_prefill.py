@@ -74,6 +74,14 @@ def gqa_prefill_shaped_fn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
         queries that do not see its token (a weight of zero times it), those whose rows share a workgroup with one that
         sees a token of its tile; keys that are not seen reach none.
     """
+    # The call in its common form is checked and made in native code; None: another form, or one to refuse.
+    stream = None if out is not None else _lib.native(q)
+    if stream is not None and q.dim() == 3 and q.shape[-1] > 0:
+        r = _lib.result(_lib.calls().shaped(q, k_cache, v_cache, block_table, cu_seqlens_q, seqlen_k, max_seqlen_q,
+                                            page_size, causal, q.shape[-1] ** -0.5 if scale is None else scale, softcap,
+                                            slopes, window, first_key, last_key, max_seqlen_k, stream))
+        if r is not None:
+            return r
     if q.dim() != 3:
         raise ValueError(f"q must be [total_q, H_q, D], got {tuple(q.shape)}")
     total_q, hq, d = q.shape
