@@ -591,8 +591,7 @@ int ti_rope_axes_append(const void* q, int64_t q_stride_t, int64_t q_stride_h, c
 
 /* Workspace of ti_gqa_tree_paged for these host-known sizes. */
 int ti_gqa_tree_workspace_bytes(int32_t batch, int32_t num_drafts, int32_t num_q_heads, int32_t num_kv_heads,
-                                int32_t head_dim, int32_t page_size, int32_t max_blocks_per_seq,
-                                int64_t* workspace_bytes_out);
+                                int32_t head_dim, int64_t* workspace_bytes_out);
 
 /*
  * Attention of every sequence's last num_drafts (1 .. 64) tokens, a drafted tree behind a context of

@@ -129,8 +129,7 @@ SIGNATURES = {
                                            ctypes.c_float, _c_vp, _c_i64, _c_i64, _c_vp, _c_vp, _c_i64,
                                            _c_i64, _c_vp, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,
                                            ctypes.c_float, _c_i32, _c_vp]),
-    "ti_gqa_tree_workspace_bytes": (ctypes.c_int, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,
-                                                   _I64P]),
+    "ti_gqa_tree_workspace_bytes": (ctypes.c_int, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _I64P]),
     "ti_gqa_tree_paged": (ctypes.c_int, [_c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_vp, _c_i64, _c_vp,
                                          _c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_i64, _c_i32, _c_i32,
                                          _c_i32, _c_i32, _c_i32, _c_i32, _c_i64, _c_i32, ctypes.c_float,

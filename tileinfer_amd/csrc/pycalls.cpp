@@ -734,19 +734,17 @@ PyObject* tree(PyObject* const* a) {
   {
     Unlocked unlocked;
     int64_t ws_bytes = 0;
-    rc = p_tree_ws(int32_t(p.batch), int32_t(q.tokens), int32_t(q.heads), int32_t(hkv), int32_t(q.dim), int32_t(p.page),
-                   int32_t(p.width), &ws_bytes);
+    rc = p_tree_ws(int32_t(p.batch), int32_t(q.tokens), int32_t(q.heads), int32_t(hkv), int32_t(q.dim), &ws_bytes);
     if (rc == TI_OK) {
       out = at::empty(q.q->sizes(), q.q->options());
-      at::Tensor ws;
-      if (ws_bytes > 0) ws = bytes_on(*q.q, ws_bytes);
+      at::Tensor ws = bytes_on(*q.q, ws_bytes);
       rc = p_tree(q.q->data_ptr(), q.st_b, q.st_t, q.st_h, p.cache->data_ptr(), v->data_ptr(),
                   static_cast<const int32_t*>(p.table->data_ptr()), p.table->stride(0),
                   static_cast<const int32_t*>(p.lens->data_ptr()),
                   mask ? static_cast<const int64_t*>(mask->data_ptr()) : nullptr,
                   mask && mask->dim() == 2 ? mask->stride(0) : 0,
                   slopes ? static_cast<const float*>(slopes->data_ptr()) : nullptr, out.data_ptr(),
-                  ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, int32_t(p.batch), int32_t(q.tokens),
+                  ws.data_ptr(), ws_bytes, int32_t(p.batch), int32_t(q.tokens),
                   int32_t(q.heads), int32_t(hkv), int32_t(q.dim), int32_t(p.page), p.rows / p.page, int32_t(p.width),
                   scale, cap, window, dtype_code(*q.q), stream);
     }

@@ -39,6 +39,7 @@ ShapedSizes shaped_sizes(int32_t batch, int32_t total_q, int32_t max_q, int32_t 
   if (cut > 0) {
     int64_t splits = slots / (cut == z.units ? real : cut);
     splits = splits > most ? most : splits;
+    splits = splits > kMaxParts ? kMaxParts : splits;
     const int64_t rows = cut * splits * kRows;
     if (splits > 1 && rows * head_dim <= int64_t(1) << 28) {  // many sequences of few rows: 1 GiB of parts at most
       z.whole = z.units - cut;

@@ -538,29 +538,26 @@ int rows_per_block(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64
 int64_t align16(int64_t x) { return (x + 15) & ~int64_t(15); }
 
 struct TreeSizes {
-  int32_t rb, runs;              // few rows: of this file's kernel
-  int32_t blocks, splits;        // many rows (splits > 0): units of shaped_rows.h
+  int32_t rb, runs;  // rows of a workgroup of this file's kernel, runs of either
+  int32_t blocks;    // many rows (blocks > 0): of 128 in the kernel of shaped_rows.h
   int64_t units, o_floats, ml_floats, bytes;
 };
 
 // Rows of a KV head beyond which the tree goes to the kernel of shaped_rows.h, whose workgroups take 128 rows at a time.
 constexpr int kFewRows = 64;
 
-TreeSizes tree_sizes(int32_t batch, int32_t drafts, int32_t hq, int32_t hkv, int32_t head_dim, int64_t max_k) {
+TreeSizes tree_sizes(int32_t batch, int32_t drafts, int32_t hq, int32_t hkv, int32_t head_dim) {
   TreeSizes s{};
   const int64_t rows = int64_t(drafts) * (hq / hkv);
   if (rows > kFewRows) {
     s.blocks = int32_t(ceil_div(rows, kRows));
     s.units = int64_t(batch) * s.blocks * hkv;
-    const int64_t slots = int64_t(device_cu_count()) * (head_dim == 256 ? 1 : 2);
-    const int64_t splits = ceil_div(2 * slots, s.units < 1 ? 1 : s.units), most = max_k / (4 * kKeys);
-    const int64_t n = splits > most ? most : splits;
-    s.splits = int32_t(n < 1 ? 1 : n);
-    if (s.splits > 1) {
-      s.o_floats = s.units * s.splits * kRows * head_dim;
-      s.ml_floats = s.units * s.splits * kRows * 2;
-    }
-    s.bytes = (s.o_floats + s.ml_floats) * 4;
+    const int64_t lists = int64_t(hkv) * s.blocks;  // workgroups of a run
+    const int64_t runs = device_cu_count() * (head_dim == 256 ? 1 : 2) / lists;  // of the workgroups that a GPU holds
+    s.runs = int32_t(runs < 1 ? 1 : runs > kMaxParts ? kMaxParts : runs);
+    s.o_floats = s.runs * lists * 2 * kRows * head_dim;
+    s.ml_floats = s.runs * lists * 2 * kRows * 2;
+    s.bytes = align16((s.o_floats + s.ml_floats) * 4 + (int64_t(batch) + 1) * 4);
     return s;
   }
   s.rb = rows_per_block(rows);
@@ -603,18 +600,13 @@ void launch_tree(const TreeArgs& a, int rb, hipStream_t s) {
 }  // namespace ti
 
 extern "C" int ti_gqa_tree_workspace_bytes(int32_t batch, int32_t num_drafts, int32_t num_q_heads, int32_t num_kv_heads,
-                                           int32_t head_dim, int32_t page_size, int32_t max_blocks_per_seq,
-                                           int64_t* workspace_bytes_out) {
+                                           int32_t head_dim, int64_t* workspace_bytes_out) {
   using namespace ti;
   const char* who = "ti_gqa_tree_workspace_bytes";
   const int rc = check_tree(who, batch, num_drafts, num_q_heads, num_kv_heads, head_dim);
   if (rc != TI_OK) return rc;
   if (!workspace_bytes_out) return fail(TI_EINVAL, "%s: null output", who);
-  if (page_size <= 0 || max_blocks_per_seq < 0) {
-    return fail(TI_EINVAL, "%s: bad table page_size=%d max_blocks_per_seq=%d", who, page_size, max_blocks_per_seq);
-  }
-  *workspace_bytes_out = tree_sizes(batch, num_drafts, num_q_heads, num_kv_heads, head_dim,
-                                    int64_t(max_blocks_per_seq) * page_size).bytes;
+  *workspace_bytes_out = tree_sizes(batch, num_drafts, num_q_heads, num_kv_heads, head_dim).bytes;
   return TI_OK;
 }
 
@@ -650,8 +642,12 @@ extern "C" int ti_gqa_tree_paged(const void* q, int64_t q_stride_b, int64_t q_st
                 max_blocks_per_seq, page_size);
   }
   if (batch == 0) return TI_OK;
-  const TreeSizes sz = tree_sizes(batch, num_drafts, num_q_heads, num_kv_heads, head_dim, tokens);
-  if (!q || !seqlen || !out || (sz.bytes > 0 && !workspace) || (max_blocks_per_seq > 0 && (!k_cache || !v_cache || !block_table))) {
+  const TreeSizes sz = tree_sizes(batch, num_drafts, num_q_heads, num_kv_heads, head_dim);
+  if (sz.units * (ceil_div(tokens, kKeys) + 1) > INT32_MAX) {  // the list is counted in 32 bits
+    return fail(TI_EINVAL, "%s: batch %d x %lld tokens x %d x %d heads is more than one call takes", who, batch,
+                static_cast<long long>(tokens), num_drafts, num_q_heads);
+  }
+  if (!q || !seqlen || !out || !workspace || (max_blocks_per_seq > 0 && (!k_cache || !v_cache || !block_table))) {
     return fail(TI_EINVAL, "%s: null pointer", who);
   }
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) |
@@ -666,7 +662,7 @@ extern "C" int ti_gqa_tree_paged(const void* q, int64_t q_stride_b, int64_t q_st
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool bf16 = dtype == TI_DTYPE_BF16;
   const int32_t near = window > tokens + kMaxDrafts ? 0 : window;  // none where it is wider than any distance
-  if (sz.splits > 0) {
+  if (sz.blocks > 0) {
     RowsArgs a{};
     a.q = static_cast<const uint16_t*>(q);
     a.q_sb = q_stride_b;
@@ -687,9 +683,10 @@ extern "C" int ti_gqa_tree_paged(const void* q, int64_t q_stride_b, int64_t q_st
     a.drafts = num_drafts;
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + sz.o_floats;
+    a.first_tile = reinterpret_cast<int32_t*>(a.part_ml + sz.ml_floats);
     a.units = int32_t(sz.units);
-    a.whole = sz.splits > 1 ? 0 : a.units;
-    a.splits = sz.splits;
+    a.runs = sz.runs;
+    a.batch = batch;
     a.blocks = sz.blocks;
     a.hq = num_q_heads;
     a.hkv = num_kv_heads;

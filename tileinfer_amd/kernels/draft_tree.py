@@ -100,11 +100,10 @@ def tree_masks(parents) -> torch.Tensor:
 
 
 @functools.lru_cache(maxsize=256)
-def _tree_workspace(batch: int, drafts: int, hq: int, hkv: int, d: int, page_size: int, width: int, device: int) -> int:
+def _tree_workspace(batch: int, drafts: int, hq: int, hkv: int, d: int, device: int) -> int:
     """Bytes for these sizes on this GPU (its number of CUs counts)."""
     nbytes = ctypes.c_int64(0)
-    _lib.check(_lib.load().ti_gqa_tree_workspace_bytes(batch, drafts, hq, hkv, d, page_size, width,
-                                                       ctypes.byref(nbytes)))
+    _lib.check(_lib.load().ti_gqa_tree_workspace_bytes(batch, drafts, hq, hkv, d, ctypes.byref(nbytes)))
     return nbytes.value
 
 
@@ -177,14 +176,14 @@ def gqa_tree_paged_fn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         return out
     q4 = _as_rows(q4)
     with _lib.on(dev):
-        nbytes = _tree_workspace(b, n, hq, hkv, d, page_size, block_table.shape[1], torch.cuda.current_device())
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        nbytes = _tree_workspace(b, n, hq, hkv, d, torch.cuda.current_device())
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         _lib.check(_lib.load().ti_gqa_tree_paged(
             q4.data_ptr(), q4.stride(0), q4.stride(1), q4.stride(2), k_cache.data_ptr(), v_cache.data_ptr(),
             block_table.data_ptr(), block_table.stride(0), seqlen_kv.data_ptr(),
             None if tree_mask is None else tree_mask.data_ptr(), mask_stride,
-            None if slopes is None else slopes.data_ptr(), out.data_ptr(),
-            None if ws is None else ws.data_ptr(), nbytes, b, n, hq, hkv, d,
+            None if slopes is None else slopes.data_ptr(), out.data_ptr(), ws.data_ptr(),
+            nbytes, b, n, hq, hkv, d,
             page_size, rows // page_size, block_table.shape[1], scale, softcap, window, code,
             _lib.stream_handle(dev)))
     return out
