@@ -331,12 +331,14 @@ __global__ __launch_bounds__(RowsShape<D>::THREADS, 2) void shaped_rows_kernel(R
     const float mul = SLOPES ? 1.f : CAP ? -2.f * a.shape.cap_log2 : a.shape.scale_log2;
     const float add = kInverse ? a.shape.cap_log2 : 0.f;
 
-    // Tiles in pieces whose block ids fit s_ids.
+    // From the last tile, the nearest keys, to the first: a slope's scores fall from tile to tile that way, where they would
+    // rise, and O be brought to a new maximum, with each (24 trees of 64 over up to 6,000 tokens YYY). Tiles are counted
+    // from there, in pieces whose block ids fit s_ids.
     const int piece = int(min(int64_t(1) << 24, int64_t(kIdSlots - 2) * a.page_size / kKeys));
-    for (int a0 = t0; a0 < t1; a0 += piece) {
-      const int a1 = min(t1, a0 + piece);
-      const int page0 = a0 * kKeys / a.page_size;
-      const int pages = (min(a1 * kKeys, sq.kv_len) - 1) / a.page_size - page0 + 1;
+    for (int a0 = 0; a0 < t1 - t0; a0 += piece) {
+      const int a1 = min(t1 - t0, a0 + piece);  // tiles t1 - 1 - a0 down to t1 - a1
+      const int page0 = (t1 - a1) * kKeys / a.page_size;
+      const int pages = (min((t1 - a0) * kKeys, sq.kv_len) - 1) / a.page_size - page0 + 1;
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the last piece is read
       for (int i = threadIdx.x; i < pages; i += 64 * W) s_ids[i] = a.block_table[b * a.bt_stride + page0 + i];
       __builtin_amdgcn_s_waitcnt(0);  // q has landed too: the loop below has waits of its own alone
@@ -345,9 +347,9 @@ __global__ __launch_bounds__(RowsShape<D>::THREADS, 2) void shaped_rows_kernel(R
       // One wave's work for a tile: the addresses of its 64 tokens' rows of this KV head, from which all loads follow (each
       // wave by itself took 1,000 cycles a tile for its rows); absent tokens are zeros, not what the cache may hold there.
       auto find = [&](int t) __attribute__((always_inline)) {
-        const int at = t * kKeys + lane, page = int(__umulhi(2u * uint32_t(at), a.page_magic) >> a.page_shift);
-        const int id = s_ids[min(page - page0, kIdSlots - 1)];
-        const bool ok = at < min(sq.kv_len, a1 * kKeys) && uint32_t(id) < uint32_t(a.num_blocks32);
+        const int at = max(t1 - 1 - t, 0) * kKeys + lane, page = int(__umulhi(2u * uint32_t(at), a.page_magic) >> a.page_shift);
+        const int id = s_ids[min(max(page - page0, 0), kIdSlots - 1)];
+        const bool ok = t < a1 && at < sq.kv_len && uint32_t(id) < uint32_t(a.num_blocks32);
         const uint64_t off = uint64_t(uint32_t(id * a.page_size + at - page * a.page_size)) * (uint32_t(a.hkv) * (2 * D)) +
                              uint32_t(kvh) * (2 * D);
         const uint64_t here = __builtin_amdgcn_ballot_w64(ok);
@@ -397,7 +399,7 @@ __global__ __launch_bounds__(RowsShape<D>::THREADS, 2) void shaped_rows_kernel(R
       };
       // The slopes and limits of tile t on its scores; the rows' maxima, and O brought to new ones.
       auto limit = [&](int t) __attribute__((always_inline)) {
-        const int first = t * kKeys;
+        const int first = (t1 - 1 - t) * kKeys;
         const uint64_t here = uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(s_here[t & 3]))))) |
                               uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(s_here[t & 3] >> 32))))) << 32;
         bool whole = here == ~uint64_t(0) && first >= all_lo && first + kKeys - 1 <= all_hi;  // uniform
@@ -509,7 +511,7 @@ __global__ __launch_bounds__(RowsShape<D>::THREADS, 2) void shaped_rows_kernel(R
         // the loads pass the CU's address unit at 64 bytes a cycle, and a wave stands still meanwhile.
         if (wave < LW) {
           if (t + 2 < a1) issue(0, t + 2, s_k + stage * kTile);
-          if (t + 1 < a1) issue(1, t + 1, s_v + (stage ^ 1) * kTile);
+          if (D == 256 && t + 1 < a1) issue(1, t + 1, s_v + (stage ^ 1) * kTile);
         }
         if (wave == W - 1) find(t + 3);
 
@@ -542,6 +544,7 @@ __global__ __launch_bounds__(RowsShape<D>::THREADS, 2) void shaped_rows_kernel(R
           }
           __builtin_amdgcn_sched_barrier(0);
         }
+        if (D == 128 && wave < LW && t + 1 < a1) issue(1, t + 1, s_v + (stage ^ 1) * kTile);
         // The output of tile t beside the cap of tile t + 1: V in groups of VG column tiles, read a group ahead.
         constexpr int VG = 4, GROUPS = KP * NDT / VG, EV = 4 * TT / GROUPS;
         u32x2 v[2][VG][2];
