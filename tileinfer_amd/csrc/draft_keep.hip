@@ -6,7 +6,8 @@
 // A path ascends, so a_j >= j and the moves go down: a thread owns 16 bytes of one plane's rows and takes the moves in
 // order, eight loads before their eight stores (a store of this or a later group lands at or below the group's last j,
 // which no later move reads: those have a_k >= k). Drafts that stay (a_j = j, always the path's first ones) cost
-// nothing. Bound: the launch for small batches, HBM for large ones.
+// nothing. Bound: the launch and a chain of four dependent loads (lengths and paths, block ids, rows) for small batches
+// (four sequences, 32 planes of 4 x 256 values: 5.4 us), those and HBM for large ones (64 with 32 drafts 13 us, 4 TB/s).
 #include "decode_common.h"
 
 namespace ti {

@@ -76,9 +76,9 @@ extern "C" int ti_gqa_prefill_shaped_workspace_bytes(int32_t batch, int32_t tota
   const int rc = check_shaped(who, batch, total_q, max_seqlen_q, num_q_heads, num_kv_heads, head_dim, max_seqlen_k);
   if (rc != TI_OK) return rc;
   if (!workspace_bytes_out) return fail(TI_EINVAL, "%s: null output", who);
-  *workspace_bytes_out = batch == 0 || total_q == 0 || max_seqlen_q == 0
-                             ? 0
-                             : shaped_sizes(batch, total_q, max_seqlen_q, num_q_heads, num_kv_heads, head_dim, max_seqlen_k).bytes;
+  const bool none = batch == 0 || total_q == 0 || max_seqlen_q == 0;
+  *workspace_bytes_out = none ? 0 : shaped_sizes(batch, total_q, max_seqlen_q, num_q_heads, num_kv_heads, head_dim,
+                                                 max_seqlen_k).bytes;
   return TI_OK;
 }
 

@@ -11,6 +11,14 @@
 // exponential-unit instructions, so that the softmax takes as many cycles as the products; it runs beside them, cut in
 // two: while the matrix unit computes the scores of tile t + 1, the vector unit turns those of tile t into weights, and
 // beside the output of tile t it caps the scores of tile t + 1. One barrier a tile; K is two tiles ahead, V one.
+//
+// Bound, at D = 256: LDS (each wave reads all of K and V for its 16 rows: 512 KB a tile at some 215 bytes a cycle, and the
+// loads write 64 KB) and the loads' way through the CU's address unit (1,400 cycles of a loading wave's 4,600 a tile), the
+// matrix unit being busy 44 % of the time: 2,048 queries over 10,240 keys within a window of 4,096 with 24/4 heads 238 us
+// (866 TFLOP/s), capped 255 to 270; a first chunk of 2,048 82, capped 85 to 93. Waves of 32 rows (half the reads) do not fit
+// 256 registers with the softmax beside the products; with 512 (four waves a CU) the compiler moved them between register
+// files (379 us against 274 then), without the overlap 279. At D = 128: the vector unit (capped 176 us, 146 without, 940
+// TFLOP/s for the same chunk with 32/8 heads) and unit starts: 12 chunks of packed documents with 32/8 heads 83 to 87 us.
 #pragma once
 
 #include "lds_tiles.h"
@@ -52,7 +60,7 @@ struct RowsArgs {
   // block of rows, side by side: the heads' rows of a token lie side by side in memory, and the blocks (on one XCD) read
   // the same ones. A sequence that lies in one run is written by it, the parts of others [run][block][KV head][first or
   // last one] are joined by a second kernel in the order of the runs. (One list of all heads' and blocks' tiles, 24 trees
-  // of 64 over up to 6,000 tokens with 32/8 heads: 258 us; of all heads', the blocks side by side: 237; so XXX.)
+  // of 64 over up to 6,000 tokens with 32/8 heads: 258 us; of all heads', the blocks side by side: 237; so 197.)
   float* part_o;   // [..][128][D] unnormalised rows
   float* part_ml;  // [..][128][2] their (m, l), m in exp2 units
   int32_t* first_tile;  // TREE: [B + 1] each sequence's first tile of one unit, and the total
@@ -95,7 +103,9 @@ __device__ __forceinline__ int tree_tiles(const RowsArgs& a, int b) {
   return (s.kv_len + kKeys - 1) / kKeys - tree_tile0(a, s);
 }
 constexpr uint32_t kMinRun = 2;  // tiles
-__device__ __forceinline__ Runs tree_runs(const RowsArgs& a, uint32_t total) { return Runs(uint32_t(a.runs), total, kMinRun); }
+__device__ __forceinline__ Runs tree_runs(const RowsArgs& a, uint32_t total) {
+  return Runs(uint32_t(a.runs), total, kMinRun);
+}
 
 __device__ __forceinline__ void load_lds16_at(uint64_t src, const uint16_t* lds) {
   const uint32_t m0 = uint32_t(reinterpret_cast<uintptr_t>((lds_ptr_t)(lds)));
@@ -305,8 +315,8 @@ __global__ __launch_bounds__(RowsShape<D>::THREADS, 2) void shaped_rows_kernel(R
     const int k_at = n * D + 8 * (g ^ swz16(n));
     const int v_row = 4 * g + (n >> 2);
     const int v_at = v_row * D + 8 * (((lane >> 1) & 1) ^ swz16(v_row)) + 4 * (lane & 1);
-    // Load j of a wave takes the tile's rows kStep j + load_row: a lane's chunk is the same in rows 16 apart, in rows 8 apart
-    // 9 places on.
+    // Load j of a wave takes the tile's rows kStep j + load_row: a lane's chunk is the same in rows 16 apart, in rows 8
+    // apart 9 places on.
     constexpr int kStep = LW * RPL;
     static_assert(kStep == 16 || kStep == 8);
     const int load_row = (wave & (LW - 1)) * RPL + lane / CH;
@@ -332,8 +342,8 @@ __global__ __launch_bounds__(RowsShape<D>::THREADS, 2) void shaped_rows_kernel(R
     const float add = kInverse ? a.shape.cap_log2 : 0.f;
 
     // From the last tile, the nearest keys, to the first: a slope's scores fall from tile to tile that way, where they would
-    // rise, and O be brought to a new maximum, with each (24 trees of 64 over up to 6,000 tokens YYY). Tiles are counted
-    // from there, in pieces whose block ids fit s_ids.
+    // rise, and O be brought to a new maximum, with each (24 trees of 64 over up to 6,000 tokens 199 us against 192). Tiles
+    // are counted from there, in pieces whose block ids fit s_ids.
     const int piece = int(min(int64_t(1) << 24, int64_t(kIdSlots - 2) * a.page_size / kKeys));
     for (int a0 = 0; a0 < t1 - t0; a0 += piece) {
       const int a1 = min(t1 - t0, a0 + piece);  // tiles t1 - 1 - a0 down to t1 - a1
@@ -347,7 +357,8 @@ __global__ __launch_bounds__(RowsShape<D>::THREADS, 2) void shaped_rows_kernel(R
       // One wave's work for a tile: the addresses of its 64 tokens' rows of this KV head, from which all loads follow (each
       // wave by itself took 1,000 cycles a tile for its rows); absent tokens are zeros, not what the cache may hold there.
       auto find = [&](int t) __attribute__((always_inline)) {
-        const int at = max(t1 - 1 - t, 0) * kKeys + lane, page = int(__umulhi(2u * uint32_t(at), a.page_magic) >> a.page_shift);
+        const int at = max(t1 - 1 - t, 0) * kKeys + lane;
+        const int page = int(__umulhi(2u * uint32_t(at), a.page_magic) >> a.page_shift);
         const int id = s_ids[min(max(page - page0, 0), kIdSlots - 1)];
         const bool ok = t < a1 && at < sq.kv_len && uint32_t(id) < uint32_t(a.num_blocks32);
         const uint64_t off = uint64_t(uint32_t(id * a.page_size + at - page * a.page_size)) * (uint32_t(a.hkv) * (2 * D)) +
@@ -507,8 +518,8 @@ __global__ __launch_bounds__(RowsShape<D>::THREADS, 2) void shaped_rows_kernel(R
         // Here K of tile t + 1 and V of tile t are in LDS, s holds the scores of tile t; every wave is done with K of tile
         // t and V of tile t - 1.
         const int stage = t & 1;
-        // The oldest wave of each SIMD, which the SIMD serves first and which would wait for the others at the barrier, loads:
-        // the loads pass the CU's address unit at 64 bytes a cycle, and a wave stands still meanwhile.
+        // The oldest wave of each SIMD, which the SIMD serves first and which would wait for the others at the barrier,
+        // loads: the loads pass the CU's address unit at 64 bytes a cycle, and a wave stands still meanwhile.
         if (wave < LW) {
           if (t + 2 < a1) issue(0, t + 2, s_k + stage * kTile);
           if (D == 256 && t + 1 < a1) issue(1, t + 1, s_v + (stage ^ 1) * kTile);
@@ -600,7 +611,8 @@ __global__ __launch_bounds__(RowsShape<D>::THREADS, 2) void shaped_rows_kernel(R
           *reinterpret_cast<u32x2*>(dst + 16 * dt) = u32x2{pack2(y[0], y[1], Tag{}), pack2(y[2], y[3], Tag{})};
         }
       } else {
-        const int64_t slot = TREE ? ((int64_t(run) * a.blocks + qb) * a.hkv + kvh) * 2 + (p == start ? 0 : 1) : int64_t(cut) * splits + split;
+        const int64_t slot = TREE ? ((int64_t(run) * a.blocks + qb) * a.hkv + kvh) * 2 + (p == start ? 0 : 1)
+                                  : int64_t(cut) * splits + split;
         const int64_t part = slot * kRows + r - qb * kRows;
         float* dst = a.part_o + part * D + 4 * g;
 #pragma unroll
@@ -690,7 +702,8 @@ void set_page(Args& a, int32_t page_size) {
 
 template <int D, bool TREE, typename Tag>
 void launch_rows(const RowsArgs& a, hipStream_t s) {
-  const dim3 grid(unsigned(TREE ? a.runs * a.blocks * a.hkv : a.whole + (a.units - a.whole) * a.splits)), block(RowsShape<D>::THREADS);
+  const dim3 block(RowsShape<D>::THREADS);
+  const dim3 grid(unsigned(TREE ? a.runs * a.blocks * a.hkv : a.whole + (a.units - a.whole) * a.splits));
   const bool cap = a.shape.cap_log2 > 0.f, slopes = a.slopes != nullptr;
   if (cap && slopes) hipLaunchKernelGGL((shaped_rows_kernel<D, true, true, TREE, Tag>), grid, block, 0, s, a);
   else if (cap) hipLaunchKernelGGL((shaped_rows_kernel<D, true, false, TREE, Tag>), grid, block, 0, s, a);
