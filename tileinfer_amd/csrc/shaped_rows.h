@@ -243,34 +243,66 @@ __global__ __launch_bounds__(RowsShape<D>::THREADS, 2) void shaped_rows_kernel(R
     }
     // This lane's rows and the keys they see, which stay in LDS: only tiles that a limit or a slope touches need them.
     const int row0 = qb * kRows + wave * 16 * C + n;
-    u32x4 q[C][KK];
-    int some_lo = INT32_MAX, some_hi = -1, all_lo = 0, all_hi = INT32_MAX;
+    // Everything that the limits come from is loaded first, at once, and Q behind it: loads land in order, and one after the
+    // other (each row's queries, then its limits) they took 4 of a short unit's 18 us.
+    int tok[C], head[C], first_of[C], last_of[C];
+    uint64_t mask_of[C];
+    float slope[C];
 #pragma unroll
     for (int rt = 0; rt < C; ++rt) {
       const int r = min(row0 + 16 * rt, rows - 1);  // rows behind the last repeat it, not stored
-      const int tok = r / a.group, head = kvh * a.group + r - tok * a.group;
-      const uint16_t* src = a.q + (TREE ? b * a.q_sb : sq.q0 * a.q_st) + tok * a.q_st + head * a.q_sh + 8 * g;
+      tok[rt] = r / a.group;
+      head[rt] = kvh * a.group + r - tok[rt] * a.group;
+    }
+    if (SLOPES) {
+#pragma unroll
+      for (int rt = 0; rt < C; ++rt) slope[rt] = a.slopes[head[rt]];
+    }
+    if constexpr (TREE) {
+#pragma unroll
+      for (int rt = 0; rt < C; ++rt) mask_of[rt] = drafts_seen(a, b, tok[rt]);
+    } else {
+      if (a.first_key) {
+#pragma unroll
+        for (int rt = 0; rt < C; ++rt) first_of[rt] = a.first_key[sq.q0 + tok[rt]];
+      }
+      if (a.last_key) {
+#pragma unroll
+        for (int rt = 0; rt < C; ++rt) last_of[rt] = a.last_key[sq.q0 + tok[rt]];
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    u32x4 q[C][KK];
+#pragma unroll
+    for (int rt = 0; rt < C; ++rt) {
+      const uint16_t* src = a.q + (TREE ? b * a.q_sb : sq.q0 * a.q_st) + tok[rt] * a.q_st + head[rt] * a.q_sh + 8 * g;
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) q[rt][kk] = load16(src + 32 * kk);
-      int pos = sq.offset + tok, lo = 0, hi;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    int some_lo = INT32_MAX, some_hi = -1, all_lo = 0, all_hi = INT32_MAX;
+#pragma unroll
+    for (int rt = 0; rt < C; ++rt) {
+      int pos = sq.offset + tok[rt], lo = 0, hi;
       if constexpr (TREE) {
-        uint64_t seen = drafts_seen(a, b, tok);
-        const int depth = __builtin_popcountll(seen & ~(uint64_t(1) << tok));
+        uint64_t seen = mask_of[rt];
+        const int depth = __builtin_popcountll(seen & ~(uint64_t(1) << tok[rt]));
         pos = sq.offset + depth;
         hi = sq.offset - 1;  // of the context; the drafts by their bits
         if (a.window > 0) seen = drafts_near(seen, s_depth, a.drafts, depth, a.window);
         if (g == 0) s_seen[wave * 16 * C + rt * 16 + n] = seen;
       } else {
-        if (a.first_key) lo = max(a.first_key[sq.q0 + tok], 0);
-        hi = min(a.last_key ? a.last_key[sq.q0 + tok] : a.causal ? pos : sq.kv_len - 1, sq.kv_len - 1);
+        if (a.first_key) lo = max(first_of[rt], 0);
+        hi = min(a.last_key ? last_of[rt] : a.causal ? pos : sq.kv_len - 1, sq.kv_len - 1);
       }
       if (a.window > 0 && pos >= a.window) lo = max(lo, pos - a.window + 1);
       if (!TREE && lo > hi) {  // sees nothing
         lo = INT32_MAX;
         hi = -1;
       }
-      const float slope = SLOPES ? a.slopes[head] * kLog2e : 0.f;
-      if (g == 0) s_row[wave * 16 * C + rt * 16 + n] = make_int4(lo, hi, pos, __float_as_int(slope));
+      if (g == 0) {
+        s_row[wave * 16 * C + rt * 16 + n] = make_int4(lo, hi, pos, SLOPES ? __float_as_int(slope[rt] * kLog2e) : 0);
+      }
       some_lo = min(some_lo, lo);
       some_hi = max(some_hi, hi);
       all_lo = max(all_lo, lo);
