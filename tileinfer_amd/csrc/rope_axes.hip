@@ -11,8 +11,11 @@
 // passes over the rows of one token (its q, k and v heads), all loaded at once. Lane i computes the angle of frequency
 // i once a wave, the lanes of a row read theirs back from LDS: a sine for every value instead would cost more time
 // than the row's bytes. Bound: HBM and the vector work of the norms for long chunks (8,191 tokens with 24/4 heads of 256
-// and norms 58 us, 4.6 TB/s; without norms 51, 5.3 TB/s), the launch for short ones (48 tokens 7.2 us). Loads with the nt
-// bit made no difference (57 against 58, 14.7 against 14.7 for 2,080 tokens of 32/8 heads of 128).
+// and norms 56.6 us, 4.7 TB/s; without norms 51, 5.3 TB/s), the launch for short ones (48 tokens 7.2 us). The norms' sums by
+// DPP and partners exchanged as 16-bit pairs, where both had been shuffles of 32-bit values: 57.8 to 56.6 us, 46.6 to 44.7
+// for 32/8 heads of 128. Loads with the nt bit made no difference.
+#include <type_traits>
+
 #include "decode_common.h"
 
 namespace ti {
@@ -44,6 +47,23 @@ struct RopeAxesArgs {
   float eps, offset;
 };
 
+// Sum over the 16 (LPR 16) or 32 lanes of a row, in all of them.
+template <int LPR>
+__device__ __forceinline__ float row_sum(float x) {
+  auto turned = [](float v, auto by) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + decltype(by)::value, 0xf, 0xf, false));
+  };
+  x += turned(x, std::integral_constant<int, 8>{});  // row_ror
+  x += turned(x, std::integral_constant<int, 4>{});
+  x += turned(x, std::integral_constant<int, 2>{});
+  x += turned(x, std::integral_constant<int, 1>{});
+  if constexpr (LPR == 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  return x;
+}
+
 template <int D, int P, typename Tag>
 __global__ __launch_bounds__(256) void rope_axes_kernel(RopeAxesArgs a) {
   constexpr int LPR = D / 8;
@@ -71,15 +91,20 @@ __global__ __launch_bounds__(256) void rope_axes_kernel(RopeAxesArgs a) {
     else src = a.v + t * a.v_st + (r - a.hq - a.hkv) * a.v_sh;
     x[i] = load16(src + 8 * l);
   }
-  u32x4 wq = {}, wk = {};
+  const int half = a.rotary / 2;
+  const bool low = 8 * l < half, turned = 8 * l < a.rotary;
+  // The lane that holds a lane's partners; its own where it turns nothing.
+  const int partner = turned ? (lane & ~(LPR - 1)) | (low ? l + half / 8 : l - half / 8) : lane;
+  u32x4 wq = {}, wk = {}, pq = {}, pk = {};  // this lane's weights and its partners'
   if (a.q_w) {
     wq = load16(a.q_w + 8 * l);
     wk = load16(a.k_w + 8 * l);
+    pq = load16(a.q_w + 8 * (partner & (LPR - 1)));
+    pk = load16(a.k_w + 8 * (partner & (LPR - 1)));
   }
   const int64_t slot = a.slots[t];
   const bool stored = slot >= 0 && slot < a.num_slots;
 
-  const int half = a.rotary / 2;
   if (lane < half) {
     const int axis = a.axis_of ? min(max(a.axis_of[lane], 0), a.axes - 1) : 0;
     const int64_t at = axis * a.pos_sa + t;
@@ -94,7 +119,6 @@ __global__ __launch_bounds__(256) void rope_axes_kernel(RopeAxesArgs a) {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  const bool low = 8 * l < half, turned = 8 * l < a.rotary;
   const int at = turned ? (low ? 8 * l : 8 * l - half) : 0;
   f32x4 c[2], s[2];
 #pragma unroll
@@ -107,7 +131,6 @@ __global__ __launch_bounds__(256) void rope_axes_kernel(RopeAxesArgs a) {
       s[j] = f32x4{};
     }
   }
-  const int partner = (lane & ~(LPR - 1)) | ((low ? l + half / 8 : l - half / 8) & (LPR - 1));
 
 #pragma unroll
   for (int i = 0; i < P; ++i) {
@@ -119,13 +142,12 @@ __global__ __launch_bounds__(256) void rope_axes_kernel(RopeAxesArgs a) {
       y[2 * j] = p.x;
       y[2 * j + 1] = p.y;
     }
+    float r = 1.f;
     if (a.q_w) {  // uniform
       float ss = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss = fmaf(y[j], y[j], ss);
-#pragma unroll
-      for (int d = LPR / 2; d > 0; d >>= 1) ss += __shfl_xor(ss, d, 64);
-      const float r = rsqrtf(ss / float(D) + a.eps);
+      r = rsqrtf(row_sum<LPR>(ss) / float(D) + a.eps);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float2 w = unpack2(is_q ? wq[j] : wk[j], Tag{});
@@ -133,16 +155,20 @@ __global__ __launch_bounds__(256) void rope_axes_kernel(RopeAxesArgs a) {
         y[2 * j + 1] *= r * (a.offset + w.y);
       }
     }
+    // The rotation's partners come as 16-bit pairs, and are normalised here again: half the exchange.
     u32x4 res;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      float other[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) other[e] = half > 0 ? __shfl(y[2 * j + e], partner, 64) : 0.f;
+      float2 other = unpack2(uint32_t(__shfl(int(x[i][j]), partner, 64)), Tag{});
+      if (a.q_w) {
+        const float2 w = unpack2(is_q ? pq[j] : pk[j], Tag{});
+        other.x *= r * (a.offset + w.x);
+        other.y *= r * (a.offset + w.y);
+      }
       // Past the rotation the value itself: a partner that is not finite stays out of it.
-      const float u = turned ? other[0] * s[j >> 1][2 * j & 3] : -0.f;
-      const float w = turned ? other[1] * s[j >> 1][(2 * j & 3) + 1] : -0.f;
-      res[j] = pack_fma2(y[2 * j], c[j >> 1][2 * j & 3], u, y[2 * j + 1], c[j >> 1][(2 * j & 3) + 1], w, Tag{});
+      const float u = turned ? other.x * s[j >> 1][2 * j & 3] : -0.f;
+      const float v = turned ? other.y * s[j >> 1][(2 * j & 3) + 1] : -0.f;
+      res[j] = pack_fma2(y[2 * j], c[j >> 1][2 * j & 3], u, y[2 * j + 1], c[j >> 1][(2 * j & 3) + 1], v, Tag{});
     }
     if (row[i] >= rows) continue;
     uint16_t* dst;
