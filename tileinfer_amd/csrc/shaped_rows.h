@@ -18,7 +18,7 @@
 // (866 TFLOP/s), capped 255 to 270; a first chunk of 2,048 82, capped 85 to 93. Waves of 32 rows (half the reads) do not fit
 // 256 registers with the softmax beside the products; with 512 (four waves a CU) the compiler moved them between register
 // files (379 us against 274 then), without the overlap 279. At D = 128: the vector unit (capped 176 us, 146 without, 940
-// TFLOP/s for the same chunk with 32/8 heads) and unit starts: 12 chunks of packed documents with 32/8 heads 83 to 87 us.
+// TFLOP/s for the same chunk with 32/8 heads) and unit starts: 12 chunks of packed documents with 32/8 heads 78 to 84 us.
 #pragma once
 
 #include "lds_tiles.h"
