@@ -627,6 +627,8 @@ int ti_gqa_tree_paged(const void* q, int64_t q_stride_b, int64_t q_stride_t, int
  * whose block is outside [0, num_blocks) are not moved.
  *   cache     planes contiguous arrays of num_blocks * page_size rows of row_elems (a multiple of 8) 16-bit elements
  *   accepted  [batch, accepted_width] at accepted_stride; num_drafts 1 .. 64
+ *   new_seqlen  [batch], apart from the other operands, which workgroups read while it is stored (an overlap with
+ *               seqlen is refused)
  * No reference counterpart.
  */
 int ti_keep_drafts(void* cache, const int32_t* block_table, int64_t block_table_stride,

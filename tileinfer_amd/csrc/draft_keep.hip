@@ -107,6 +107,11 @@ extern "C" int ti_keep_drafts(void* cache, const int32_t* block_table, int64_t b
     return fail(TI_EINVAL, "%s: null pointer", who);
   }
   if (reinterpret_cast<uintptr_t>(cache) & 15) return fail(TI_EINVAL, "%s: cache must be 16-byte aligned", who);
+  // A sequence's workgroups read its length while the first of them stores the new one.
+  const uintptr_t old_at = reinterpret_cast<uintptr_t>(seqlen), new_at = reinterpret_cast<uintptr_t>(new_seqlen);
+  if (old_at < new_at + 4 * uintptr_t(batch) && new_at < old_at + 4 * uintptr_t(batch)) {
+    return fail(TI_EINVAL, "%s: new_seqlen and seqlen overlap", who);
+  }
   KeepArgs a{};
   a.cache = static_cast<uint16_t*>(cache);
   a.plane = num_blocks * page_size * row_elems;
