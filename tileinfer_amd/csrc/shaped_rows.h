@@ -145,8 +145,8 @@ struct RowsShape {
   static constexpr int THREADS = 64 * W;
 };
 
-// CAP: the scores are capped. SLOPES: they are biased.
-template <int D, bool CAP, bool SLOPES, bool TREE, typename Tag>
+// CAP: how the scores are capped. SLOPES: they are biased (kWideCap: they may be).
+template <int D, int CAP, bool SLOPES, bool TREE, typename Tag>
 __global__ __launch_bounds__(RowsShape<D>::THREADS, 2) void shaped_rows_kernel(RowsArgs a) {
   constexpr int C = RowsShape<D>::C, W = RowsShape<D>::W;
   constexpr int TT = kKeys / 16, KP = kKeys / 32;
@@ -256,7 +256,7 @@ __global__ __launch_bounds__(RowsShape<D>::THREADS, 2) void shaped_rows_kernel(R
     }
     if (SLOPES) {
 #pragma unroll
-      for (int rt = 0; rt < C; ++rt) slope[rt] = a.slopes[head[rt]];
+      for (int rt = 0; rt < C; ++rt) slope[rt] = CAP == kWideCap && !a.slopes ? 0.f : a.slopes[head[rt]];
     }
     if constexpr (TREE) {
 #pragma unroll
@@ -433,7 +433,9 @@ __global__ __launch_bounds__(RowsShape<D>::THREADS, 2) void shaped_rows_kernel(R
       };
       // A dot product as the score that is kept (without its slope).
       auto shape_of = [&](float dot) __attribute__((always_inline)) {
-        if constexpr (CAP) {
+        if constexpr (CAP == kWideCap) {
+          return capped_wide(dot, a.shape);
+        } else if constexpr (CAP) {
           const float r = __builtin_amdgcn_rcpf(1.f + fast_exp2(dot * a.shape.cap_in));
           return kInverse ? r : fmaf(-2.f * a.shape.cap_log2, r, a.shape.cap_log2);
         } else {
@@ -736,11 +738,13 @@ template <int D, bool TREE, typename Tag>
 void launch_rows(const RowsArgs& a, hipStream_t s) {
   const dim3 block(RowsShape<D>::THREADS);
   const dim3 grid(unsigned(TREE ? a.runs * a.blocks * a.hkv : a.whole + (a.units - a.whole) * a.splits));
-  const bool cap = a.shape.cap_log2 > 0.f, slopes = a.slopes != nullptr;
-  if (cap && slopes) hipLaunchKernelGGL((shaped_rows_kernel<D, true, true, TREE, Tag>), grid, block, 0, s, a);
-  else if (cap) hipLaunchKernelGGL((shaped_rows_kernel<D, true, false, TREE, Tag>), grid, block, 0, s, a);
-  else if (slopes) hipLaunchKernelGGL((shaped_rows_kernel<D, false, true, TREE, Tag>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((shaped_rows_kernel<D, false, false, TREE, Tag>), grid, block, 0, s, a);
+  const int cap = cap_of(a.shape);
+  const bool slopes = a.slopes != nullptr;
+  if (cap == kWideCap) hipLaunchKernelGGL((shaped_rows_kernel<D, kWideCap, true, TREE, Tag>), grid, block, 0, s, a);
+  else if (cap && slopes) hipLaunchKernelGGL((shaped_rows_kernel<D, kCap, true, TREE, Tag>), grid, block, 0, s, a);
+  else if (cap) hipLaunchKernelGGL((shaped_rows_kernel<D, kCap, false, TREE, Tag>), grid, block, 0, s, a);
+  else if (slopes) hipLaunchKernelGGL((shaped_rows_kernel<D, kNoCap, true, TREE, Tag>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((shaped_rows_kernel<D, kNoCap, false, TREE, Tag>), grid, block, 0, s, a);
   const int joined = TREE ? a.units : a.splits > 1 ? a.units - a.whole : 0;
   if (joined > 0) {
     hipLaunchKernelGGL((shaped_merge_kernel<D, TREE, Tag>), dim3(unsigned(joined) * (kRows / 16)), dim3(256), 0, s, a);

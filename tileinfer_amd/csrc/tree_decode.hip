@@ -96,7 +96,7 @@ struct TreeTile {
 
 // RG: row groups of 16. CAP: the scores are capped, by the waves that compute them, each its own once (beside the output
 // every wave of a row group would cap all of them: 32 x 16,384 tokens with 32/8 heads of 128 405 us against 333).
-template <int D, int RG, bool CAP, typename Tag>
+template <int D, int RG, int CAP, typename Tag>
 __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel(TreeArgs a) {
   constexpr int T = TreeTile<D>::T, TT = T / 16, KP = T / 32;
   constexpr int KS = CAP || TT * RG >= kWaves ? 1 : kWaves / (TT * RG);  // parts of k in the first product
@@ -316,7 +316,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel(TreeArgs a)
           s[0] += s[1];
           if constexpr (CAP) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[0][e] = capped(s[0][e], a.shape);
+            for (int e = 0; e < 4; ++e) s[0][e] = CAP == kWideCap ? capped_wide(s[0][e], a.shape) : capped(s[0][e], a.shape);
           }
           s_s[i & 1][q_ks][q_rg][q_tt + w][lane] = s[0];
         }
@@ -590,7 +590,7 @@ int check_tree(const char* who, int32_t batch, int32_t drafts, int32_t hq, int32
   return TI_OK;
 }
 
-template <int D, bool CAP, typename Tag>
+template <int D, int CAP, typename Tag>
 void launch_tree(const TreeArgs& a, int rb, hipStream_t s) {
   const dim3 grid(unsigned(a.runs) * unsigned(a.hkv)), block(64 * kWaves);
   if (rb == 16) hipLaunchKernelGGL((tree_decode_kernel<D, 1, CAP, Tag>), grid, block, 0, s, a);
@@ -740,15 +740,17 @@ extern "C" int ti_gqa_tree_paged(const void* q, int64_t q_stride_b, int64_t q_st
   a.runs = sz.runs;
   a.window = near;
   a.shape = score_shape(scale, softcap);
-  const bool cap = a.shape.cap_log2 > 0.f;
+  const int cap = cap_of(a.shape);
   auto launch = [&](auto tag) {
     using Tag = decltype(tag);
     if (head_dim == 256) {
-      if (cap) launch_tree<256, true, Tag>(a, sz.rb, s);
-      else launch_tree<256, false, Tag>(a, sz.rb, s);
+      if (cap == kWideCap) launch_tree<256, kWideCap, Tag>(a, sz.rb, s);
+      else if (cap == kCap) launch_tree<256, kCap, Tag>(a, sz.rb, s);
+      else launch_tree<256, kNoCap, Tag>(a, sz.rb, s);
     } else {
-      if (cap) launch_tree<128, true, Tag>(a, sz.rb, s);
-      else launch_tree<128, false, Tag>(a, sz.rb, s);
+      if (cap == kWideCap) launch_tree<128, kWideCap, Tag>(a, sz.rb, s);
+      else if (cap == kCap) launch_tree<128, kCap, Tag>(a, sz.rb, s);
+      else launch_tree<128, kNoCap, Tag>(a, sz.rb, s);
     }
   };
   if (bf16) launch(Bf16{});
