@@ -15,14 +15,14 @@ bool vec_rows(const void* p, int64_t st, int64_t sh) {
 }
 
 struct ShapedSizes {
-  int32_t blocks, splits;
+  int32_t blocks, splits, slots;
   int64_t units, whole, o_floats, ml_floats, bytes;
 };
 
 // How units are cut. A CU holds one workgroup at D = 256, two at 128 (slots). Where the units do not fill the slots, all
 // are cut into as many parts as fill them; where they fill them some times over and the units of a chunk are alike
 // (one sequence, at least as much context as chunk), those of the last, partial round are. Parts have at least four
-// tiles.
+// tiles, and only units that exist have them: at most as many as fill the slots, 34 MB.
 ShapedSizes shaped_sizes(int32_t batch, int32_t total_q, int32_t max_q, int32_t hq, int32_t hkv, int32_t head_dim,
                          int64_t max_k) {
   ShapedSizes z{};
@@ -40,10 +40,12 @@ ShapedSizes shaped_sizes(int32_t batch, int32_t total_q, int32_t max_q, int32_t 
     int64_t splits = slots / (cut == z.units ? real : cut);
     splits = splits > most ? most : splits;
     splits = splits > kMaxParts ? kMaxParts : splits;
-    const int64_t rows = cut * splits * kRows;
-    if (splits > 1 && rows * head_dim <= int64_t(1) << 28) {  // many sequences of few rows: 1 GiB of parts at most
+    // A padded batch's workgroups: 16,384 of head_dim 128, 8,192 of 256, most of which have no rows to take.
+    if (splits > 1 && cut * splits * kRows * head_dim <= int64_t(1) << 28) {
       z.whole = z.units - cut;
       z.splits = int32_t(splits);
+      z.slots = int32_t(cut == z.units && real < cut ? real : cut);
+      const int64_t rows = z.slots * splits * kRows;
       z.o_floats = rows * head_dim;
       z.ml_floats = rows * 2;
       z.bytes = (z.o_floats + z.ml_floats) * 4;
@@ -157,6 +159,7 @@ extern "C" int ti_gqa_prefill_shaped(const void* q, int64_t q_stride_t, int64_t 
   a.group = num_q_heads / num_kv_heads;
   a.blocks = z.blocks;
   a.splits = z.splits;
+  a.slots = z.slots;
   a.num_blocks32 = int32_t(num_blocks);
   set_page(a, page_size);
   a.max_blocks = max_blocks_per_seq;

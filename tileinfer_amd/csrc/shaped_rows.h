@@ -55,7 +55,8 @@ struct RowsArgs {
   int64_t mask_sb;
   int32_t drafts;
   // Prefill: units in the order of (sequence, block from the last one, KV head). The first `whole` of them are a workgroup's
-  // each, the keys of the others are cut into `splits` parts, of which a second kernel joins [unit - whole][splits].
+  // each, the keys of the others are cut into `splits` parts, of which a second kernel joins [part_slot][splits]. There are
+  // `slots` of them: units that exist, where `units` counts the longest chunk's for every sequence.
   // TREE: the sequences' tiles are one list, cut into `runs` of equal length, each taken by a workgroup for each KV head and
   // block of rows, side by side: the heads' rows of a token lie side by side in memory, and the blocks (on one XCD) read
   // the same ones. A sequence that lies in one run is written by it, the parts of others [run][block][KV head][first or
@@ -64,7 +65,7 @@ struct RowsArgs {
   float* part_o;   // [..][128][D] unnormalised rows
   float* part_ml;  // [..][128][2] their (m, l), m in exp2 units
   int32_t* first_tile;  // TREE: [B + 1] each sequence's first tile of one unit, and the total
-  int32_t units, whole, splits, blocks, runs, batch;
+  int32_t units, whole, splits, slots, blocks, runs, batch;
   int32_t hq, hkv, group, num_blocks32, page_size, max_blocks, window;  // window 0: none
   // at / page_size = mulhi(2 at, page_magic) >> page_shift for at below 2^31: page_shift = ceil(log2 page_size),
   // page_magic = ceil(2^(31 + page_shift) / page_size)
@@ -92,6 +93,21 @@ struct Queries {
     offset = kv_len - q_len;  // query i's row sits at position offset + i; TREE: the context's length
   }
 };
+
+// Prefill: the place of a cut unit's parts. In one sequence its place behind the whole ones; of several, all cut, its place
+// among the units that exist, by a wave's sum over the sequences before. Offsets that go back may have more units than
+// the rows say, and than there are slots: those behind the last one are not cut.
+__device__ __forceinline__ int part_slot(const RowsArgs& a, int b, int qb, int kvh) {
+  if (a.batch == 1) return (a.blocks - 1 - qb) * a.hkv + kvh - a.whole;
+  int before = 0;
+  for (int b0 = 0; b0 < b; b0 += 64) {
+    const int other = b0 + int(threadIdx.x & 63);
+    const Queries<false> s(a, min(other, b));
+    const int n = other < b ? min((s.q_len * a.group + kRows - 1) / kRows, a.blocks) : 0;
+    before += __builtin_amdgcn_readlane(wave_prefix_sum(n), 63);
+  }
+  return (before + qb) * a.hkv + kvh;
+}
 
 // TREE: the tiles of a unit, from the first that any of its rows may see.
 __device__ __forceinline__ int tree_tile0(const RowsArgs& a, const Queries<true>& s) {
@@ -207,8 +223,7 @@ __global__ __launch_bounds__(RowsShape<D>::THREADS, 2) void shaped_rows_kernel(R
     if (unit >= a.whole) {
       const int rest = a.units - a.whole, i = unit - a.whole;
       split = i / rest;
-      cut = i - split * rest;
-      unit = a.whole + cut;
+      unit = a.whole + i - split * rest;
       splits = a.splits;
     }
     const int per_seq = a.blocks * a.hkv;
@@ -231,8 +246,15 @@ __global__ __launch_bounds__(RowsShape<D>::THREADS, 2) void shaped_rows_kernel(R
         continue;
       }
       t_rel = int(rel);
-    } else if (qb * kRows >= rows) {
-      return;
+    } else {
+      if (qb * kRows >= rows) return;
+      if (splits > 1) {
+        cut = part_slot(a, b, qb, kvh);
+        if (cut >= a.slots) {
+          if (split > 0) return;
+          splits = 1;
+        }
+      }
     }
 
     if constexpr (TREE) {
@@ -675,8 +697,12 @@ __global__ __launch_bounds__(256) void shaped_merge_kernel(RowsArgs a) {
   const int rows = sq.q_len * a.group;
   if (qb * kRows + r0 >= rows) return;
   int parts = a.splits;
-  int64_t row_first = int64_t(item) * a.splits * kRows, row_next = row_first, step = kRows;
-  if constexpr (TREE) {
+  int64_t row_first = 0, row_next = 0, step = kRows;
+  if constexpr (!TREE) {
+    const int slot = part_slot(a, b, qb, kvh);
+    if (slot >= a.slots) return;  // not cut
+    row_first = row_next = int64_t(slot) * a.splits * kRows;
+  } else {
     const uint32_t f0 = uint32_t(a.first_tile[b]), nt = uint32_t(a.first_tile[b + 1]) - f0;
     parts = 0;
     if (nt > 0) {
