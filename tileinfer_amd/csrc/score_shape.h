@@ -24,8 +24,10 @@ __device__ __forceinline__ float capped(float dot, const ScoreShape& s) {
   return fmaf(-2.f * s.cap_log2, r, s.cap_log2);
 }
 
-// Caps beyond this (an error of 2.6e-5, a twentieth of half an fp16 step of a weight) take the form below, which costs
-// ten more instructions a score: a call with a cap of 1e4 would have scores of any size off by 1e-3.
+// Caps beyond this (an error of 2.6e-5, a twentieth of half an fp16 step of a weight) take the form below: a call with a
+// cap of 1e4 would have scores of any size off by 1e-3. It costs ten more instructions a score (2,048 queries in a window
+// of 4,096 with 24/4 heads of 256 and a cap of 1,000 318 us against 260 by the difference; a step of 32 x 16,384 tokens
+// the same).
 constexpr float kCloseCap = 256.f;
 
 // |y| < 1/2: y (945 + 105 y^2 + y^4) / (945 + 420 y^2 + 15 y^4), from the continued fraction of tanh, off by less than
