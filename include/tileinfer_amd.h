@@ -575,7 +575,7 @@ int ti_evict_kvcache(void* k_cache, void* v_cache, const float* mass, int64_t ma
  *   q, k, v, q_out   rows of head_dim (128 or 256), 16-byte aligned, strides multiples of 8 elements
  *   positions        [num_axes (1 .. 4), n_tokens] of position_bits (32 or 64) bits, token stride 1
  *   inv_freq, axis_of  [rotary_dim / 2]; axis_of NULL: axis 0, entries outside are clamped to the axes there are
- *   rotary_dim       a multiple of 16 up to min(head_dim, 128); 0: no rotation
+ *   rotary_dim       a multiple of 16 up to head_dim; 0: no rotation
  *   caches           rows of num_kv_heads * head_dim at cache_row_stride
  * At most 2^26 rows (n_tokens times heads of q, k and v). No reference counterpart (its positions have one axis).
  */

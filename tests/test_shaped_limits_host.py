@@ -24,3 +24,16 @@ def test_shaped_workspace_is_that_of_the_units_there_are():
                                               (7, 343, 300, 8, 2, 128), (1, 300, 300, 24, 4, 256), (60, 60, 1, 24, 4, 256)):
         assert lib.ti_gqa_prefill_shaped_workspace_bytes(batch, total, longest, hq, hkv, d, 1 << 17, ctypes.byref(n)) == 0
         assert n.value <= 512 * 128 * (128 + 2) * 4, (batch, total, longest, n.value)
+
+
+def test_rope_turns_whole_heads():
+    """Heads of 256 may be turned whole, as qknorm_rope_append turns them; no head past its end."""
+    p, lib = _addr(), _lib.load()
+    good = [p, 512, 256, p, 512, 256, p, 512, 256, p, 8, 32, p, p, p, p, 1.0, p, 512, 256, p, p, 512, 20, p, 0, 3, 2, 2, 256,
+            256, 1e-6, 0, None]  # no tokens: checked, not launched
+    for head_dim, rotary in ((256, 256), (256, 240), (256, 144), (256, 0), (128, 128)):
+        good[29], good[30] = head_dim, rotary
+        assert lib.ti_rope_axes_append(*good) == _lib.TI_OK, (head_dim, rotary, lib.ti_last_error())
+    _refused("ti_rope_axes_append", good, [(30, 144), (30, 256), (30, 136)], _lib.TI_EUNSUPPORTED)
+    good[29] = 256
+    _refused("ti_rope_axes_append", good, [(30, 272), (30, 200)], _lib.TI_EUNSUPPORTED)

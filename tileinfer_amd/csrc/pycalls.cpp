@@ -666,7 +666,7 @@ PyObject* rope_axes_append(PyObject* const* a) {
   const bool wide = pos->scalar_type() == at::kLong;
   const int64_t axes = pos->dim() == 2 ? pos->size(0) : 1;
   if (code < 0 || n <= 0 || hq <= 0 || hkv <= 0 || (d != 128 && d != 256) || k.sizes() != v.sizes() || k.size(0) != n ||
-      k.size(2) != d || half < 0 || half % 8 != 0 || 2 * half > 128 || inv->scalar_type() != at::kFloat ||
+      k.size(2) != d || half < 0 || half % 8 != 0 || 2 * half > d || inv->scalar_type() != at::kFloat ||
       !inv->is_contiguous() || (!wide && pos->scalar_type() != at::kInt) || pos->dim() < 1 || pos->dim() > 2 ||
       pos->size(-1) != n || pos->stride(-1) != 1 || axes < 1 || axes > 4 || !int32_vector(*slots, n, dev) ||
       kc->dim() != 2 || vc->sizes() != kc->sizes() || vc->strides() != kc->strides() || kc->size(1) != hkv * d ||

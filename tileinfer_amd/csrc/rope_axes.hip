@@ -9,11 +9,11 @@
 //
 // A row is D / 8 lanes of 16 bytes, so that a wave takes 2 (D = 256) or 4 (D = 128) rows at a time; a wave takes P such
 // passes over the rows of one token (its q, k and v heads), all loaded at once. Lane i computes the angle of frequency
-// i once a wave, the lanes of a row read theirs back from LDS: a sine for every value instead would cost more time
-// than the row's bytes. Bound: HBM and the vector work of the norms for long chunks (8,191 tokens with 24/4 heads of 256
-// and norms 56.6 us, 4.7 TB/s; without norms 51, 5.3 TB/s), the launch for short ones (48 tokens 7.2 us). The norms' sums by
-// DPP and partners exchanged as 16-bit pairs, where both had been shuffles of 32-bit values: 57.8 to 56.6 us, 46.6 to 44.7
-// for 32/8 heads of 128. Loads with the nt bit made no difference.
+// i (and of i + 64) once a wave, the lanes of a row read theirs back from LDS: a sine for every value instead would cost
+// more time than the row's bytes. Bound: HBM and the vector work of the norms for long chunks (8,191 tokens with 24/4 heads
+// of 256 and norms 56.6 us, 4.7 TB/s; without norms 51, 5.3 TB/s), the launch for short ones (48 tokens 7.2 us). The norms'
+// sums by DPP and partners exchanged as 16-bit pairs, where both had been shuffles of 32-bit values: 57.8 to 56.6 us, 46.6 to
+// 44.7 for 32/8 heads of 128. Loads with the nt bit made no difference.
 #include <type_traits>
 
 #include "decode_common.h"
@@ -68,7 +68,8 @@ template <int D, int P, typename Tag>
 __global__ __launch_bounds__(256) void rope_axes_kernel(RopeAxesArgs a) {
   constexpr int LPR = D / 8;
   constexpr int RPW = 64 / LPR;
-  __shared__ __align__(16) float s_cs[4][2][64];
+  constexpr int MAX_HALF = D / 2;  // frequencies
+  __shared__ __align__(16) float s_cs[4][2][MAX_HALF];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t item = blockIdx.x * 4u + uint32_t(wave);
@@ -105,16 +106,17 @@ __global__ __launch_bounds__(256) void rope_axes_kernel(RopeAxesArgs a) {
   const int64_t slot = a.slots[t];
   const bool stored = slot >= 0 && slot < a.num_slots;
 
-  if (lane < half) {
-    const int axis = a.axis_of ? min(max(a.axis_of[lane], 0), a.axes - 1) : 0;
+#pragma unroll 1
+  for (int f = lane; f < half; f += 64) {  // once; twice for more than 128 turned values
+    const int axis = a.axis_of ? min(max(a.axis_of[f], 0), a.axes - 1) : 0;
     const int64_t at = axis * a.pos_sa + t;
     const double pos = a.wide ? double(static_cast<const int64_t*>(a.positions)[at])
                               : double(static_cast<const int32_t*>(a.positions)[at]);
-    const double turns = pos * (double(a.inv_freq[lane]) * 0.15915494309189533577);  // 1 / (2 pi)
+    const double turns = pos * (double(a.inv_freq[f]) * 0.15915494309189533577);  // 1 / (2 pi)
     float s, c;
     sincospif(2.f * float(turns - rint(turns)), &s, &c);
-    s_cs[wave][0][lane] = c;
-    s_cs[wave][1][lane] = s;
+    s_cs[wave][0][f] = c;
+    s_cs[wave][1][f] = s;
   }
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
@@ -223,8 +225,8 @@ extern "C" int ti_rope_axes_append(const void* q, int64_t q_stride_t, int64_t q_
   if (head_dim != 128 && head_dim != 256) {
     return fail(TI_EUNSUPPORTED, "%s: head_dim %d not built (128, 256)", who, head_dim);
   }
-  if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim > 128 || rotary_dim % 16 != 0) {
-    return fail(TI_EUNSUPPORTED, "%s: rotary_dim %d is not a multiple of 16 up to min(head_dim, 128)", who, rotary_dim);
+  if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 16 != 0) {
+    return fail(TI_EUNSUPPORTED, "%s: rotary_dim %d is not a multiple of 16 up to head_dim", who, rotary_dim);
   }
   if (position_bits != 32 && position_bits != 64) {
     return fail(TI_EUNSUPPORTED, "%s: positions of %d bits (32, 64)", who, position_bits);

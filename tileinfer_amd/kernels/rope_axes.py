@@ -60,7 +60,7 @@ def rope_axes_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, position
         q: ``[T, H_q, D]``, k, v ``[T, H_kv, D]``, D 128 or 256, any strides (for instance slices of one
             projection)
         positions: ``[A, T]`` (A 1 to 4) or ``[T]``, int32 or int64
-        inv_freq: ``[rotary_dim / 2]`` float32; rotary_dim a multiple of 16, at most 128 and D. Frequency ``i``
+        inv_freq: ``[rotary_dim / 2]`` float32; rotary_dim a multiple of 16, at most D. Frequency ``i``
             turns the pair ``(i, i + rotary_dim / 2)`` of every query and key head
         axes: ``[rotary_dim / 2]`` int32, the axis of every frequency (``rope_axes``; entries outside ``0 .. A - 1``
             are clamped); None: axis 0
@@ -97,8 +97,8 @@ def rope_axes_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, position
     if inv_freq.dim() != 1 or inv_freq.dtype != torch.float32:
         raise ValueError(f"inv_freq must be [rotary_dim / 2] float32, got {tuple(inv_freq.shape)} {inv_freq.dtype}")
     half = inv_freq.shape[0]
-    if half % 8 or 2 * half > min(d, 128):
-        raise ValueError(f"rotary_dim {2 * half} must be a multiple of 16 and at most {min(d, 128)}")
+    if half % 8 or 2 * half > d:
+        raise ValueError(f"rotary_dim {2 * half} must be a multiple of 16 and at most {d}")
     if positions.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
     if positions.dim() == 1:
