@@ -11,9 +11,9 @@
 // passes over the rows of one token (its q, k and v heads), all loaded at once. Lane i computes the angle of frequency
 // i (and of i + 64) once a wave, the lanes of a row read theirs back from LDS: a sine for every value instead would cost
 // more time than the row's bytes. Bound: HBM and the vector work of the norms for long chunks (8,191 tokens with 24/4 heads
-// of 256 and norms 56.6 us, 4.7 TB/s; without norms 51, 5.3 TB/s), the launch for short ones (48 tokens 7.2 us). The norms'
-// sums by DPP and partners exchanged as 16-bit pairs, where both had been shuffles of 32-bit values: 57.8 to 56.6 us, 46.6 to
-// 44.7 for 32/8 heads of 128. Loads with the nt bit made no difference.
+// of 256 and norms 56 to 59 us, 4.6 to 4.8 TB/s; without norms 50, 5.3 TB/s), the launch for short ones (48 tokens 7 to
+// 8 us). The norms' sums by DPP and partners exchanged as 16-bit pairs, where both had been shuffles of 32-bit values: 58.5
+// to 57.1 us in turn, 47.5 to 45.1 for 32/8 heads of 128. Loads with the nt bit made no difference.
 #include <type_traits>
 
 #include "decode_common.h"
@@ -197,7 +197,8 @@ void launch_rope_axes(RopeAxesArgs a, hipStream_t s) {
 }
 
 // Passes of a wave: four where the rows fill the GPU several times over (the angles once for four passes, four loads
-// in flight), one where they do not and each pass would wait for the one before.
+// in flight), one where they do not and each pass would wait for the one before. With 24/4 heads of 256, one against four:
+// 8,191 tokens 87 us against 56, 1,024 (where the rule changes) 13.1 against 11.4, up to 512 8.1 to 8.6 either way.
 template <int D, typename Tag>
 void launch_rope_axes_dim(const RopeAxesArgs& a, hipStream_t s) {
   const int64_t passes = int64_t(a.tokens) * ceil_div(a.hq + 2 * int64_t(a.hkv), 64 / (D / 8));

@@ -13,12 +13,13 @@
 // beside the output of tile t it caps the scores of tile t + 1. One barrier a tile; K is two tiles ahead, V one.
 //
 // Bound, at D = 256: LDS (each wave reads all of K and V for its 16 rows: 512 KB a tile at some 215 bytes a cycle, and the
-// loads write 64 KB) and the loads' way through the CU's address unit (1,400 cycles of a loading wave's 4,600 a tile), the
-// matrix unit being busy 44 % of the time: 2,048 queries over 10,240 keys within a window of 4,096 with 24/4 heads 238 us
-// (866 TFLOP/s), capped 255 to 270; a first chunk of 2,048 82, capped 85 to 93. Waves of 32 rows (half the reads) do not fit
-// 256 registers with the softmax beside the products; with 512 (four waves a CU) the compiler moved them between register
-// files (379 us against 274 then), without the overlap 279. At D = 128: the vector unit (capped 176 us, 146 without, 940
-// TFLOP/s for the same chunk with 32/8 heads) and unit starts: 12 chunks of packed documents with 32/8 heads 78 to 84 us.
+// loads write 64 KB) and the loads' way through the CU's address unit (1,250 to 1,350 cycles of a loading wave's 4,600 a
+// tile, capped 5,100), the matrix unit being busy 38 % of the time, capped 35 %: 2,048 queries over 10,240 keys within a
+// window of 4,096 with 24/4 heads 244 us (845 TFLOP/s), capped 254 to 281; a first chunk of 2,048 82, capped 81 to 92.
+// Waves of 32 rows (half the reads) do not fit 256 registers with the softmax beside the products; with 512 (four waves a
+// CU) the compiler moved them between register files (379 us against 274 then), without the overlap 279. At D = 128: the
+// vector unit (capped 180 us, 150 without, 918 TFLOP/s for the same chunk with 32/8 heads) and unit starts: 12 chunks of
+// packed documents with 32/8 heads 76 to 84 us.
 #pragma once
 
 #include "lds_tiles.h"
@@ -118,7 +119,8 @@ __device__ __forceinline__ int tree_tiles(const RowsArgs& a, int b) {
   const Queries<true> s(a, b);
   return (s.kv_len + kKeys - 1) / kKeys - tree_tile0(a, s);
 }
-constexpr uint32_t kMinRun = 2;  // tiles
+// Tiles of a run at least: 32 drafts over 700 tokens with 24/4 heads of 256 30.6 us, with runs of one 32.3; long lists alike.
+constexpr uint32_t kMinRun = 2;
 __device__ __forceinline__ Runs tree_runs(const RowsArgs& a, uint32_t total) {
   return Runs(uint32_t(a.runs), total, kMinRun);
 }

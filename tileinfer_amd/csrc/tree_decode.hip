@@ -17,9 +17,10 @@
 // by side, since the heads' rows of a token lie side by side in memory. A sequence that lies in one run is written by it,
 // others leave (m, l, o) parts in 32 bits that a second kernel joins in the order of the runs.
 //
-// Bound: HBM for long batches (a step of 32 x 16,384 tokens with 32/8 heads of 128, capped, 333 us, 6.4 TB/s; with 24/4
-// heads of 256 319 us, 6.7 TB/s), the start of a run and the join's launch for short ones (16 sequences of 512 to 8,192
-// tokens with one token of 24/4 heads 57 us, with eight 79; one of 700 tokens with eight 16).
+// Bound: HBM for long batches (a step of 32 x 16,384 tokens with 32/8 heads of 128, capped, 331 to 342 us, 6.3 to 6.5 TB/s;
+// with 24/4 heads of 256 320 us, 6.7 TB/s), the start of a run and the join's launch for short ones (16 sequences of 512 to
+// 8,192 tokens with one token of 24/4 heads 57 us, with eight 77 to 79, where the scores, statistics and products of four
+// row groups follow one another in a tile; one of 700 tokens with eight 16).
 //
 // Trees of more than 64 rows a KV head go to the kernel of shaped_rows.h (kFewRows).
 #include <type_traits>
@@ -68,7 +69,10 @@ __device__ __forceinline__ int tile_count(const TreeArgs& a, int len, int tile) 
 }
 
 // Calls of at least this many 32 KiB tiles load their rows with the streaming policy; shorter ones, which the last-level
-// cache may still hold, keep the default one.
+// cache may still hold, keep the default one. Streamed against not, 32 sequences with 32/8 heads of 128: of 16,384 tokens
+// 331 us against 379, of 2,400 (9,600 tiles) 58 against 65, of 600 (where the rule changes) 21.9 against 22.6; below it the
+// look for shared blocks costs more than it gains (8 sequences of 2,000 tokens with eight drafts of 24/4 heads of 256 37.5
+// against 34.3, 128 of 150 tokens 40.7 against 38.9).
 constexpr int64_t kStreamTiles = 2400;
 
 __device__ __forceinline__ Runs runs_of(const TreeArgs& a, uint32_t total) { return Runs(uint32_t(a.runs), total, 1u); }
