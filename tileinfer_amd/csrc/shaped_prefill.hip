@@ -22,9 +22,9 @@ struct ShapedSizes {
 // How units are cut. A CU holds one workgroup at D = 256, two at 128 (slots). Where the units do not fill the slots, all
 // are cut into as many parts as fill them; where they fill them some times over and the units of a chunk are alike
 // (one sequence, at least as much context as chunk), those of the last, partial round are. Parts have at least four
-// tiles, and only units that exist have them: at most as many as fill the slots, 34 MB. Cut against whole, 24/4 heads of 256,
-// capped: 64 queries over 8,256 keys 45 us against 277; 2,048 over 10,240, whose last round is cut, 553 against 641, in a
-// window of 4,096 276 against 317; but the last round of a first chunk of 2,048, its shortest units, 99 against 86.
+// tiles, and only units that exist have them: at most as many as fill the slots, 34 MB. Cut against whole, 24/4 heads of
+// 256, capped: 64 queries over 8,256 keys 45 us against 277; 2,048 over 10,240, whose last round is cut, 553 against 641,
+// in a window of 4,096 276 against 317; but the last round of a first chunk of 2,048, its shortest units, 99 against 86.
 ShapedSizes shaped_sizes(int32_t batch, int32_t total_q, int32_t max_q, int32_t hq, int32_t hkv, int32_t head_dim,
                          int64_t max_k) {
   ShapedSizes z{};

@@ -119,7 +119,8 @@ __device__ __forceinline__ int tree_tiles(const RowsArgs& a, int b) {
   const Queries<true> s(a, b);
   return (s.kv_len + kKeys - 1) / kKeys - tree_tile0(a, s);
 }
-// Tiles of a run at least: 32 drafts over 700 tokens with 24/4 heads of 256 30.6 us, with runs of one 32.3; long lists alike.
+// Tiles of a run at least: 32 drafts over 700 tokens with 24/4 heads of 256 30.6 us, with runs of one tile 32.3; long lists
+// take the same either way.
 constexpr uint32_t kMinRun = 2;
 __device__ __forceinline__ Runs tree_runs(const RowsArgs& a, uint32_t total) {
   return Runs(uint32_t(a.runs), total, kMinRun);
